@@ -266,6 +266,19 @@ int bt_gla_chunked(const void* proj, long long row_stride, int q_off, int k_off,
                    float log_scale, float* state, const int* slots, const int* seq_start, float* out,
                    long long out_row_stride, float* scratch, int max_new, int n_seqs, int n_heads, int dim, int vdim, int dtype,
                    cudaStream_t stream);
+// A cache held in 4 bits (csrc/cache4.cuh), its attention, and the norm and rotation of what goes there.
+int bt_cache4_append(const void* k, long long k_row, long long k_head, const void* v, long long v_row, long long v_head, void* pool,
+                     long long n_pages, const int* positions, const int* token_seq, const int* ctx_len, const int* table, int n_table,
+                     int table_stride, int table_len, int* status, int n_tokens, int n_kv_heads, int dim, int dtype, cudaStream_t stream);
+int bt_cache4_gather(void* k, long long k_row, long long k_head, void* v, long long v_row, long long v_head, const void* pool,
+                     long long n_pages, const int* positions, const int* token_seq, const int* table, int n_table, int table_stride,
+                     int table_len, int* status, int n_tokens, int n_kv_heads, int dim, int dtype, cudaStream_t stream);
+int bt_cache4_attention(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
+                        int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,
+                        int n_kv_heads, int dim, float scale, int window, int keep_first, int dtype, cudaStream_t stream);
+int bt_qk_norm_rotary(const void* src, long long src_row, void* dst, long long dst_row, const int* positions, const float* freq,
+                      const float* q_weight, const float* k_weight, int n_tokens, int n_heads, int n_kv_heads, int dim, int rot, float eps,
+                      float size, int interleaved, int dtype, cudaStream_t stream);
 int bt_add_vector(float* x, const float* vec, long long n_rows, int width, cudaStream_t stream);
 int bt_add_rows(float* x, const float* a, const float* b, const float* c, long long n, cudaStream_t stream);
 

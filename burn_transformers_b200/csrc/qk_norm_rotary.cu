@@ -1,0 +1,240 @@
+// Norms of a step's query and key heads and their rotation by position, in one pass over the projections.
+//
+// Per token and head: y = x / sqrt(mean(x^2) + eps) * weight (one weight for all query heads, one for all key heads; without
+// weights x as it is), then pairs of the first `rot` channels, (i, i + rot / 2) or (2i, 2i + 1), turned by pos * f_i with cosine and
+// sine times `size`.  Sums and products are 32-bit, rounded once.  Angles: pos * f_i is formed in 64 bits and taken into one turn
+// there, so that far positions lose nothing (a 32-bit product is off by pos * f / 2^24: 0.06 at position 10^6).
+//
+// Bound by memory: every channel is read and written once.  A warp takes one token and some of its heads.  Its lanes form the token's cosines
+// and sines once, in shared memory, and keep the eight pairs that a lane turns in registers; a lane holds 16 channels of a head (the
+// two pieces of 8 that turn into one another, or 16 in a row), so that nothing but the norm's sum goes between lanes.  How many heads
+// a warp takes: all of them when there are enough tokens to fill the GPU, as few as fit its lanes when there are not.
+#include "common.cuh"
+
+namespace bt {
+
+constexpr int QN_WARPS = 8;
+
+struct QnParams {
+  const void* src;
+  void* dst;
+  long long src_row, dst_row;          // elements between tokens
+  const int* positions;
+  const float* freq;                   // [rot / 2]
+  const float *q_weight, *k_weight;    // [dim] or null
+  int n_tokens, n_heads, n_vecs;       // n_vecs: query heads and key heads, side by side
+  int dim, rot;
+  int vecs_per_warp, warps_per_token;
+  float eps, size;
+  int interleaved, normed;
+};
+
+__device__ __forceinline__ float2 qn_turn(int pos, float f, float size) {
+  double t = (double)pos * (double)f * 0.31830988618379067154;      // half turns
+  t -= 2.0 * rint(0.5 * t);
+  float s, c;
+  sincospif((float)t, &s, &c);
+  return make_float2(c * size, s * size);
+}
+
+template <typename T>
+__device__ __forceinline__ void qn_load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    unpack16(*reinterpret_cast<const uint4*>(p), x);
+  } else {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void qn_store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+// LANES: lanes a head (a power of two, 16 channels each; those past the head's channels idle).
+template <typename T, int LANES>
+__global__ void __launch_bounds__(QN_WARPS * 32)
+qk_norm_rotary_kernel(QnParams p) {
+  __shared__ float2 s_turn[QN_WARPS][128];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long job = (long long)blockIdx.x * QN_WARPS + warp;
+  const int token = (int)(job / p.warps_per_token), part = (int)(job % p.warps_per_token);
+  if (token >= p.n_tokens) return;
+  const int pos = p.positions[token];
+  float2* turn = s_turn[warp];
+  for (int i = lane; i < p.rot / 2; i += 32) turn[i] = qn_turn(pos, p.freq[i], p.size);
+  __syncwarp();
+  // this lane's two pieces of 8 channels: pieces that turn into one another, or (past the turned ones, and for neighbours) in a row
+  const int c = lane % LANES, sub = lane / LANES, pairs = p.interleaved ? 0 : p.rot / 16;
+  const bool mine = 16 * c < p.dim, turned = 16 * c < p.rot;
+  const int a = c < pairs ? 8 * c : 16 * c, b = c < pairs ? 8 * (c + pairs) : 16 * c + 8;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 w = turned ? turn[8 * c + i] : make_float2(1.f, 0.f);
+    cs[i] = w.x;
+    sn[i] = w.y;
+  }
+  const int first = part * p.vecs_per_warp, last = min(p.n_vecs, first + p.vecs_per_warp);
+  const T* src = reinterpret_cast<const T*>(p.src) + token * p.src_row;
+  T* dst = reinterpret_cast<T*>(p.dst) + token * p.dst_row;
+  float wa[8], wb[8];
+  const float* held = nullptr;
+  for (int v0 = first; v0 < last; v0 += 32 / LANES) {
+    const int v = v0 + sub;
+    const bool here = mine && v < last;
+    float x[8], y[8];
+    if (here) {
+      qn_load8<T>(src + (long long)v * p.dim + a, x);
+      qn_load8<T>(src + (long long)v * p.dim + b, y);
+    }
+    if (p.normed) {
+      float sum = 0.f;
+      if (here) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float r = rsqrtf(sum / (float)p.dim + p.eps);
+      const float* weight = v < p.n_heads ? p.q_weight : p.k_weight;
+      if (here && weight != held) {
+        qn_load8<float>(weight + a, wa);
+        qn_load8<float>(weight + b, wb);
+        held = weight;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= r * wa[i];
+        y[i] *= r * wb[i];
+      }
+    }
+    if (!here) continue;
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = x[2 * i], w = x[2 * i + 1], g = y[2 * i], h = y[2 * i + 1];
+        x[2 * i] = u * cs[i] - w * sn[i];
+        x[2 * i + 1] = w * cs[i] + u * sn[i];
+        y[2 * i] = g * cs[4 + i] - h * sn[4 + i];
+        y[2 * i + 1] = h * cs[4 + i] + g * sn[4 + i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = x[i], w = y[i];
+        x[i] = u * cs[i] - w * sn[i];
+        y[i] = w * cs[i] + u * sn[i];
+      }
+    }
+    qn_store8<T>(dst + (long long)v * p.dim + a, x);
+    qn_store8<T>(dst + (long long)v * p.dim + b, y);
+  }
+}
+
+// Any head size up to 256, any even `rot`, any alignment: a warp a (token, head), a lane a pair or a channel at a time.
+template <typename T>
+__global__ void __launch_bounds__(QN_WARPS * 32)
+qk_norm_rotary_any_kernel(QnParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long job = (long long)blockIdx.x * QN_WARPS + (threadIdx.x >> 5);
+  const int token = (int)(job / p.n_vecs), v = (int)(job % p.n_vecs);
+  if (token >= p.n_tokens) return;
+  const int pos = p.positions[token], half = p.rot / 2, slots = half + p.dim - p.rot;
+  const T* src = reinterpret_cast<const T*>(p.src) + token * p.src_row + (long long)v * p.dim;
+  T* dst = reinterpret_cast<T*>(p.dst) + token * p.dst_row + (long long)v * p.dim;
+  const float* weight = v < p.n_heads ? p.q_weight : p.k_weight;
+  float x[8], y[8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = lane + 32 * i;
+    x[i] = y[i] = 0.f;
+    if (s < half) {
+      x[i] = to_float(src[p.interleaved ? 2 * s : s]);
+      y[i] = to_float(src[p.interleaved ? 2 * s + 1 : s + half]);
+    } else if (s < slots) {
+      x[i] = to_float(src[half + s]);
+    }
+    sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
+  }
+  const float r = p.normed ? rsqrtf(warp_sum(sum) / (float)p.dim + p.eps) : 1.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = lane + 32 * i;
+    if (s < half) {
+      const int a = p.interleaved ? 2 * s : s, b = p.interleaved ? 2 * s + 1 : s + half;
+      const float2 w = qn_turn(pos, p.freq[s], p.size);
+      const float u = p.normed ? x[i] * (r * weight[a]) : x[i], z = p.normed ? y[i] * (r * weight[b]) : y[i];
+      dst[a] = from_float<T>(u * w.x - z * w.y);
+      dst[b] = from_float<T>(z * w.x + u * w.y);
+    } else if (s < slots) {
+      dst[half + s] = from_float<T>(p.normed ? x[i] * (r * weight[half + s]) : x[i]);
+    }
+  }
+}
+
+template <typename T>
+static int launch_qn(QnParams p, bool whole, cudaStream_t stream) {
+  if (whole) {
+    const int lanes = p.dim <= 16 ? 1 : p.dim <= 32 ? 2 : p.dim <= 64 ? 4 : p.dim <= 128 ? 8 : 16;
+    const int side = 32 / lanes, rounds = (p.n_vecs + side - 1) / side;
+    // rounds a warp: all of them once the tokens alone give every multiprocessor 64 warps
+    const long long wanted = 64ll * (sm_count() > 0 ? sm_count() : 148);
+    long long split = (wanted + p.n_tokens - 1) / p.n_tokens;
+    if (split > rounds) split = rounds;
+    const int per = (int)((rounds + split - 1) / split);
+    p.vecs_per_warp = per * side;
+    p.warps_per_token = (rounds + per - 1) / per;
+    const long long blocks = ((long long)p.n_tokens * p.warps_per_token + QN_WARPS - 1) / QN_WARPS;
+    BT_CHECK(blocks < (1ll << 31), "qk_norm_rotary: %d tokens of %d heads are too many for one launch", p.n_tokens, p.n_vecs);
+    const dim3 grid((unsigned)blocks), block(QN_WARPS * 32);
+    switch (lanes) {
+      case 1: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 1>, grid, block, 0, stream, 1, p)); break;
+      case 2: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 2>, grid, block, 0, stream, 1, p)); break;
+      case 4: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 4>, grid, block, 0, stream, 1, p)); break;
+      case 8: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 8>, grid, block, 0, stream, 1, p)); break;
+      default: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 16>, grid, block, 0, stream, 1, p));
+    }
+    return 0;
+  }
+  const long long blocks = ((long long)p.n_tokens * p.n_vecs + QN_WARPS - 1) / QN_WARPS;
+  BT_CHECK(blocks < (1ll << 31), "qk_norm_rotary: %d tokens of %d heads are too many for one launch", p.n_tokens, p.n_vecs);
+  BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_any_kernel<T>, dim3((unsigned)blocks), dim3(QN_WARPS * 32), 0, stream, 1, p));
+  return 0;
+}
+
+}  // namespace bt
+
+// src, dst (which may be the same): rows of n_heads query heads and n_kv_heads key heads of `dim` channels.  dtype: 0 32-bit, 1 bfloat16.
+extern "C" int bt_qk_norm_rotary(const void* src, long long src_row, void* dst, long long dst_row, const int* positions, const float* freq,
+                                 const float* q_weight, const float* k_weight, int n_tokens, int n_heads, int n_kv_heads, int dim, int rot,
+                                 float eps, float size, int interleaved, int dtype, cudaStream_t stream) {
+  using namespace bt;
+  BT_CHECK(dim > 0 && dim <= 256 && rot >= 0 && rot <= dim && rot % 2 == 0, "qk_norm_rotary: %d turned channels of %d", rot, dim);
+  BT_CHECK(n_tokens >= 0 && n_heads >= 0 && n_kv_heads >= 0 && n_heads + n_kv_heads > 0, "qk_norm_rotary: bad sizes tokens=%d heads=%d key heads=%d",
+           n_tokens, n_heads, n_kv_heads);
+  BT_CHECK((q_weight == nullptr) == (k_weight == nullptr), "qk_norm_rotary: give both weights or neither");
+  BT_CHECK(dtype == kF32 || dtype == kBF16, "qk_norm_rotary: unknown element type %d", dtype);
+  if (n_tokens == 0) return 0;
+  QnParams p{src, dst, src_row, dst_row, positions, freq, q_weight, k_weight, n_tokens, n_heads, n_heads + n_kv_heads, dim, rot, 0, 0, eps,
+             size, interleaved, q_weight != nullptr};
+  const int step = dtype == kF32 ? 4 : 8;
+  auto at16 = [](const void* x) { return (unsigned long long)x % 16 == 0; };
+  const bool whole = dim % 16 == 0 && rot % 16 == 0 && src_row % step == 0 && dst_row % step == 0 && at16(src) && at16(dst) && at16(q_weight) &&
+                     at16(k_weight);
+  if (dtype == kF32) return launch_qn<float>(p, whole, stream);
+  return launch_qn<__nv_bfloat16>(p, whole, stream);
+}

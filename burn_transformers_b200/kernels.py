@@ -596,7 +596,9 @@ _STATUS_TEXT = {1: "decode attention gave up waiting for a copy of cache pages",
                 6: "the tcgen05 prefill attention gave up waiting for a stage of its pipeline (or found its shared memory "
                    "misaligned)",
                 7: "the tcgen05 matrix product for few rows gave up waiting for a stage of its pipeline",
-                8: "the experts' tcgen05 product gave up waiting for a stage of its pipeline"}
+                8: "the experts' tcgen05 product gave up waiting for a stage of its pipeline",
+                9: "a step of a 4-bit cache named a sequence, position or page outside its table or pool",
+                10: "the attention over a 4-bit cache gave up waiting for a copy or a stage of its pipeline"}
 
 
 def check_status(device) -> None:
@@ -1921,3 +1923,185 @@ def gla_scan(proj, q_off, k_off, v_off, q_scale: float, dt, log_scale: float, st
                                  c_int(g_off), _ptr(mixed), c_longlong(mixed.shape[1] if mixed is not None else 0),
                                  c_int(_code(proj.dtype)), _stream()))
     return weight is not None
+
+
+# ---- queries and keys normed and turned; a cache held in 4 bits -------------------------------
+
+def _rows_view(t, name, width, dtype) -> int:
+    """`t` as rows of at least `width` contiguous elements; returns the elements between rows."""
+    if not t.is_cuda:
+        raise KernelError(f"{name}: lies on {t.device}; the kernels of this library run on a CUDA device only")
+    if t.dtype is not dtype:
+        raise ShapeError(f"{name}: expected dtype {dtype}, found {t.dtype}")
+    if t.dim() != 2 or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ShapeError(f"{name}: expected rows of at least {width} contiguous elements, found shape {list(t.shape)}, strides "
+                         f"{list(t.stride())}")
+    return t.stride(0)
+
+
+def _together(first, *others) -> None:
+    """All on one device, the current one: a launch goes to the current device's stream and reads the others' pointers as its own."""
+    device = first.device
+    if device.index != torch.cuda.current_device():
+        raise KernelError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+    for t in others:
+        if t is not None and t.device != device:
+            raise KernelError(f"tensors on {device} and {t.device} in one call")
+
+
+def _enough(t, name, count) -> None:
+    if t.shape[0] < count:
+        raise ShapeError(f"{name}: {t.shape[0]} entries where the step needs {count}")
+
+
+def qk_norm_rotary(proj, positions, inv_freq, *, n_tokens, n_heads, n_kv_heads, head_dim, rot_dims, q_weight=None, k_weight=None,
+                   eps=0.0, interleaved=False, size=1.0, out=None):
+    """The query and key heads of a step's projections, each normed over its channels and turned by its token's position, in one pass.
+
+    proj: rows [queries | keys | anything], `n_heads` and `n_kv_heads` heads of `head_dim` (at most 256) channels.  With `q_weight`
+    and `k_weight` ([head_dim], 32-bit; both or neither) a head becomes x / sqrt(mean(x^2) + eps) * weight.  Then its first `rot_dims`
+    channels turn by positions * inv_freq ([rot_dims / 2], 32-bit), channel i with i + rot_dims / 2, or 2i with 2i + 1 if
+    `interleaved`, cosine and sine times `size`; the angles are formed in 64-bit.  In place, or into `out`, other rows of at least
+    (n_heads + n_kv_heads) * head_dim elements, which then receive nothing but the queries and keys."""
+    if proj.dtype not in DTYPE_CODE:
+        raise ShapeError(f"qk_norm_rotary: unsupported element type {proj.dtype}")
+    if n_heads < 0 or n_kv_heads < 0 or n_heads + n_kv_heads < 1 or not 1 <= head_dim <= 256:
+        raise ShapeError(f"qk_norm_rotary: {n_heads} query and {n_kv_heads} key heads of {head_dim} channels (1 to 256)")
+    if rot_dims < 0 or rot_dims > head_dim or rot_dims % 2:
+        raise ShapeError(f"qk_norm_rotary: {rot_dims} of {head_dim} channels cannot turn in pairs")
+    if (q_weight is None) != (k_weight is None):
+        raise ShapeError("qk_norm_rotary: give both weights or neither")
+    width = (n_heads + n_kv_heads) * head_dim
+    row = _rows_view(proj, "proj", width, proj.dtype)
+    out_row = row
+    if out is not None:
+        out_row = _rows_view(out, "out", width, proj.dtype)
+        _enough(out, "out", n_tokens)
+    _enough(proj, "proj", n_tokens)
+    _need(positions, "positions", torch.int32, (None,))
+    _enough(positions, "positions", n_tokens)
+    if rot_dims:
+        _need(inv_freq, "inv_freq", torch.float32, (None,))
+        _enough(inv_freq, "inv_freq", rot_dims // 2)
+    if q_weight is not None:
+        _need(q_weight, "q_weight", torch.float32, (head_dim,))
+        _need(k_weight, "k_weight", torch.float32, (head_dim,))
+    _together(proj, positions, out, q_weight, k_weight, inv_freq if rot_dims else None)
+    _work(10.0 * n_tokens * width, 2.0 * n_tokens * width * proj.element_size())
+    _check(library().bt_qk_norm_rotary(
+        _ptr(proj), c_longlong(row), _ptr(proj if out is None else out), c_longlong(out_row), _ptr(positions),
+        _ptr(inv_freq if rot_dims else None), _ptr(q_weight), _ptr(k_weight), c_int(n_tokens), c_int(n_heads), c_int(n_kv_heads),
+        c_int(head_dim), c_int(rot_dims), c_float(eps), c_float(size), c_int(1 if interleaved else 0), c_int(DTYPE_CODE[proj.dtype]),
+        _stream()))
+
+
+def cache4_record_bytes(head_dim: int) -> int:
+    """Bytes of one page of one key head in a 4-bit cache: 64 positions' codes and scales of keys and values (csrc/cache4.cuh)."""
+    if head_dim <= 0 or head_dim > 256 or head_dim % 32:
+        raise ShapeError(f"heads of {head_dim} channels; the 4-bit cache takes multiples of 32 up to 256")
+    return 68 * head_dim
+
+
+def _cache4_pool(pool, n_kv_heads, head_dim, table, table_len, n_seqs) -> None:
+    _need(pool, "pool", torch.uint8, (None, n_kv_heads, cache4_record_bytes(head_dim)))
+    _need(table, "table", torch.int32, (None, None))
+    if not 1 <= table_len <= table.shape[1]:
+        raise ShapeError(f"table: rows of {table.shape[1]} pages hold no list of {table_len}")
+    if table.shape[0] < n_seqs:
+        raise ShapeError(f"table: {table.shape[0]} rows for {n_seqs} sequences")
+
+
+def _cache4_heads(t, name, like=None):
+    """`t` as [tokens, key heads, channels] with contiguous channels: its strides between tokens and heads."""
+    if not t.is_cuda:
+        raise KernelError(f"{name}: lies on {t.device}; the kernels of this library run on a CUDA device only")
+    if t.dtype not in DTYPE_CODE or (like is not None and t.dtype is not like.dtype):
+        raise ShapeError(f"{name}: unsupported element type {t.dtype}" if like is None else f"{name}: expected dtype {like.dtype}, found {t.dtype}")
+    if t.dim() != 3 or t.stride(2) != 1 or (like is not None and t.shape[1:] != like.shape[1:]):
+        raise ShapeError(f"{name}: expected [tokens, key heads, channels] with contiguous channels"
+                         + (f" like {list(like.shape)}" if like is not None else "") + f", found shape {list(t.shape)}, strides {list(t.stride())}")
+    return c_longlong(t.stride(0)), c_longlong(t.stride(1))
+
+
+def cache4_append(k, v, pool, positions, token_seq, ctx_len, table, table_len, *, n_tokens):
+    """Files the new tokens' keys and values in a layer's 4-bit pages.
+
+    k, v: [tokens, key heads, head_dim], views of the step's projections (any strides but the channels'); pool: uint8 [pages, key
+    heads, cache4_record_bytes(head_dim)].  Every 32 channels share a scale of one byte; a value becomes the nearest of the multiples
+    -7 to 7 of it (csrc/cache4.cuh, csrc/cache4.cu).  Where the pages come round (`table_len` pages hold less than a sequence), only the
+    positions they still hold after the step are written; `ctx_len`: the sequences' lengths after the step.  The step's positions
+    must differ from one another within a sequence, and no two sequences of a step may share a page that it writes."""
+    rows = [*_cache4_heads(k, "k"), *_cache4_heads(v, "v", k)]
+    _cache4_pool(pool, k.shape[1], k.shape[2], table, table_len, 0)
+    _enough(k, "k", n_tokens)
+    _enough(v, "v", n_tokens)
+    for t, name in ((positions, "positions"), (token_seq, "token_seq"), (ctx_len, "ctx_len")):
+        _need(t, name, torch.int32, (None,))
+    _enough(positions, "positions", n_tokens)
+    _enough(token_seq, "token_seq", n_tokens)
+    _together(k, v, pool, positions, token_seq, ctx_len, table)
+    elements = 2 * n_tokens * k.shape[1] * k.shape[2]
+    _work(0.0, elements * (k.element_size() + 17 / 32))
+    _check(library().bt_cache4_append(
+        _ptr(k), rows[0], rows[1], _ptr(v), rows[2], rows[3], _ptr(pool), c_longlong(pool.shape[0]), _ptr(positions), _ptr(token_seq),
+        _ptr(ctx_len), _ptr(table), c_int(min(table.shape[0], ctx_len.shape[0])), c_int(table.shape[1]), c_int(table_len),
+        _ptr(kernel_status(k.device)), c_int(n_tokens), c_int(k.shape[1]), c_int(k.shape[2]), c_int(DTYPE_CODE[k.dtype]), _stream()))
+
+
+def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_tokens):
+    """What a layer's 4-bit pages hold for `n_tokens` (sequence, position) pairs, as the values the codes stand for: into the rows
+    k and v, [tokens, key heads, head_dim] (any strides but the channels'), 32-bit or bfloat16, exact in both."""
+    rows = [*_cache4_heads(k, "k"), *_cache4_heads(v, "v", k)]
+    _cache4_pool(pool, k.shape[1], k.shape[2], table, table_len, 0)
+    _enough(k, "k", n_tokens)
+    _enough(v, "v", n_tokens)
+    for t, name in ((positions, "positions"), (token_seq, "token_seq")):
+        _need(t, name, torch.int32, (None,))
+        _enough(t, name, n_tokens)
+    _together(k, v, pool, positions, token_seq, table)
+    elements = 2 * n_tokens * k.shape[1] * k.shape[2]
+    _work(0.0, elements * (k.element_size() + 17 / 32))
+    _check(library().bt_cache4_gather(
+        _ptr(k), rows[0], rows[1], _ptr(v), rows[2], rows[3], _ptr(pool), c_longlong(pool.shape[0]), _ptr(positions), _ptr(token_seq),
+        _ptr(table), c_int(table.shape[0]), c_int(table.shape[1]), c_int(table_len), _ptr(kernel_status(k.device)), c_int(n_tokens),
+        c_int(k.shape[1]), c_int(k.shape[2]), c_int(DTYPE_CODE[k.dtype]), _stream()))
+
+
+def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window=0, keep_first=0) -> int:
+    """32-bit words of `scratch` that cache4_attention wants for a step of these sizes."""
+    return 0
+
+
+def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads,
+                     head_dim, scale, window=0, keep_first=0, scratch=None):
+    """Causal attention of a step's queries over a layer's 4-bit pages, which hold the step's own keys and values too.
+
+    q: rows whose first n_heads * head_dim elements are the query heads (bfloat16 or 32-bit); out: [tokens, n_heads * head_dim] of
+    the same type.  Sequence s brings the tokens seq_start[s] .. seq_start[s + 1] behind past_len[s] others, at most `max_new` of
+    them, and is no longer than `max_ctx` after the step.  A query at position p sees the keys j <= p with j > p - window (`window`
+    0: all) or j < keep_first.  Rows of `out` behind the last sequence stay as they are.  Where the pages come round, what a query
+    sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0."""
+    if q.dtype not in DTYPE_CODE:
+        raise ShapeError(f"cache4_attention: unsupported element type {q.dtype}")
+    if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
+        raise ShapeError(f"cache4_attention: {n_heads} query heads cannot share {n_kv_heads} key heads")
+    if window < 0 or keep_first < 0 or max_new < 0 or n_seqs < 0:
+        raise ShapeError(f"cache4_attention: window {window}, kept positions {keep_first}, {max_new} new tokens of {n_seqs} sequences")
+    width = n_heads * head_dim
+    row = _rows_view(q, "q", width, q.dtype)
+    _need(out, "out", q.dtype, (None, width))
+    _enough(q, "q", n_tokens)
+    _enough(out, "out", n_tokens)
+    _cache4_pool(pool, n_kv_heads, head_dim, table, table_len, n_seqs)
+    _need(seq_start, "seq_start", torch.int32, (None,))
+    _need(past_len, "past_len", torch.int32, (None,))
+    _enough(seq_start, "seq_start", n_seqs + 1)
+    _enough(past_len, "past_len", n_seqs)
+    if max_ctx > table_len * PAGE_SIZE and (keep_first or not window or table_len * PAGE_SIZE < window + max_new - 1):
+        raise ShapeError(f"cache4_attention: {table_len} pages that come round do not hold what queries of a context of {max_ctx} see "
+                         f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
+    _together(q, out, pool, table, seq_start, past_len)
+    _check(library().bt_cache4_attention(
+        _ptr(q), c_longlong(row), _ptr(out), _ptr(pool), c_longlong(pool.shape[0]), _ptr(table), c_int(table.shape[1]), c_int(table_len),
+        _ptr(kernel_status(q.device)), _ptr(seq_start), _ptr(past_len), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads),
+        c_int(head_dim), c_float(scale), c_int(window), c_int(keep_first), c_int(DTYPE_CODE[q.dtype]), _stream()))

@@ -1,0 +1,194 @@
+"""The 4-bit cache on the device: what it holds after a step, bit for bit, and the attention over it, against the definitions in
+64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import plain_cache4 as plain
+from burn_transformers_b200 import kernels
+from burn_transformers_b200.errors import KernelError
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+PAGE = 64
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=DEV)
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+class Step:
+    """The integers of a step; pages handed out in a scrambled order, two pages of the pool in nobody's list."""
+
+    def __init__(self, pasts, news, ring=None, seed=7):
+        self.pasts, self.news, self.lens = pasts, news, [p + n for p, n in zip(pasts, news)]
+        self.width = ring or max(1, -(-max(self.lens) // PAGE))
+        self.pages = len(news) * self.width + 2
+        order = np.random.default_rng(seed).permutation(self.pages)
+        self.lists = order[:len(news) * self.width].reshape(len(news), self.width)
+        self.n, self.n_seqs = sum(news), len(news)
+        self.starts = np.concatenate([[0], np.cumsum(news)])
+        self.seq_start, self.past, self.ctx, self.table = ints(self.starts), ints(pasts), ints(self.lens), ints(self.lists)
+        self.positions = ints(np.concatenate([np.arange(p, p + n) for p, n in zip(pasts, news)]))
+        self.token_seq = ints(np.concatenate([np.full(n, s) for s, n in enumerate(news)]))
+
+    def sizes(self, heads, kv, dim, window=0, keep=0):
+        return dict(n_tokens=self.n, n_seqs=self.n_seqs, max_new=max(self.news), max_ctx=max(self.lens), n_heads=heads, n_kv_heads=kv,
+                    head_dim=dim, window=window, keep_first=keep)
+
+
+def awkward_rows(rng, n, kv, dim, dtype):
+    """Rows whose groups end where a rule could slip: ties between codes, a largest number at and beside a scale's seventh multiple,
+    zeros, subnormals, numbers past the format, infinities and NaN."""
+    x = rng.standard_normal((n, kv, dim)) * np.exp(3 * rng.standard_normal((n, kv, 1)))
+    g = x.reshape(-1, 32)
+    b = rng.integers(0, 255, len(g))
+    s = plain.SCALES[b]
+    for i in range(len(g)):
+        kind = i % 11
+        if kind == 0:
+            g[i] = s[i] * (rng.integers(-7, 7, 32) + 0.5)
+            g[i, 0] = 7 * s[i]
+        elif kind == 1:
+            g[i] = np.clip(g[i], -1, 1) * s[i]
+            g[i, 5] = 7 * s[i] * (1 + 2.0 ** -7)
+        elif kind == 2:
+            g[i] = np.clip(g[i], -1, 1) * s[i]
+            g[i, 31] = -7 * s[i]
+        elif kind == 3:
+            g[i] = 0.0
+        elif kind == 4:
+            g[i] *= 1e-30 if i % 2 else 1e-41
+        elif kind == 5:
+            g[i] *= 1e6
+        elif kind == 6 and i % 2:
+            g[i, 7] = [np.nan, np.inf, -np.inf][i % 3]
+        elif kind == 7:
+            g[i] = s[i] * (rng.integers(-7, 7, 32) + 0.5) * (1 + 2.0 ** -23 * rng.integers(-2, 3, 32))
+            g[i, 3] = 7 * s[i]
+    return torch.tensor(g.reshape(n, kv, dim)).to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv, dim", [(1, 32), (3, 64), (2, 96), (8, 128), (5, 256)])
+@pytest.mark.parametrize("pasts, news", [([0], [1]), ([63, 64, 0], [2, 1, 130]), ([5, 700], [600, 1])])
+def test_what_the_pages_hold_is_the_definition_bit_for_bit(dtype, kv, dim, pasts, news):
+    step, rng = Step(pasts, news), np.random.default_rng(dim + len(news))
+    rows = awkward_rows(rng, step.n + 3, 2 * kv, dim, dtype)
+    k, v = rows[:, :kv], rows[:, kv:]
+    before = torch.randint(0, 256, (step.pages, kv, kernels.cache4_record_bytes(dim)), dtype=torch.uint8, device=DEV)
+    pool = before.clone()
+    kernels.cache4_append(k, v, pool, step.positions, step.token_seq, step.ctx, step.table, step.width, n_tokens=step.n)
+    want = before.cpu().numpy().copy()
+    xk, xv = host(k), host(v)
+    hk, hv = plain.held(xk), plain.held(xv)
+    for t in range(step.n):
+        seq, pos = int(step.token_seq[t]), int(step.positions[t])
+        page, r, at = step.lists[seq, pos // PAGE], pos % PAGE, dim // 2
+        for h in range(kv):
+            one = plain.record(np.repeat(xk[t, h][None], PAGE, 0), np.repeat(xv[t, h][None], PAGE, 0))
+            for first, size in ((0, at), (32 * dim, at), (64 * dim, dim // 32), (66 * dim, dim // 32)):
+                want[page, h, first + r * size:first + (r + 1) * size] = one[first:first + size]
+    assert np.array_equal(pool.cpu().numpy(), want)
+    got_k = torch.full((step.n + 2, kv, dim), 9.0, dtype=dtype, device=DEV)
+    got_v = torch.full_like(got_k, 9.0)
+    kernels.cache4_gather(pool, step.positions, step.token_seq, step.table, step.width, got_k, got_v, n_tokens=step.n)
+    assert np.array_equal(host(got_k[:step.n]), hk[:step.n], equal_nan=True)
+    assert np.array_equal(host(got_v[:step.n]), hv[:step.n], equal_nan=True)
+    assert bool((got_k[step.n:] == 9).all()) and bool((got_v[step.n:] == 9).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rows_of_any_stride_and_alignment(dtype, shift):
+    kv, dim, step = 2, 64, Step([10, 0], [1, 70])
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    proj = torch.randn(step.n, 5 * kv * dim + 7 + shift, generator=gen, device=DEV).to(dtype)[:, shift:]
+    k = proj[:, 3:3 + 2 * kv * dim].view(step.n, kv, 2 * dim)[..., :dim]      # heads two heads apart
+    v = proj[:, 300:300 + kv * dim].view(step.n, kv, dim)
+    pool = torch.zeros(step.pages, kv, kernels.cache4_record_bytes(dim), dtype=torch.uint8, device=DEV)
+    kernels.cache4_append(k, v, pool, step.positions, step.token_seq, step.ctx, step.table, step.width, n_tokens=step.n)
+    rows = torch.zeros(step.n, 3 * kv * dim + shift, dtype=dtype, device=DEV)[:, shift:]
+    got_k, got_v = rows[:, :kv * dim].view(step.n, kv, dim), rows[:, 2 * kv * dim:].view(step.n, kv, dim)
+    kernels.cache4_gather(pool, step.positions, step.token_seq, step.table, step.width, got_k, got_v, n_tokens=step.n)
+    assert np.array_equal(host(got_k), plain.held(host(k))) and np.array_equal(host(got_v), plain.held(host(v)))
+    assert bool((rows[:, kv * dim:2 * kv * dim] == 0).all())
+
+
+def test_a_ring_keeps_its_newest_positions():
+    kv, dim, step = 1, 32, Step([100, 0], [300, 10], ring=3)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k, v = (torch.randn(step.n, kv, dim, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    pool = torch.zeros(step.pages, kv, kernels.cache4_record_bytes(dim), dtype=torch.uint8, device=DEV)
+    kernels.cache4_append(k, v, pool, step.positions, step.token_seq, step.ctx, step.table, step.width, n_tokens=step.n)
+    got_k, got_v = torch.empty_like(k), torch.empty_like(v)
+    kernels.cache4_gather(pool, step.positions, step.token_seq, step.table, step.width, got_k, got_v, n_tokens=step.n)
+    kept = [t for t in range(step.n) if int(step.positions[t]) >= step.lens[int(step.token_seq[t])] - 3 * PAGE]
+    assert len(kept) == 3 * PAGE + 10
+    assert np.array_equal(host(got_k)[kept], plain.held(host(k))[kept]) and np.array_equal(host(got_v)[kept], plain.held(host(v))[kept])
+
+
+def filled(step, kv, dim, rng, spread=1.0):
+    """A pool whose records hold every sequence's keys and values; everything else in it (rows past a sequence's end, pages of nobody)
+    stands for NaN.  Returns the pool and the held values, [positions, kv, dim] a sequence."""
+    pool = np.full((step.pages, kv, kernels.cache4_record_bytes(dim)), 255, dtype=np.uint8)
+    keys, values = [], []
+    for s, length in enumerate(step.lens):
+        gain = np.exp(0.5 * rng.standard_normal((kv, dim)))
+        k = rng.standard_normal((length, kv, dim)) * gain * spread
+        v = rng.standard_normal((length, kv, dim)) * np.exp(rng.standard_normal((length, kv, 1)))
+        keys.append(plain.held(k))
+        values.append(plain.held(v))
+        lost = max(0, -(-length // PAGE) - step.width)       # pages of a ring that have come round
+        for page in range(lost, -(-length // PAGE)):
+            for h in range(kv):
+                rows = [np.full((PAGE, dim), np.nan) for _ in range(2)]
+                n = min(PAGE, length - page * PAGE)
+                rows[0][:n], rows[1][:n] = k[page * PAGE:page * PAGE + n, h], v[page * PAGE:page * PAGE + n, h]
+                pool[step.lists[s, page % step.width], h] = plain.record(*rows)
+    return torch.tensor(pool, device=DEV), keys, values
+
+
+def attend(step, q, pool, heads, kv, dim, window, keep, scale, rows=2, **kw):
+    sizes = step.sizes(heads, kv, dim, window, keep)
+    out = torch.full((step.n + rows, heads * dim), 7.0, dtype=q.dtype, device=DEV)
+    scratch = torch.full((max(1, kernels.cache4_attention_scratch_floats(**sizes)),), float("nan"), device=DEV)
+    kernels.cache4_attention(q, out, pool, step.table, step.width, step.seq_start, step.past, scale=scale, scratch=scratch, **sizes, **kw)
+    kernels.check_status(torch.device(DEV))
+    assert bool((out[step.n:] == 7).all())
+    return out[:step.n]
+
+
+def compare(step, got, q, keys, values, heads, kv, dim, window, keep, scale):
+    bits = 8 if got.dtype == torch.bfloat16 else 24
+    for s in range(step.n_seqs):
+        a, b = step.starts[s], step.starts[s + 1]
+        if a == b:
+            continue
+        x = host(q[a:b, :heads * dim]).reshape(-1, heads, dim)
+        y, size, reach, count = plain.attention(x, keys[s], values[s], step.pasts[s], scale, window, keep)
+        far = np.abs(host(got[a:b]).reshape(y.shape) - y) / (plain.allowed(bits, y, size, reach, count, dim) + 1e-300)      # (a channel of zeros allows nothing)
+        assert far.max() <= 1.0, (s, float(far.max()), np.unravel_index(far.argmax(), far.shape))
+
+
+STEPS = [([0], [1]), ([62, 63, 64, 900], [1, 1, 1, 1]), ([0, 0, 0], [1, 65, 200]), ([3, 0, 300, 129], [70, 1, 129, 0]),
+         ([1000, 2], [16, 3])]
+SEES = [(0, 0), (1, 0), (50, 3), (64, 64), (100, 130)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv, dim", [(1, 1, 32), (4, 4, 64), (8, 1, 128), (6, 2, 96), (2, 1, 256), (15, 3, 64), (16, 2, 128)])
+@pytest.mark.parametrize("pasts, news", STEPS)
+@pytest.mark.parametrize("window, keep", SEES)
+def test_attention(dtype, heads, kv, dim, pasts, news, window, keep):
+    step, rng = Step(pasts, news), np.random.default_rng(heads * dim + window)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim + 24))).to(dtype).to(DEV)
+    scale = dim ** -0.5
+    got = attend(step, q, pool, heads, kv, dim, window, keep, scale)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, scale)
+    assert torch.equal(got, attend(step, q, pool, heads, kv, dim, window, keep, scale))
