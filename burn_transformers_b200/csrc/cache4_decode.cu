@@ -1,0 +1,461 @@
+// Attention over a 4-bit cache (cache4.cuh) for steps that bring few tokens a sequence: bfloat16 queries, heads of 64 or 128 channels.
+//
+// A block serves one (sequence, key head) and 8 or 16 columns: the query heads that share the key head, for each new token.  Each of its
+// four warps takes pages of the visible run by itself, through a ring of its own (a page of a key head is one record: one bulk copy), so
+// that no barrier stands between pages.  With the keys on the 16 rows of an mma.sync tile and the columns on its 8:
+//   S^T = K q^T   a lane's 16 (8) bytes of a key row are 32 (16) channels in a row; the contraction may take the channels in any order, so
+//                 that the codes go to the tensor cores as they come out of the word (nibbles i and i + 4), and the queries are put in
+//                 that order once;
+//   O^T = V^T P^T a lane takes the same bytes of two keys and pairs their nibbles; the rows of a score tile are keys in such an order
+//                 that the weights, transposed by movmatrix, meet their keys' values.
+// A code n becomes the bfloat16 128 + n by setting the exponent's bits (a shift and one logical operation for two codes), and (128 + n) s
+// - 136 s in one multiply-add for two is the value itself, exactly: 136 s has 8 significant bits.  Maximum, sum and products are 32-bit; the
+// weights are rounded to bfloat16 for the second product, as the other attention kernels of this library do.
+//
+// What bounds it: the integer pipe, which takes the codes apart (about 7 operations a key and key head of 128 channels and warp), close
+// to the memory behind it (136 bytes).  The run is cut into `n_splits` pieces where sequences and heads do not fill the GPU; their
+// partial results (maximum, sum, weighted values) are joined in order by a second kernel.
+// Keys that a column does not see get the weight 0 exactly, and what lies in a page past the sequence's end (any bytes) is never
+// multiplied; a value filed as NaN reaches the columns that see its key and no other.
+#include "cache4.cuh"
+#include "decode_mma.cuh"
+
+namespace bt {
+
+constexpr int C4D_WARPS = 4;
+constexpr int C4D_WAIT_LIMIT = 1 << 20;
+
+struct Cache4DecodeParams {
+  const __nv_bfloat16* q;
+  long long q_row;
+  __nv_bfloat16* out;
+  const int *seq_start, *past_len;
+  int n_heads, group, col_blocks;
+  float scale_log2;
+  int window, keep_first;
+  float* part;                 // [unit][split][columns][HD], then [unit][split][columns][2]
+  long long part_ml;           // where the second begins
+};
+
+template <int HD>
+constexpr int c4d_slots() { return HD == 128 ? 2 : 3; }
+template <int HD, int NT>
+constexpr size_t c4d_smem() { return (size_t)C4D_WARPS * c4d_slots<HD>() * c4_record(HD); }
+
+// Two codes as bfloat16 128 + n: nibble `I` of both halves of `w`.
+template <int I>
+__device__ __forceinline__ unsigned c4d_pair(unsigned w) {
+  return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
+}
+__device__ __forceinline__ unsigned c4d_fma2(unsigned a, unsigned b, unsigned c) {
+  unsigned d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// A scale byte's bfloat16 bits (low half).
+__device__ __forceinline__ unsigned c4d_scale(unsigned b) { return b == 255u ? 0x7fc0u : b * 16u + 0x3580u; }
+__device__ __forceinline__ unsigned c4d_shift(unsigned s2) {
+  const unsigned c = 0xc308c308u;      // -136 in both halves
+  return c4d_fma2(s2, c, 0x80008000u);
+}
+__device__ __forceinline__ unsigned c4d_transpose(unsigned v) {
+  unsigned d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
+  return d;
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(C4D_WARPS * 32, NT == 1 ? 3 : 2)
+cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
+  constexpr int SLOTS = c4d_slots<HD>(), REC = c4_record(HD), G = HD / 32;
+  constexpr int KW = HD / 32;            // 32-bit words of a key row a lane holds
+  constexpr int VW = HD / 64;            // of a value row
+  constexpr int MT = HD / 16;
+  constexpr int COLS = 8 * NT;
+  extern __shared__ __align__(128) unsigned char c4d_raw[];
+  __shared__ __align__(8) unsigned long long s_full[C4D_WARPS][SLOTS];
+  __shared__ float s_ml[C4D_WARPS][COLS][2];
+  __shared__ int s_failed;
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int split = blockIdx.x, n_splits = gridDim.x, seq = blockIdx.z;
+  const int kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS;
+  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0, n_cols = n_new * p.group - col0;
+  if (n_cols <= 0) return;
+  const int past = p.past_len[seq];
+  const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
+  // the pages that any column sees: kept ones before the window's, then the window's
+  const int lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
+  const int pg_lo = lo / C4_PAGE, pg_hi = pos_last / C4_PAGE;
+  const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
+  const int n_pages = kept_only + pg_hi - pg_lo + 1;
+  const int per = max((n_pages + n_splits - 1) / n_splits, min(C4D_WARPS, n_pages));      // (a page a warp at least)
+  const int first = split * per, mine = min(n_pages, first + per) - first;
+  const long long unit = (long long)seq * gridDim.y + blockIdx.y;
+  if (mine <= 0) return;                 // (the join counts the pieces in the same way)
+  auto page_at = [&](int i) { return i < kept_only ? i : pg_lo + (i - kept_only); };
+
+  if (lane == 0) {
+    for (int s = 0; s < SLOTS; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(ds_smem(&s_full[warp][s])));
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (tid == 0) s_failed = 0;
+  __syncthreads();
+  unsigned char* ring = c4d_raw + warp * SLOTS * REC;
+  const int count = mine > warp ? (mine - warp + C4D_WARPS - 1) / C4D_WARPS : 0;      // this warp's pages: first + warp + 4 i
+  auto ask = [&](int i, const unsigned char* rec) {      // (one lane)
+    const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]);
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((unsigned)REC) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                     ds_smem(ring + i % SLOTS * REC)),
+                 "l"(rec), "r"((unsigned)REC), "r"(bar)
+                 : "memory");
+  };
+  if (lane < min(SLOTS, count)) ask(lane, c4_page(c, seq, page_at(first + warp + C4D_WARPS * lane), kv_head, HD));
+
+  // the queries, column g (+ 8) of the second operand: this lane's channels in the order in which codes leave a word
+  unsigned qf[NT][KW][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = 8 * n + g;
+    uint4 raw[HD / 32];
+#pragma unroll
+    for (int w = 0; w < KW; ++w) raw[w] = make_uint4(0, 0, 0, 0);
+    if (col < n_cols) {
+      const int token = (col0 + col) / p.group, head = kv_head * p.group + (col0 + col) % p.group;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (t0 + token) * p.q_row + (long long)head * HD + q * (HD / 4));
+#pragma unroll
+      for (int w = 0; w < KW; ++w) raw[w] = src[w];
+    }
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      qf[n][w][0] = __byte_perm(raw[w].x, raw[w].z, 0x5410);      // channels 0, 4
+      qf[n][w][1] = __byte_perm(raw[w].x, raw[w].z, 0x7632);      // 1, 5
+      qf[n][w][2] = __byte_perm(raw[w].y, raw[w].w, 0x5410);      // 2, 6
+      qf[n][w][3] = __byte_perm(raw[w].y, raw[w].w, 0x7632);      // 3, 7
+    }
+  }
+  // this lane's columns of a score tile: 2q, 2q + 1 (+ 8)
+  int pos[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) pos[n][e] = past + min(col0 + 8 * n + 2 * q + e, n_new * p.group - 1) / p.group;
+  float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[n][e] = -INFINITY;
+      l[n][e] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
+  }
+  const int kg = (g >> 1) + 4 * (g & 1);      // the key on row g of a tile of 16 (row g + 8: 8 further)
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    const int key0 = page_at(first + warp + C4D_WARPS * i) * C4_PAGE;
+    const unsigned char* rec = ring + i % SLOTS * REC;
+    {
+      const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]), parity = (unsigned)(i / SLOTS) & 1u;
+      bool landed = false;
+      for (int t = 0; t < C4D_WAIT_LIMIT && !landed; ++t) {
+        unsigned done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        landed = done != 0;
+      }
+      ok = __all_sync(0xffffffffu, landed);
+      if (!ok) break;
+    }
+    // ---- scores of the page's 64 keys ----
+    float s[NT][4][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][t][e] = 0.f;
+      unsigned w[2][KW], s2[2], sh[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = 16 * t + 8 * h + kg;
+        const unsigned char* row = rec + key * (HD / 2) + q * (HD / 8);
+        if constexpr (KW == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(row);
+          w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(row);
+          w[h][0] = v.x; w[h][1] = v.y;
+        }
+        const unsigned b = c4d_scale(rec[c4_key_scales(HD) + key * G + q * G / 4]);
+        s2[h] = b | b << 16;
+        sh[h] = c4d_shift(s2[h]);
+      }
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        unsigned x[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[h][0] = c4d_fma2(c4d_pair<0>(w[h][k]), s2[h], sh[h]);
+          x[h][1] = c4d_fma2(c4d_pair<1>(w[h][k]), s2[h], sh[h]);
+          x[h][2] = c4d_fma2(c4d_pair<2>(w[h][k]), s2[h], sh[h]);
+          x[h][3] = c4d_fma2(c4d_pair<3>(w[h][k]), s2[h], sh[h]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          ds_mma(s[n][t], x[0][0], x[1][0], x[0][1], x[1][1], qf[n][k][0], qf[n][k][1]);
+          ds_mma(s[n][t], x[0][2], x[1][2], x[0][3], x[1][3], qf[n][k][2], qf[n][k][3]);
+        }
+      }
+    }
+    // ---- which of them a column sees; maximum, weights ----
+    const bool whole = key0 + C4_PAGE - 1 <= pos_first &&
+                       (p.window <= 0 || key0 > pos_last - p.window || key0 + C4_PAGE <= p.keep_first);
+    auto seen = [&](int key, int at) { return key <= at && (p.window <= 0 || key > at - p.window || key < p.keep_first); };
+    unsigned pt[NT][4][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = s[n][t][e] * p.scale_log2;
+          if (!whole && !seen(key0 + 16 * t + 8 * (e >> 1) + kg, pos[n][e & 1])) v = -INFINITY;
+          s[n][t][e] = v;
+          top[e & 1] = fmaxf(top[e & 1], v);
+        }
+      float use[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+        const float m_new = fmaxf(m[n][e], top[e]);
+        use[e] = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = ds_exp2(m[n][e] - use[e]);      // 0 for a column that had seen nothing yet
+        m[n][e] = m_new;
+        l[n][e] *= alpha;
+#pragma unroll
+        for (int k = 0; k < MT; ++k) {
+          acc[n][k][e] *= alpha;
+          acc[n][k][e + 2] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = ds_exp2(s[n][t][e] - use[e & 1]);
+          l[n][e & 1] += w[e];
+        }
+        pt[n][t][0] = c4d_transpose(ds_pack(w[0], w[1]));
+        pt[n][t][1] = c4d_transpose(ds_pack(w[2], w[3]));
+      }
+    }
+    // ---- weighted values: a lane's keys of a tile are q, q + 4, q + 8, q + 12 ----
+    bool odd = false;                       // a value of NaN among this lane's
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      unsigned w[4][VW], b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = 16 * t + q + 4 * j;
+        const unsigned char* row = rec + c4_value_codes(HD) + key * (HD / 2) + g * (HD / 16);
+        if constexpr (VW == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(row);
+          w[j][0] = v.x; w[j][1] = v.y;
+        } else {
+          w[j][0] = *reinterpret_cast<const unsigned*>(row);
+        }
+        const unsigned raw = rec[c4_value_scales(HD) + key * G + g * G / 8];
+        b[j] = raw * 16u + 0x3580u;
+        const bool past_end = !whole && key0 + key > pos_last;
+        if (raw == 255u || past_end) {      // (NaN is seen to below; what lies past the end is not there)
+          b[j] = 0u;
+          odd |= !past_end;
+        }
+      }
+      const unsigned s01 = b[0] | b[1] << 16, s23 = b[2] | b[3] << 16;
+      const unsigned h01 = c4d_shift(s01), h23 = c4d_shift(s23);
+#pragma unroll
+      for (int k = 0; k < VW; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const unsigned a = __byte_perm(w[0][k], w[1][k], half ? 0x7632 : 0x5410), d = __byte_perm(w[2][k], w[3][k], half ? 0x7632 : 0x5410);
+          unsigned x[4], y[4];
+          x[0] = c4d_fma2(c4d_pair<0>(a), s01, h01);
+          x[1] = c4d_fma2(c4d_pair<1>(a), s01, h01);
+          x[2] = c4d_fma2(c4d_pair<2>(a), s01, h01);
+          x[3] = c4d_fma2(c4d_pair<3>(a), s01, h01);
+          y[0] = c4d_fma2(c4d_pair<0>(d), s23, h23);
+          y[1] = c4d_fma2(c4d_pair<1>(d), s23, h23);
+          y[2] = c4d_fma2(c4d_pair<2>(d), s23, h23);
+          y[3] = c4d_fma2(c4d_pair<3>(d), s23, h23);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            ds_mma(acc[n][4 * k + 2 * half], x[0], x[1], y[0], y[1], pt[n][t][0], pt[n][t][1]);
+            ds_mma(acc[n][4 * k + 2 * half + 1], x[2], x[3], y[2], y[3], pt[n][t][0], pt[n][t][1]);
+          }
+        }
+    }
+    if (__any_sync(0xffffffffu, odd)) {      // the columns that see a key whose values are NaN
+      for (int key = 0; key < C4_PAGE; ++key) {
+        if (rec[c4_value_scales(HD) + key * G + g * G / 8] != 255u) continue;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (seen(key0 + key, pos[n][e])) {
+#pragma unroll
+              for (int k = 0; k < MT; ++k) acc[n][k][e] = acc[n][k][e + 2] = NAN;
+            }
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && i + SLOTS < count) {
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      ask(i + SLOTS, c4_page(c, seq, page_at(first + warp + C4D_WARPS * (i + SLOTS)), kv_head, HD));
+    }
+  }
+  if (!ok) {
+    s_failed = 1;
+    let_copies_land();
+  }
+  // ---- the warps' results, joined in shared memory (over the rings) ----
+  float* s_acc = reinterpret_cast<float*>(c4d_raw);      // [warp][column][HD]
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+      if (g == 0) {
+        s_ml[warp][8 * n + 2 * q + e][0] = m[n][e];
+        s_ml[warp][8 * n + 2 * q + e][1] = l[n][e];
+      }
+    }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* row = s_acc + (warp * COLS + 8 * n + 2 * q + e) * HD + g * (HD / 8);
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {      // tile k: channels 2k, 2k + 1 of this lane's
+        row[2 * k] = acc[n][k][e];
+        row[2 * k + 1] = acc[n][k][e + 2];
+      }
+    }
+  __syncthreads();
+  if (s_failed && tid == 0 && c.status) atomicExch(c.status, 10);
+  for (int i = tid; i < COLS * HD; i += C4D_WARPS * 32) {
+    const int col = i / HD, d = i % HD;
+    if (col >= n_cols) break;
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < C4D_WARPS; ++w) top = fmaxf(top, s_ml[w][col][0]);
+    const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < C4D_WARPS; ++w) {
+      const float weight = ds_exp2(s_ml[w][col][0] - use);
+      sum += s_ml[w][col][1] * weight;
+      o += s_acc[(w * COLS + col) * HD + d] * weight;
+    }
+    if (s_failed) sum = NAN;
+    if (n_splits == 1) {
+      const int token = (col0 + col) / p.group, head = kv_head * p.group + (col0 + col) % p.group;
+      p.out[((long long)(t0 + token) * p.n_heads + head) * HD + d] = __float2bfloat16_rn(o / sum);
+    } else {
+      const long long at = (unit * n_splits + split) * COLS + col;
+      p.part[at * HD + d] = o;
+      if (d == 0) {
+        p.part[p.part_ml + 2 * at] = top;
+        p.part[p.part_ml + 2 * at + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the pieces of a (sequence, key head, columns) in their order.  A block a unit, a thread a channel.
+template <int HD, int NT>
+__global__ void __launch_bounds__(HD)
+cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
+  constexpr int COLS = 8 * NT;
+  pdl_trigger();
+  pdl_wait();
+  const int seq = blockIdx.z, kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS, col = blockIdx.x;
+  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  if (col0 + col >= n_new * p.group) return;
+  const int past = p.past_len[seq];
+  const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
+  const int pg_lo = (p.window > 0 ? max(0, pos_first - p.window + 1) : 0) / C4_PAGE;
+  const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
+  const int n_pages = kept_only + pos_last / C4_PAGE - pg_lo + 1;
+  const int per = max((n_pages + n_splits - 1) / n_splits, min(C4D_WARPS, n_pages)), used = (n_pages + per - 1) / per;
+  const long long unit = (long long)seq * gridDim.y + blockIdx.y;
+  float top = -INFINITY, sum = 0.f, o = 0.f;
+  for (int s = 0; s < used; ++s) {
+    const long long at = (unit * n_splits + s) * COLS + col;
+    const float m = p.part[p.part_ml + 2 * at], l = p.part[p.part_ml + 2 * at + 1], x = p.part[at * HD + threadIdx.x];
+    const float m_new = fmaxf(top, m), use = m_new == -INFINITY ? 0.f : m_new;
+    const float a = ds_exp2(top - use), b = ds_exp2(m - use);
+    sum = sum * a + l * b;
+    o = o * a + x * b;
+    top = m_new;
+  }
+  const int token = (col0 + col) / p.group, head = kv_head * p.group + (col0 + col) % p.group;
+  p.out[((long long)(t0 + token) * p.n_heads + head) * HD + threadIdx.x] = __float2bfloat16_rn(o / sum);
+}
+
+template <int HD, int NT>
+static int launch_c4d(const Cache4DecodeParams& p, const Cache4View& c, int n_seqs, int n_splits, cudaStream_t stream) {
+  constexpr size_t smem = c4d_smem<HD, NT>();
+  static_assert(smem >= sizeof(float) * C4D_WARPS * 8 * NT * HD, "the joined results outgrow the rings");
+  auto kern = cache4_decode_kernel<HD, NT>;
+  static SharedMemoryAllowance allowed;
+  BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
+  const dim3 grid(n_splits, c.n_kv_heads * p.col_blocks, n_seqs);
+  BT_PDL_OK("cache4_decode", launch_pdl(kern, grid, dim3(C4D_WARPS * 32), smem, stream, 1, p, c));
+  if (n_splits > 1)
+    BT_PDL_OK("cache4_join", launch_pdl(cache4_join_kernel<HD, NT>, dim3(8 * NT, c.n_kv_heads * p.col_blocks, n_seqs), dim3(HD), 0, stream, 1, p, n_splits));
+  return 0;
+}
+
+}  // namespace bt
+
+// Arguments as bt_cache4_attention (bfloat16).  max_new * (n_heads / n_kv_heads) columns a key head go in blocks of 8 or 16.
+// scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * column blocks * splits * columns * (dim + 2).
+extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
+                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
+                                int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
+                                float* scratch, long long scratch_floats, cudaStream_t stream) {
+  using namespace bt;
+  BT_CHECK(dim == 64 || dim == 128, "cache4_attention: the kernel for few tokens takes heads of 64 or 128 channels, not %d", dim);
+  BT_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "cache4_attention: %d query heads cannot share %d key heads", n_heads, n_kv_heads);
+  BT_CHECK(n_pages > 0 && table != nullptr && table_len > 0 && n_seqs >= 0 && max_new >= 0 && window >= 0 && keep_first >= 0,
+           "cache4_attention: bad sizes pages=%lld table_len=%d sequences=%d window=%d kept=%d", n_pages, table_len, n_seqs, window, keep_first);
+  auto at16 = [](const void* x) { return (unsigned long long)x % 16 == 0; };
+  BT_CHECK(at16(pool) && at16(q) && q_row % 8 == 0, "cache4_attention: pool and query rows must lie on 16-byte boundaries");
+  if (n_seqs == 0 || max_new == 0) return 0;
+  const int group = n_heads / n_kv_heads;
+  const long long cols = (long long)max_new * group;
+  const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
+  BT_CHECK(n_seqs <= 65535 && (long long)n_kv_heads * blocks <= 65535 && n_splits >= 1 && n_splits <= 65535, "cache4_attention: grid too large");
+  const long long parts = (long long)n_seqs * n_kv_heads * blocks * n_splits * 8 * nt;
+  BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
+           "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
+  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks,
+                             scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
+  const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
+  if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, stream);
+  return nt == 1 ? launch_c4d<128, 1>(p, c, n_seqs, n_splits, stream) : launch_c4d<128, 2>(p, c, n_seqs, n_splits, stream);
+}

@@ -2067,20 +2067,50 @@ def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_token
         c_int(k.shape[1]), c_int(k.shape[2]), c_int(DTYPE_CODE[k.dtype]), _stream()))
 
 
+def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
+    """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
+
+    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, blocks of 8 or 16 of them."""
+    columns = max_new * (n_heads // n_kv_heads)
+    if head_dim not in (64, 128) or columns > 16:
+        return "any", 1, 0
+    wide = 8 if columns <= 8 else 16
+    units = max(1, n_seqs * n_kv_heads)
+    span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
+    pages = max(1, -(-span // PAGE_SIZE))
+    # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
+    splits = max(1, min(-(-6 * _sm_count() // units), -(-pages // 4)))
+    return "few", splits, units * splits * wide * (head_dim + 2) if splits > 1 else 0
+
+
+_SM_COUNTS: dict = {}
+
+
+def _sm_count() -> int:
+    device = torch.cuda.current_device()
+    if device not in _SM_COUNTS:
+        _SM_COUNTS[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return _SM_COUNTS[device]
+
+
 def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window=0, keep_first=0) -> int:
     """32-bit words of `scratch` that cache4_attention wants for a step of these sizes."""
-    return 0
+    if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
+        raise ShapeError(f"cache4_attention: {n_heads} query heads cannot share {n_kv_heads} key heads")
+    return _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)[2]
 
 
 def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads,
-                     head_dim, scale, window=0, keep_first=0, scratch=None):
+                     head_dim, scale, window=0, keep_first=0, scratch=None, impl=None):
     """Causal attention of a step's queries over a layer's 4-bit pages, which hold the step's own keys and values too.
 
     q: rows whose first n_heads * head_dim elements are the query heads (bfloat16 or 32-bit); out: [tokens, n_heads * head_dim] of
     the same type.  Sequence s brings the tokens seq_start[s] .. seq_start[s + 1] behind past_len[s] others, at most `max_new` of
     them, and is no longer than `max_ctx` after the step.  A query at position p sees the keys j <= p with j > p - window (`window`
     0: all) or j < keep_first.  Rows of `out` behind the last sequence stay as they are.  Where the pages come round, what a query
-    sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0."""
+    sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0.  `scratch`: 32-bit, cache4_attention_scratch_floats of the same
+    sizes (more does no harm); two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that takes
+    every case."""
     if q.dtype not in DTYPE_CODE:
         raise ShapeError(f"cache4_attention: unsupported element type {q.dtype}")
     if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
@@ -2100,7 +2130,21 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     if max_ctx > table_len * PAGE_SIZE and (keep_first or not window or table_len * PAGE_SIZE < window + max_new - 1):
         raise ShapeError(f"cache4_attention: {table_len} pages that come round do not hold what queries of a context of {max_ctx} see "
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
-    _together(q, out, pool, table, seq_start, past_len)
+    _together(q, out, pool, table, seq_start, past_len, scratch)
+    kind, splits, floats = "any", 1, 0
+    if impl != "any" and q.dtype is torch.bfloat16 and q.data_ptr() % 16 == 0 and row % 8 == 0:
+        kind, splits, floats = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
+    if floats:
+        if scratch is None:
+            raise ShapeError(f"cache4_attention: a step of these sizes needs {floats} floats of scratch")
+        _need(scratch, "scratch", torch.float32, (None,))
+        _enough(scratch, "scratch", floats)
+    if kind == "few":
+        _check(library().bt_cache4_decode(
+            _ptr(q), c_longlong(row), _ptr(out), _ptr(pool), c_longlong(pool.shape[0]), _ptr(table), c_int(table.shape[1]), c_int(table_len),
+            _ptr(kernel_status(q.device)), _ptr(seq_start), _ptr(past_len), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads),
+            c_int(head_dim), c_float(scale), c_int(window), c_int(keep_first), c_int(splits), _ptr(scratch), c_longlong(floats), _stream()))
+        return
     _check(library().bt_cache4_attention(
         _ptr(q), c_longlong(row), _ptr(out), _ptr(pool), c_longlong(pool.shape[0]), _ptr(table), c_int(table.shape[1]), c_int(table_len),
         _ptr(kernel_status(q.device)), _ptr(seq_start), _ptr(past_len), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads),

@@ -192,3 +192,28 @@ def test_attention(dtype, heads, kv, dim, pasts, news, window, keep):
     got = attend(step, q, pool, heads, kv, dim, window, keep, scale)
     compare(step, got, q, keys, values, heads, kv, dim, window, keep, scale)
     assert torch.equal(got, attend(step, q, pool, heads, kv, dim, window, keep, scale))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv, dim", [(4, 2, 64), (8, 1, 128)])
+@pytest.mark.parametrize("pasts, news", [([70, 300], [3, 2]), ([0, 100], [140, 1])])
+@pytest.mark.parametrize("window, keep", [(0, 0), (40, 3)])
+def test_a_key_or_value_of_nan_reaches_the_queries_that_see_it_and_no_other(dtype, heads, kv, dim, pasts, news, window, keep):
+    step, rng = Step(pasts, news), np.random.default_rng(dim)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).to(dtype).to(DEV)
+    clean = attend(step, q, pool, heads, kv, dim, window, keep, dim ** -0.5)
+    for where, which in ((1, 1), (60, 1), (71, 1), (71, 0), (99, 1), (2, 0)):
+        bad, group, h = pool.clone(), rng.integers(dim // 32), rng.integers(kv)
+        s = 0 if where < step.lens[0] else 1
+        at = (66 if which else 64) * dim + where % PAGE * (dim // 32) + group
+        bad[int(step.lists[s, where // PAGE]), h, at] = 255
+        got = attend(step, q, bad, heads, kv, dim, window, keep, dim ** -0.5).view(step.n, heads, dim)
+        hit = torch.zeros(step.n, heads, dim, dtype=torch.bool, device=DEV)
+        for t in range(step.starts[s], step.starts[s + 1]):
+            p = int(step.positions[t])
+            if where <= p and (not window or where > p - window or where < keep):
+                channels = slice(32 * group, 32 * group + 32) if which else slice(0, dim)
+                hit[t, h * (heads // kv):(h + 1) * (heads // kv), channels] = True
+        assert torch.equal(torch.isnan(got), hit), (where, which)
+        assert torch.equal(got[~hit], clean.view(got.shape)[~hit])
