@@ -38,6 +38,7 @@ def library() -> ctypes.CDLL:
         lib.bt_lightning_chunked_scratch_floats.restype = c_longlong
         lib.bt_mlstm_chunked_scratch_floats.restype = c_longlong
         lib.bt_launch_count.restype = c_longlong
+        _declare(lib)
         if lib.bt_abi_version() != 1:
             raise KernelError(f"{path} has an unexpected interface version")
         _LIB = lib
@@ -1926,73 +1927,111 @@ def gla_scan(proj, q_off, k_off, v_off, q_scale: float, dt, log_scale: float, st
 
 
 # ---- queries and keys normed and turned; a cache held in 4 bits -------------------------------
+# A decode step makes these calls once a layer and kernels of a few microseconds wait for them: their checks are single expressions
+# that name a fault only once they have found one, and the library's functions take plain integers (`_ARGUMENTS`).
 
-def _rows_view(t, name, width, dtype) -> int:
-    """`t` as rows of at least `width` contiguous elements; returns the elements between rows."""
+_ARGUMENTS = {
+    "bt_qk_norm_rotary": "plplppppiiiiiffiip",
+    "bt_cache4_append": "pllpllplppppiiipiiiip",
+    "bt_cache4_gather": "pllpllplpppiiipiiiip",
+    "bt_cache4_attention": "plpplpiipppiiiiifiiip",
+    "bt_cache4_decode": "plpplpiipppiiiiifiiiplp",
+}
+
+
+def _declare(lib) -> None:
+    kinds = {"p": c_void_p, "l": c_longlong, "i": c_int, "f": c_float}
+    for name, letters in _ARGUMENTS.items():
+        getattr(lib, name).argtypes = [kinds[c] for c in letters]
+
+
+def _fault(t, name, device, dtype, shape, note="contiguous") -> None:
+    """Raises what is wrong with one argument: its kind, its device, its element type, or its extents or layout."""
+    if not isinstance(t, torch.Tensor):
+        raise ShapeError(f"{name}: expected a tensor, found {type(t).__name__}")
     if not t.is_cuda:
         raise KernelError(f"{name}: lies on {t.device}; the kernels of this library run on a CUDA device only")
+    if t.get_device() != device:
+        raise KernelError(f"{name}: lies on cuda:{t.get_device()}, but the current device, whose stream the call goes to, is cuda:{device}")
     if t.dtype is not dtype:
         raise ShapeError(f"{name}: expected dtype {dtype}, found {t.dtype}")
-    if t.dim() != 2 or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ShapeError(f"{name}: expected rows of at least {width} contiguous elements, found shape {list(t.shape)}, strides "
-                         f"{list(t.stride())}")
+    raise ShapeError(f"{name}: expected {shape}, {note}; found shape {list(t.shape)}, strides {list(t.stride())}")
+
+
+def _int_list(t, name, device, count) -> int:
+    """The address of a contiguous list of at least `count` int32."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.shape[0] >= count
+            and t.is_contiguous()):
+        _fault(t, name, device, torch.int32, f"a list of at least {count}")
+    return t.data_ptr()
+
+
+def _float_list(t, name, device, count) -> int:
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.dim() == 1 and t.shape[0] >= count
+            and t.is_contiguous()):
+        _fault(t, name, device, torch.float32, f"a list of at least {count}")
+    return t.data_ptr()
+
+
+def _row_stride(t, name, device, dtype, count, width, written=False) -> int:
+    """Elements between the rows of `t`: at least `count` rows of at least `width` contiguous elements (apart, if they are written)."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.shape[0] >= count
+            and t.shape[1] >= width and (t.stride(1) == 1 or width == 1) and (not written or count < 2 or t.stride(0) >= width)):
+        _fault(t, name, device, dtype, f"at least {count} rows of at least {width} elements", "contiguous within a row, rows apart")
     return t.stride(0)
 
 
-def _together(first, *others) -> None:
-    """All on one device, the current one: a launch goes to the current device's stream and reads the others' pointers as its own."""
-    device = first.device
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.device != device:
-            raise KernelError(f"tensors on {device} and {t.device} in one call")
+def _element_code(t, name) -> int:
+    code = DTYPE_CODE.get(getattr(t, "dtype", None))
+    if code is None:
+        raise ShapeError(f"{name}: expected a bfloat16 or 32-bit tensor, found {getattr(t, 'dtype', type(t).__name__)}")
+    return code
 
 
-def _enough(t, name, count) -> None:
-    if t.shape[0] < count:
-        raise ShapeError(f"{name}: {t.shape[0]} entries where the step needs {count}")
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+_STATUS_ADDRESS: dict = {}
+
+
+def _status_address(device: int) -> int:
+    """The address of kernel_status (which stays where it is)."""
+    hit = _STATUS_ADDRESS.get(device)
+    if hit is None:
+        hit = _STATUS_ADDRESS[device] = kernel_status(torch.device("cuda", device)).data_ptr()
+    return hit
 
 
 def qk_norm_rotary(proj, positions, inv_freq, *, n_tokens, n_heads, n_kv_heads, head_dim, rot_dims, q_weight=None, k_weight=None,
                    eps=0.0, interleaved=False, size=1.0, out=None):
     """The query and key heads of a step's projections, each normed over its channels and turned by its token's position, in one pass.
 
-    proj: rows [queries | keys | anything], `n_heads` and `n_kv_heads` heads of `head_dim` (at most 256) channels.  With `q_weight`
-    and `k_weight` ([head_dim], 32-bit; both or neither) a head becomes x / sqrt(mean(x^2) + eps) * weight.  Then its first `rot_dims`
-    channels turn by positions * inv_freq ([rot_dims / 2], 32-bit), channel i with i + rot_dims / 2, or 2i with 2i + 1 if
-    `interleaved`, cosine and sine times `size`; the angles are formed in 64-bit.  In place, or into `out`, other rows of at least
-    (n_heads + n_kv_heads) * head_dim elements, which then receive nothing but the queries and keys."""
-    if proj.dtype not in DTYPE_CODE:
-        raise ShapeError(f"qk_norm_rotary: unsupported element type {proj.dtype}")
-    if n_heads < 0 or n_kv_heads < 0 or n_heads + n_kv_heads < 1 or not 1 <= head_dim <= 256:
-        raise ShapeError(f"qk_norm_rotary: {n_heads} query and {n_kv_heads} key heads of {head_dim} channels (1 to 256)")
+    proj: rows [queries | keys | anything], `n_heads` and `n_kv_heads` heads of `head_dim` (at most 256) channels, bfloat16 or 32-bit.
+    With `q_weight` and `k_weight` ([head_dim], 32-bit; both or neither) a head becomes x / sqrt(mean(x^2) + eps) * weight.  Then its
+    first `rot_dims` channels turn by positions * inv_freq ([rot_dims / 2], 32-bit), channel i with i + rot_dims / 2, or 2i with 2i + 1
+    if `interleaved`, cosine and sine times `size`; the angles are formed in 64-bit.  In place, or into `out`, other rows of at least
+    (n_heads + n_kv_heads) * head_dim elements that do not overlap `proj`, which then receive nothing but the queries and keys."""
+    code = _element_code(proj, "proj")
+    if n_tokens < 0 or n_heads < 0 or n_kv_heads < 0 or n_heads + n_kv_heads < 1 or not 1 <= head_dim <= 256:
+        raise ShapeError(f"qk_norm_rotary: {n_tokens} tokens, {n_heads} query and {n_kv_heads} key heads of {head_dim} channels (1 to 256)")
     if rot_dims < 0 or rot_dims > head_dim or rot_dims % 2:
         raise ShapeError(f"qk_norm_rotary: {rot_dims} of {head_dim} channels cannot turn in pairs")
     if (q_weight is None) != (k_weight is None):
         raise ShapeError("qk_norm_rotary: give both weights or neither")
+    device = torch.cuda.current_device()
     width = (n_heads + n_kv_heads) * head_dim
-    row = _rows_view(proj, "proj", width, proj.dtype)
-    out_row = row
-    if out is not None:
-        out_row = _rows_view(out, "out", width, proj.dtype)
-        _enough(out, "out", n_tokens)
-    _enough(proj, "proj", n_tokens)
-    _need(positions, "positions", torch.int32, (None,))
-    _enough(positions, "positions", n_tokens)
-    if rot_dims:
-        _need(inv_freq, "inv_freq", torch.float32, (None,))
-        _enough(inv_freq, "inv_freq", rot_dims // 2)
+    row = _row_stride(proj, "proj", device, proj.dtype, n_tokens, width, out is None)
+    to, to_row = (proj, row) if out is None else (out, _row_stride(out, "out", device, proj.dtype, n_tokens, width, True))
+    at = _int_list(positions, "positions", device, n_tokens)
+    freq = _float_list(inv_freq, "inv_freq", device, rot_dims // 2) if rot_dims else 0
+    qw = kw = 0
     if q_weight is not None:
-        _need(q_weight, "q_weight", torch.float32, (head_dim,))
-        _need(k_weight, "k_weight", torch.float32, (head_dim,))
-    _together(proj, positions, out, q_weight, k_weight, inv_freq if rot_dims else None)
-    _work(10.0 * n_tokens * width, 2.0 * n_tokens * width * proj.element_size())
-    _check(library().bt_qk_norm_rotary(
-        _ptr(proj), c_longlong(row), _ptr(proj if out is None else out), c_longlong(out_row), _ptr(positions),
-        _ptr(inv_freq if rot_dims else None), _ptr(q_weight), _ptr(k_weight), c_int(n_tokens), c_int(n_heads), c_int(n_kv_heads),
-        c_int(head_dim), c_int(rot_dims), c_float(eps), c_float(size), c_int(1 if interleaved else 0), c_int(DTYPE_CODE[proj.dtype]),
-        _stream()))
+        qw, kw = _float_list(q_weight, "q_weight", device, head_dim), _float_list(k_weight, "k_weight", device, head_dim)
+    if _PROFILE is not None:
+        _work(10.0 * n_tokens * width, 2.0 * n_tokens * width * proj.element_size())
+    _check(library().bt_qk_norm_rotary(proj.data_ptr(), row, to.data_ptr(), to_row, at, freq, qw, kw, n_tokens, n_heads, n_kv_heads, head_dim,
+                                       rot_dims, eps, size, 1 if interleaved else 0, code, _raw_stream(device)))
 
 
 def cache4_record_bytes(head_dim: int) -> int:
@@ -2002,85 +2041,72 @@ def cache4_record_bytes(head_dim: int) -> int:
     return 68 * head_dim
 
 
-def _cache4_pool(pool, n_kv_heads, head_dim, table, table_len, n_seqs) -> None:
-    _need(pool, "pool", torch.uint8, (None, n_kv_heads, cache4_record_bytes(head_dim)))
-    _need(table, "table", torch.int32, (None, None))
-    if not 1 <= table_len <= table.shape[1]:
-        raise ShapeError(f"table: rows of {table.shape[1]} pages hold no list of {table_len}")
-    if table.shape[0] < n_seqs:
-        raise ShapeError(f"table: {table.shape[0]} rows for {n_seqs} sequences")
+def _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs) -> None:
+    if head_dim <= 0 or head_dim > 256 or head_dim % 32:
+        cache4_record_bytes(head_dim)
+    if not (isinstance(pool, torch.Tensor) and pool.dtype is torch.uint8 and pool.get_device() == device and pool.dim() == 3
+            and pool.shape[0] >= 1 and pool.shape[1] == n_kv_heads and pool.shape[2] == 68 * head_dim and pool.is_contiguous()):
+        _fault(pool, "pool", device, torch.uint8, f"[pages, {n_kv_heads}, {68 * head_dim}]")
+    if not (isinstance(table, torch.Tensor) and table.dtype is torch.int32 and table.get_device() == device and table.dim() == 2
+            and table.shape[0] >= n_seqs and table.shape[1] >= table_len >= 1 and table.is_contiguous()):
+        if isinstance(table, torch.Tensor) and table.dim() == 2 and not 1 <= table_len <= table.shape[1]:
+            raise ShapeError(f"table: rows of {table.shape[1]} pages hold no list of {table_len}")
+        _fault(table, "table", device, torch.int32, f"[at least {n_seqs} sequences, at least {table_len} pages]")
 
 
-def _cache4_heads(t, name, like=None):
-    """`t` as [tokens, key heads, channels] with contiguous channels: its strides between tokens and heads."""
-    if not t.is_cuda:
-        raise KernelError(f"{name}: lies on {t.device}; the kernels of this library run on a CUDA device only")
-    if t.dtype not in DTYPE_CODE or (like is not None and t.dtype is not like.dtype):
-        raise ShapeError(f"{name}: unsupported element type {t.dtype}" if like is None else f"{name}: expected dtype {like.dtype}, found {t.dtype}")
-    if t.dim() != 3 or t.stride(2) != 1 or (like is not None and t.shape[1:] != like.shape[1:]):
-        raise ShapeError(f"{name}: expected [tokens, key heads, channels] with contiguous channels"
-                         + (f" like {list(like.shape)}" if like is not None else "") + f", found shape {list(t.shape)}, strides {list(t.stride())}")
-    return c_longlong(t.stride(0)), c_longlong(t.stride(1))
+def _cache4_heads(t, name, device, dtype, count, heads, dim, written=False) -> None:
+    """`t` as [tokens, key heads, channels] with contiguous channels."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 3 and t.shape[0] >= count
+            and t.shape[1] == heads and t.shape[2] == dim and t.stride(2) == 1
+            and not (written and ((count > 1 and t.stride(0) == 0) or (heads > 1 and t.stride(1) == 0)))):
+        _fault(t, name, device, dtype, f"[at least {count} tokens, {heads} key heads, {dim} channels]", "contiguous channels")
 
 
 def cache4_append(k, v, pool, positions, token_seq, ctx_len, table, table_len, *, n_tokens):
     """Files the new tokens' keys and values in a layer's 4-bit pages.
 
-    k, v: [tokens, key heads, head_dim], views of the step's projections (any strides but the channels'); pool: uint8 [pages, key
-    heads, cache4_record_bytes(head_dim)].  Every 32 channels share a scale of one byte; a value becomes the nearest of the multiples
-    -7 to 7 of it (csrc/cache4.cuh, csrc/cache4.cu).  Where the pages come round (`table_len` pages hold less than a sequence), only the
-    positions they still hold after the step are written; `ctx_len`: the sequences' lengths after the step.  The step's positions
-    must differ from one another within a sequence, and no two sequences of a step may share a page that it writes."""
-    rows = [*_cache4_heads(k, "k"), *_cache4_heads(v, "v", k)]
-    _cache4_pool(pool, k.shape[1], k.shape[2], table, table_len, 0)
-    _enough(k, "k", n_tokens)
-    _enough(v, "v", n_tokens)
-    for t, name in ((positions, "positions"), (token_seq, "token_seq"), (ctx_len, "ctx_len")):
-        _need(t, name, torch.int32, (None,))
-    _enough(positions, "positions", n_tokens)
-    _enough(token_seq, "token_seq", n_tokens)
-    _together(k, v, pool, positions, token_seq, ctx_len, table)
-    elements = 2 * n_tokens * k.shape[1] * k.shape[2]
-    _work(0.0, elements * (k.element_size() + 17 / 32))
+    k, v: [tokens, key heads, head_dim], bfloat16 or 32-bit views of the step's projections (any strides but the channels'); pool:
+    uint8 [pages, key heads, cache4_record_bytes(head_dim)].  Every 32 channels share a scale of one byte; a value becomes the nearest
+    of the multiples -7 to 7 of it (csrc/cache4.cuh, csrc/cache4.cu).  Where the pages come round (`table_len` pages hold less than a
+    sequence), only the positions they still hold after the step are written; `ctx_len`: the sequences' lengths after the step.  The
+    step's positions must differ from one another within a sequence, and no two sequences of a step may share a page that it writes.
+    A token whose sequence, position or page lies outside the table or the pool is not filed; `check_status` reports it."""
+    code = _element_code(k, "k")
+    device = torch.cuda.current_device()
+    if n_tokens < 0 or k.dim() != 3:
+        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(k.shape)}")
+    heads, dim = k.shape[1], k.shape[2]
+    _cache4_pages(pool, table, table_len, device, heads, dim, 0)
+    _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim)
+    _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim)
+    at, seq = _int_list(positions, "positions", device, n_tokens), _int_list(token_seq, "token_seq", device, n_tokens)
+    length = _int_list(ctx_len, "ctx_len", device, 0)
+    if _PROFILE is not None:
+        _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
     _check(library().bt_cache4_append(
-        _ptr(k), rows[0], rows[1], _ptr(v), rows[2], rows[3], _ptr(pool), c_longlong(pool.shape[0]), _ptr(positions), _ptr(token_seq),
-        _ptr(ctx_len), _ptr(table), c_int(min(table.shape[0], ctx_len.shape[0])), c_int(table.shape[1]), c_int(table_len),
-        _ptr(kernel_status(k.device)), c_int(n_tokens), c_int(k.shape[1]), c_int(k.shape[2]), c_int(DTYPE_CODE[k.dtype]), _stream()))
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), pool.data_ptr(), pool.shape[0], at, seq, length,
+        table.data_ptr(), min(table.shape[0], ctx_len.shape[0]), table.shape[1], table_len, _status_address(device), n_tokens, heads, dim,
+        code, _raw_stream(device)))
 
 
 def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_tokens):
     """What a layer's 4-bit pages hold for `n_tokens` (sequence, position) pairs, as the values the codes stand for: into the rows
-    k and v, [tokens, key heads, head_dim] (any strides but the channels'), 32-bit or bfloat16, exact in both."""
-    rows = [*_cache4_heads(k, "k"), *_cache4_heads(v, "v", k)]
-    _cache4_pool(pool, k.shape[1], k.shape[2], table, table_len, 0)
-    _enough(k, "k", n_tokens)
-    _enough(v, "v", n_tokens)
-    for t, name in ((positions, "positions"), (token_seq, "token_seq")):
-        _need(t, name, torch.int32, (None,))
-        _enough(t, name, n_tokens)
-    _together(k, v, pool, positions, token_seq, table)
-    elements = 2 * n_tokens * k.shape[1] * k.shape[2]
-    _work(0.0, elements * (k.element_size() + 17 / 32))
+    k and v, [tokens, key heads, head_dim] (any strides but the channels'), 32-bit or bfloat16, exact in both.  A pair outside the table
+    or the pool yields NaN, and `check_status` reports it."""
+    code = _element_code(k, "k")
+    device = torch.cuda.current_device()
+    if n_tokens < 0 or k.dim() != 3:
+        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(k.shape)}")
+    heads, dim = k.shape[1], k.shape[2]
+    _cache4_pages(pool, table, table_len, device, heads, dim, 0)
+    _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim, True)
+    _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim, True)
+    at, seq = _int_list(positions, "positions", device, n_tokens), _int_list(token_seq, "token_seq", device, n_tokens)
+    if _PROFILE is not None:
+        _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
     _check(library().bt_cache4_gather(
-        _ptr(k), rows[0], rows[1], _ptr(v), rows[2], rows[3], _ptr(pool), c_longlong(pool.shape[0]), _ptr(positions), _ptr(token_seq),
-        _ptr(table), c_int(table.shape[0]), c_int(table.shape[1]), c_int(table_len), _ptr(kernel_status(k.device)), c_int(n_tokens),
-        c_int(k.shape[1]), c_int(k.shape[2]), c_int(DTYPE_CODE[k.dtype]), _stream()))
-
-
-def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
-    """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
-
-    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, blocks of 8 or 16 of them."""
-    columns = max_new * (n_heads // n_kv_heads)
-    if head_dim not in (64, 128) or columns > 16:
-        return "any", 1, 0
-    wide = 8 if columns <= 8 else 16
-    units = max(1, n_seqs * n_kv_heads)
-    span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
-    pages = max(1, -(-span // PAGE_SIZE))
-    # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
-    splits = max(1, min(-(-6 * _sm_count() // units), -(-pages // 4)))
-    return "few", splits, units * splits * wide * (head_dim + 2) if splits > 1 else 0
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), pool.data_ptr(), pool.shape[0], at, seq,
+        table.data_ptr(), table.shape[0], table.shape[1], table_len, _status_address(device), n_tokens, heads, dim, code, _raw_stream(device)))
 
 
 _SM_COUNTS: dict = {}
@@ -2093,10 +2119,33 @@ def _sm_count() -> int:
     return _SM_COUNTS[device]
 
 
-def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window=0, keep_first=0) -> int:
-    """32-bit words of `scratch` that cache4_attention wants for a step of these sizes."""
+def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
+    """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
+
+    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, blocks of 8 or 16 of them."""
+    columns = max_new * (n_heads // n_kv_heads)
+    if (head_dim != 64 and head_dim != 128) or columns > 16:
+        return "any", 1, 0
+    wide = 8 if columns <= 8 else 16
+    units = max(1, n_seqs * n_kv_heads)
+    span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
+    pages = max(1, -(-span // PAGE_SIZE))
+    # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
+    splits = max(1, min(-(-6 * _sm_count() // units), -(-pages // 4)))
+    return "few", splits, units * splits * wide * (head_dim + 2) if splits > 1 else 0
+
+
+def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
     if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise ShapeError(f"cache4_attention: {n_heads} query heads cannot share {n_kv_heads} key heads")
+    if min(n_tokens, n_seqs, max_new, max_ctx, window, keep_first) < 0:
+        raise ShapeError(f"cache4_attention: {n_tokens} tokens of {n_seqs} sequences, {max_new} new at most, context {max_ctx}, window {window}, "
+                         f"kept positions {keep_first}: none may be negative")
+
+
+def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window=0, keep_first=0) -> int:
+    """32-bit words of `scratch` that cache4_attention wants for a step of these sizes."""
+    _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
     return _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)[2]
 
 
@@ -2108,44 +2157,37 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     the same type.  Sequence s brings the tokens seq_start[s] .. seq_start[s + 1] behind past_len[s] others, at most `max_new` of
     them, and is no longer than `max_ctx` after the step.  A query at position p sees the keys j <= p with j > p - window (`window`
     0: all) or j < keep_first.  Rows of `out` behind the last sequence stay as they are.  Where the pages come round, what a query
-    sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0.  `scratch`: 32-bit, cache4_attention_scratch_floats of the same
-    sizes (more does no harm); two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that takes
-    every case."""
-    if q.dtype not in DTYPE_CODE:
-        raise ShapeError(f"cache4_attention: unsupported element type {q.dtype}")
-    if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
-        raise ShapeError(f"cache4_attention: {n_heads} query heads cannot share {n_kv_heads} key heads")
-    if window < 0 or keep_first < 0 or max_new < 0 or n_seqs < 0:
-        raise ShapeError(f"cache4_attention: window {window}, kept positions {keep_first}, {max_new} new tokens of {n_seqs} sequences")
+    sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0.  `scratch`: 32-bit, cache4_attention_scratch_floats
+    of the same sizes (more does no harm); two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that
+    takes every case.  A page outside the pool is reported by `check_status`, as is a kernel that gave up waiting."""
+    code = _element_code(q, "q")
+    _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
+    device = torch.cuda.current_device()
     width = n_heads * head_dim
-    row = _rows_view(q, "q", width, q.dtype)
-    _need(out, "out", q.dtype, (None, width))
-    _enough(q, "q", n_tokens)
-    _enough(out, "out", n_tokens)
-    _cache4_pool(pool, n_kv_heads, head_dim, table, table_len, n_seqs)
-    _need(seq_start, "seq_start", torch.int32, (None,))
-    _need(past_len, "past_len", torch.int32, (None,))
-    _enough(seq_start, "seq_start", n_seqs + 1)
-    _enough(past_len, "past_len", n_seqs)
+    _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs)
+    row = _row_stride(q, "q", device, q.dtype, n_tokens, width)
+    if not (isinstance(out, torch.Tensor) and out.dtype is q.dtype and out.get_device() == device and out.dim() == 2 and out.shape[1] == width
+            and out.shape[0] >= n_tokens and out.is_contiguous()):
+        _fault(out, "out", device, q.dtype, f"[at least {n_tokens}, {width}]")
+    starts, pasts = _int_list(seq_start, "seq_start", device, n_seqs + 1), _int_list(past_len, "past_len", device, n_seqs)
     if max_ctx > table_len * PAGE_SIZE and (keep_first or not window or table_len * PAGE_SIZE < window + max_new - 1):
         raise ShapeError(f"cache4_attention: {table_len} pages that come round do not hold what queries of a context of {max_ctx} see "
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
-    _together(q, out, pool, table, seq_start, past_len, scratch)
+    if impl not in (None, "any"):
+        raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
     kind, splits, floats = "any", 1, 0
-    if impl != "any" and q.dtype is torch.bfloat16 and q.data_ptr() % 16 == 0 and row % 8 == 0:
+    if impl is None and code == 1 and q.data_ptr() % 16 == 0 and row % 8 == 0:
         kind, splits, floats = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
+    partial = 0
     if floats:
         if scratch is None:
             raise ShapeError(f"cache4_attention: a step of these sizes needs {floats} floats of scratch")
-        _need(scratch, "scratch", torch.float32, (None,))
-        _enough(scratch, "scratch", floats)
+        partial = _float_list(scratch, "scratch", device, floats)
+    if _PROFILE is not None:
+        _work()
+    head = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
+            _status_address(device), starts, pasts, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, window, keep_first)
     if kind == "few":
-        _check(library().bt_cache4_decode(
-            _ptr(q), c_longlong(row), _ptr(out), _ptr(pool), c_longlong(pool.shape[0]), _ptr(table), c_int(table.shape[1]), c_int(table_len),
-            _ptr(kernel_status(q.device)), _ptr(seq_start), _ptr(past_len), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads),
-            c_int(head_dim), c_float(scale), c_int(window), c_int(keep_first), c_int(splits), _ptr(scratch), c_longlong(floats), _stream()))
-        return
-    _check(library().bt_cache4_attention(
-        _ptr(q), c_longlong(row), _ptr(out), _ptr(pool), c_longlong(pool.shape[0]), _ptr(table), c_int(table.shape[1]), c_int(table_len),
-        _ptr(kernel_status(q.device)), _ptr(seq_start), _ptr(past_len), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads),
-        c_int(head_dim), c_float(scale), c_int(window), c_int(keep_first), c_int(DTYPE_CODE[q.dtype]), _stream()))
+        _check(library().bt_cache4_decode(*head, splits, partial, floats, _raw_stream(device)))
+    else:
+        _check(library().bt_cache4_attention(*head, code, _raw_stream(device)))
