@@ -8,9 +8,9 @@
 //                 that order once;
 //   O^T = V^T P^T a lane takes the same bytes of two keys and pairs their nibbles; the rows of a score tile are keys in such an order
 //                 that the weights, transposed by movmatrix, meet their keys' values.
-// A code n becomes the bfloat16 128 + n by setting the exponent's bits (a shift and one logical operation for two codes), and (128 + n) s
-// - 136 s in one multiply-add for two is the value itself, exactly: 136 s has 8 significant bits.  Maximum, sum and products are 32-bit; the
-// weights are rounded to bfloat16 for the second product, as the other attention kernels of this library do.
+// Two codes become their bfloat16 values by a shift, a logical operation and a multiply-add (cache4_codes.cuh), without rounding.
+// Maximum, sum and products are 32-bit; the weights are rounded to bfloat16 for the second product, as the other attention kernels of
+// this library do.
 //
 // What bounds it: the integer pipe, which takes the codes apart (about 7 operations a key and key head of 128 channels and warp), close
 // to the memory behind it (136 bytes).  The run is cut into `n_splits` pieces where sequences and heads do not fill the GPU; their
@@ -18,6 +18,7 @@
 // Keys that a column does not see get the weight 0 exactly, and what lies in a page past the sequence's end (any bytes) is never
 // multiplied; a value filed as NaN reaches the columns that see its key and no other.
 #include "cache4.cuh"
+#include "cache4_codes.cuh"
 #include "decode_mma.cuh"
 
 namespace bt {
@@ -42,22 +43,6 @@ constexpr int c4d_slots() { return HD == 128 ? 2 : 3; }
 template <int HD, int NT>
 constexpr size_t c4d_smem() { return (size_t)C4D_WARPS * c4d_slots<HD>() * c4_record(HD); }
 
-// Two codes as bfloat16 128 + n: nibble `I` of both halves of `w`.
-template <int I>
-__device__ __forceinline__ unsigned c4d_pair(unsigned w) {
-  return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
-}
-__device__ __forceinline__ unsigned c4d_fma2(unsigned a, unsigned b, unsigned c) {
-  unsigned d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// A scale byte's bfloat16 bits (low half).
-__device__ __forceinline__ unsigned c4d_scale(unsigned b) { return b == 255u ? 0x7fc0u : b * 16u + 0x3580u; }
-__device__ __forceinline__ unsigned c4d_shift(unsigned s2) {
-  const unsigned c = 0xc308c308u;      // -136 in both halves
-  return c4d_fma2(s2, c, 0x80008000u);
-}
 __device__ __forceinline__ unsigned c4d_transpose(unsigned v) {
   unsigned d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
@@ -193,19 +178,19 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
           const uint2 v = *reinterpret_cast<const uint2*>(row);
           w[h][0] = v.x; w[h][1] = v.y;
         }
-        const unsigned b = c4d_scale(rec[c4_key_scales(HD) + key * G + q * G / 4]);
+        const unsigned b = c4_scale_bits(rec[c4_key_scales(HD) + key * G + q * G / 4]);
         s2[h] = b | b << 16;
-        sh[h] = c4d_shift(s2[h]);
+        sh[h] = c4_shift(s2[h]);
       }
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         unsigned x[2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x[h][0] = c4d_fma2(c4d_pair<0>(w[h][k]), s2[h], sh[h]);
-          x[h][1] = c4d_fma2(c4d_pair<1>(w[h][k]), s2[h], sh[h]);
-          x[h][2] = c4d_fma2(c4d_pair<2>(w[h][k]), s2[h], sh[h]);
-          x[h][3] = c4d_fma2(c4d_pair<3>(w[h][k]), s2[h], sh[h]);
+          x[h][0] = c4_fma2(c4_pair<0>(w[h][k]), s2[h], sh[h]);
+          x[h][1] = c4_fma2(c4_pair<1>(w[h][k]), s2[h], sh[h]);
+          x[h][2] = c4_fma2(c4_pair<2>(w[h][k]), s2[h], sh[h]);
+          x[h][3] = c4_fma2(c4_pair<3>(w[h][k]), s2[h], sh[h]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -284,21 +269,21 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
         }
       }
       const unsigned s01 = b[0] | b[1] << 16, s23 = b[2] | b[3] << 16;
-      const unsigned h01 = c4d_shift(s01), h23 = c4d_shift(s23);
+      const unsigned h01 = c4_shift(s01), h23 = c4_shift(s23);
 #pragma unroll
       for (int k = 0; k < VW; ++k)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const unsigned a = __byte_perm(w[0][k], w[1][k], half ? 0x7632 : 0x5410), d = __byte_perm(w[2][k], w[3][k], half ? 0x7632 : 0x5410);
           unsigned x[4], y[4];
-          x[0] = c4d_fma2(c4d_pair<0>(a), s01, h01);
-          x[1] = c4d_fma2(c4d_pair<1>(a), s01, h01);
-          x[2] = c4d_fma2(c4d_pair<2>(a), s01, h01);
-          x[3] = c4d_fma2(c4d_pair<3>(a), s01, h01);
-          y[0] = c4d_fma2(c4d_pair<0>(d), s23, h23);
-          y[1] = c4d_fma2(c4d_pair<1>(d), s23, h23);
-          y[2] = c4d_fma2(c4d_pair<2>(d), s23, h23);
-          y[3] = c4d_fma2(c4d_pair<3>(d), s23, h23);
+          x[0] = c4_fma2(c4_pair<0>(a), s01, h01);
+          x[1] = c4_fma2(c4_pair<1>(a), s01, h01);
+          x[2] = c4_fma2(c4_pair<2>(a), s01, h01);
+          x[3] = c4_fma2(c4_pair<3>(a), s01, h01);
+          y[0] = c4_fma2(c4_pair<0>(d), s23, h23);
+          y[1] = c4_fma2(c4_pair<1>(d), s23, h23);
+          y[2] = c4_fma2(c4_pair<2>(d), s23, h23);
+          y[3] = c4_fma2(c4_pair<3>(d), s23, h23);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             ds_mma(acc[n][4 * k + 2 * half], x[0], x[1], y[0], y[1], pt[n][t][0], pt[n][t][1]);

@@ -1,0 +1,520 @@
+// Attention over a 4-bit cache (cache4.cuh) for steps that bring many tokens a sequence, on the fifth-generation tensor cores:
+// bfloat16 queries, heads of 64 or 128 channels.
+//
+// A block serves one (sequence, key head) and 256 rows: row r is query head r % group of new token r / group, so that heads which
+// share a key head share its keys, however many new tokens there are.  The rows are two tiles of 128 (rows of the tensor memory), and the
+// visible keys go by in tiles of 128.  Four warpgroups:
+//   0, 1  softmax, a thread a row of tile 0 or 1: scores from tensor memory into registers, running maximum and sum in 32-bit, weights
+//         as bfloat16 back into tensor memory, from where P V takes them.  The output accumulates there and is rescaled only when a
+//         row's maximum has outgrown the one its weights are formed with by more than 2^8;
+//   2     takes the codes apart: a lane reads 16 bytes (32 channels, one scale) of the next tile's keys and values ahead, turns them into
+//         the exact bfloat16 values (cache4_decode.cu says how) and stores them where the products read them.  A word of eight codes
+//         leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers are renamed;
+//   3     one warp issues S = Q K^T and O += P V of both tiles in turn: while one tile's products run the other's weights are formed.
+// Keys and values are taken apart once for both tiles.  With heads of 128 channels the weights lie over the scores they were made of
+// (the tensor memory is full), so that a tile's next scores wait for its last product; heads of 64 have room for both.
+// Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of tiles, whose results a second kernel joins in order.
+//
+// Masked keys get the weight 0 exactly.  A value filed as NaN reaches the rows that see its key and no other: in a tile that every row
+// of the block sees it is multiplied as it is; in the few others (seven at most: the diagonal's three, as many at the window's far edge,
+// the last kept one) it is multiplied as 0 and noted, and the rows look at the notes at the end.
+// All hand-overs go through mbarriers; every wait is bounded, and one that runs out sets the status word.
+#include "attention_tcgen05.cuh"
+#include "cache4.cuh"
+#include "cache4_codes.cuh"
+
+namespace bt {
+
+constexpr int C4P_THREADS = 512;
+constexpr int C4P_ROWS = 256;
+constexpr int C4P_EDGES = 8;            // tiles that not every row of a block sees: at most 7
+
+struct Cache4PromptParams {
+  const __nv_bfloat16* q;
+  long long q_row;
+  __nv_bfloat16* out;
+  const int *seq_start, *past_len;
+  int n_heads, group;
+  float scale_log2;
+  int window, keep_first;
+  float* part;                 // [unit][split][256][HD], then [unit][split][256][2]
+  long long part_ml;
+};
+
+template <int HD>
+struct C4pShape {
+  static constexpr int TILE = HD / 64 * 2 * TA_BOX_BYTES;        // 128 rows of a head
+  static constexpr size_t SMEM = (size_t)6 * TILE;               // two tiles of queries, two stages of keys and of values
+  static constexpr bool OVER = 2 * (TA_BK + HD + 64) > 512;      // the weights lie over the scores
+};
+
+// The tiles of keys that a block's rows see, and how they are cut: the same for the attention and the kernel that joins.
+struct C4pRun {
+  int past, pos_first, pos_last, kept_only, kt_lo, n_tiles, per;
+  __device__ C4pRun(int past_, int n_new, int row0, int group, int window, int keep_first, int n_splits) : past(past_) {
+    pos_first = past + row0 / group;
+    pos_last = past + min(n_new * group - 1, row0 + C4P_ROWS - 1) / group;
+    const int lo = window > 0 ? max(0, pos_first - window + 1) : 0;
+    kt_lo = lo / TA_BK;
+    kept_only = window > 0 ? min((min(keep_first, pos_last + 1) + TA_BK - 1) / TA_BK, kt_lo) : 0;
+    n_tiles = kept_only + pos_last / TA_BK - kt_lo + 1;
+    per = (n_tiles + n_splits - 1) / n_splits;
+  }
+  __device__ int tile_at(int i) const { return i < kept_only ? i : kt_lo + (i - kept_only); }
+};
+
+__device__ __forceinline__ void c4p_bar_arrive_warp(unsigned long long* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) ta_bar_arrive(bar);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(C4P_THREADS, 1)
+cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
+  using Shape = C4pShape<HD>;
+  constexpr int TILE = Shape::TILE, CH = HD / 32;
+  constexpr bool OVER = Shape::OVER;
+  extern __shared__ __align__(1024) unsigned char c4p_raw[];
+  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ unsigned s_nan[C4P_EDGES][CH][4];      // a bit a key of a tile that not every row sees
+  __shared__ int s_edge_key[C4P_EDGES], s_edges;
+  __shared__ unsigned s_tmem;
+  __shared__ int s_failed;
+  unsigned char *Qs = c4p_raw, *Ks = Qs + 2 * TILE, *Vs = Ks + 2 * TILE;
+  unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // [stage]
+  unsigned long long *s_full = bars + 8, *p_ready = bars + 10, *o_done = bars + 12;                     // [tile of rows], one phase a tile of keys
+
+  const int kv_head = (int)blockIdx.x % c.n_kv_heads, seq = (int)blockIdx.x / c.n_kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  pdl_trigger();
+  pdl_wait();
+  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * C4P_ROWS;      // (the longest blocks first)
+  const int n_rows = min(C4P_ROWS, n_new * p.group - row0);
+  if (n_rows <= 0) return;
+  const C4pRun run(p.past_len[seq], n_new, row0, p.group, p.window, p.keep_first, (int)gridDim.z);
+  const int it0 = (int)blockIdx.z * run.per, n_tiles = min(run.n_tiles, it0 + run.per) - it0;
+  if (n_tiles <= 0) return;
+  if ((ta_smem(c4p_raw) & 1023u) != 0) {      // the swizzled layouts need the alignment: refuse rather than compute nonsense
+    if (tid == 0 && c.status) atomicExch(c.status, 10);
+    return;
+  }
+  const int n_sub = n_rows > TA_BQ ? 2 : 1;      // tiles of rows
+
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      ta_bar_init(&k_full[s], 4);
+      ta_bar_init(&k_empty[s], 1);
+      ta_bar_init(&v_full[s], 4);
+      ta_bar_init(&v_empty[s], 1);
+      ta_bar_init(&s_full[s], 1);
+      ta_bar_init(&p_ready[s], 4);
+      ta_bar_init(&o_done[s], 1);
+    }
+    s_failed = 0;
+    s_edges = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (tid < C4P_EDGES * CH * 4) (&s_nan[0][0][0])[tid] = 0u;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(ta_smem(&s_tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  // queries: 16-byte pieces of 8 channels, into the order in which codes leave a word; rows past the last are zero
+  for (int i = tid; i < n_sub * TA_BQ * (HD / 8); i += C4P_THREADS) {
+    const int r = i / (HD / 8), piece = i % (HD / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < n_rows) {
+      const int token = (row0 + r) / p.group, head = kv_head * p.group + (row0 + r) % p.group;
+      v = *reinterpret_cast<const uint4*>(p.q + (t0 + token) * p.q_row + (long long)head * HD + piece * 8);
+    }
+    const uint4 w = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                               __byte_perm(v.y, v.w, 0x7632));
+    unsigned char* dst = Qs + r / TA_BQ * TILE + piece / 8 * (2 * TA_BOX_BYTES) + r % TA_BQ * 128;
+    *reinterpret_cast<uint4*>(dst + (((piece & 7) ^ (r & 7)) << 4)) = w;
+  }
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  ta_fence_before();
+  __syncthreads();
+  ta_fence_after();
+  const unsigned tmem = s_tmem, tmem_o = tmem + 2 * TA_BK;      // S of both tiles, O of both, (P of both)
+  auto tmem_p = [&](int sub) { return OVER ? tmem + (unsigned)(sub * TA_BK) : tmem_o + (unsigned)(2 * HD + sub * 64); };
+
+  // registers: 512 threads x 128 at launch; 2 x 128 x 176 + 2 x 128 x 80 is the same
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
+    // ---- softmax: a thread a row; warp w reaches the lanes of quarter w % 4 ----
+    const int sub = warp >> 2, r = (warp & 3) * 32 + lane;
+    if (sub < n_sub) {
+      const int row = min(row0 + sub * TA_BQ + r, n_new * p.group - 1), pos = run.past + row / p.group;
+      const int at_first = run.past + (row0 + sub * TA_BQ) / p.group;
+      const int at_last = run.past + min(n_new * p.group - 1, row0 + sub * TA_BQ + TA_BQ - 1) / p.group;
+      const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+      const unsigned my_s = tmem + (unsigned)(sub * TA_BK) + lanes, my_o = tmem_o + (unsigned)(sub * HD) + lanes, my_p = tmem_p(sub) + lanes;
+      const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+      float m = -INFINITY, l = 0.f;      // the reference maximum (base 2, scaled) and the sum of weights formed with it
+      bool ok = true;
+#pragma unroll 1
+      for (int it = 0; it < n_tiles; ++it) {
+        const int key0 = run.tile_at(it0 + it) * TA_BK;
+        ok = __all_sync(0xffffffffu, ta_bar_wait(&s_full[sub], it & 1));
+        if (!ok) break;                  // (uniform in the warp; the others run into their own bounds)
+        ta_fence_after();
+        unsigned a[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ta_ld32_issue(my_s + 32u * q, a[q]);
+        ta_ld_wait(a[0], a[1]);
+        ta_ld_wait(a[2], a[3]);
+        // from here on the largest score has the largest weight
+        if (p.scale_log2 <= 0.f) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) a[q][i] = p.scale_log2 < 0.f ? a[q][i] ^ 0x80000000u : __float_as_uint(__uint_as_float(a[q][i]) * 0.f);
+        }
+        const bool whole = key0 + TA_BK - 1 <= at_first && (p.window <= 0 || key0 > at_last - p.window || key0 + TA_BK <= p.keep_first);
+        if (!whole) {                    // a bit a key
+          const int lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) - key0, hi = pos - key0;
+          const int kept = p.window > 0 ? min(p.keep_first, pos + 1) - key0 : 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int first = lo - 32 * q, last = hi - 32 * q, below = kept - 32 * q;
+            unsigned seen = last >= 31 ? 0xffffffffu : last < 0 ? 0u : (2u << last) - 1u;
+            seen &= first <= 0 ? 0xffffffffu : first > 31 ? 0u : 0xffffffffu << first;
+            seen |= below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) a[q][i] = (seen >> i) & 1u ? a[q][i] : __float_as_uint(-INFINITY);
+          }
+        }
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains side by side)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t4[q] = ta_max3(t4[q], __uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1]));
+        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * scale;
+        if (it > 0) {                    // (the product before still reads its weights and adds to O)
+          ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[sub], (it - 1) & 1));
+          if (!ok) break;
+          ta_fence_after();
+        }
+        const bool grown = top > m + TS_GROWTH || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, grown)) {
+          const float m_new = grown ? top : m;
+          const float alpha = grown ? ta_exp2(m - m_new) : 1.f;      // 0 for a row that had seen nothing yet
+          l *= alpha;
+          m = m_new;
+          if (it > 0) {
+#pragma unroll 1
+            for (int q = 0; q < HD; q += 32) {
+              unsigned o[32];
+              ta_ld32_issue(my_o + (unsigned)q, o);
+              ta_ld_wait1(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              ta_st32(my_o + (unsigned)q, o);
+            }
+          }
+        }
+        const float m_use = m == -INFINITY ? 0.f : m;
+        const unsigned long long scale2 = ta_two(__float_as_uint(scale), __float_as_uint(scale));
+        const unsigned long long shift2 = ta_two(__float_as_uint(-m_use), __float_as_uint(-m_use));
+        unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          unsigned w[32];
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              unsigned x, y;
+              ta_halves(ta_fma2(ta_two(a[2 * h + q][i], a[2 * h + q][i + 1]), scale2, shift2), x, y);
+              x = __float_as_uint(ta_exp2(__uint_as_float(x)));
+              y = __float_as_uint(ta_exp2(__uint_as_float(y)));
+              sum[(i >> 1) & 3] = ta_add2(sum[(i >> 1) & 3], ta_two(x, y));
+              w[q * 16 + (i >> 1)] = ta_pack(__uint_as_float(x), __uint_as_float(y));
+            }
+          ta_st32(my_p + 32u * h, w);
+        }
+        {
+          unsigned x, y;
+          ta_halves(ta_add2(ta_add2(sum[0], sum[1]), ta_add2(sum[2], sum[3])), x, y);
+          l += __uint_as_float(x) + __uint_as_float(y);
+        }
+        ta_st_wait();
+        ta_fence_before();
+        c4p_bar_arrive_warp(&p_ready[sub], lane);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[sub], (n_tiles - 1) & 1));
+      ta_fence_after();
+      if (!ok) {
+        s_failed = 1;
+      } else {
+        // channels whose values are NaN for a key that this row sees in a tile that others do not
+        unsigned lost = 0;
+        const int edges = *(volatile int*)&s_edges;
+        for (int e = 0; e < edges; ++e) {
+          const int key0 = s_edge_key[e];
+          for (int j = 0; j < CH * 4; ++j) {
+            unsigned bits = s_nan[e][j >> 2][j & 3];
+            while (bits) {
+              const int key = key0 + 32 * (j & 3) + __ffs(bits) - 1;
+              bits &= bits - 1;
+              if (key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first)) lost |= 1u << (j >> 2);
+            }
+          }
+        }
+        const bool mine = sub * TA_BQ + r < n_rows;
+        const bool cut = gridDim.z > 1;
+        const float inv = cut ? 1.f : 1.f / l;
+        const int token = row / p.group, head = kv_head * p.group + row % p.group;
+        __nv_bfloat16* dst = p.out + ((long long)(t0 + token) * p.n_heads + head) * HD;
+        const long long unit = (((long long)blockIdx.x * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * C4P_ROWS + sub * TA_BQ + r;
+        float* part = p.part + unit * HD;
+#pragma unroll 1
+        for (int q = 0; q < CH; ++q) {
+          unsigned raw[32];
+          ta_ld32_issue(my_o + 32u * q, raw);
+          ta_ld_wait1(raw);
+          if (!mine) continue;
+          const float f = (lost >> q) & 1u ? NAN : inv;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {      // columns 0 .. 7 are the channels 0 4 1 5 2 6 3 7
+            float o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(raw[i + (j < 4 ? 2 * j : 2 * j - 7)]) * f;
+            if (cut) {
+              reinterpret_cast<float4*>(part + 32 * q + i)[0] = make_float4(o[0], o[1], o[2], o[3]);
+              reinterpret_cast<float4*>(part + 32 * q + i)[1] = make_float4(o[4], o[5], o[6], o[7]);
+            } else {
+              *reinterpret_cast<uint4*>(dst + 32 * q + i) =
+                  make_uint4(ta_pack(o[0], o[1]), ta_pack(o[2], o[3]), ta_pack(o[4], o[5]), ta_pack(o[6], o[7]));
+            }
+          }
+        }
+        if (cut && mine) {
+          p.part[p.part_ml + 2 * unit] = m;
+          p.part[p.part_ml + 2 * unit + 1] = l;
+        }
+      }
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    // ---- takes the codes apart ----
+    // a warp's 32 lanes read 16 bytes each of 8 (16) rows in a row; eight lanes of a store cover eight rows' same piece
+    constexpr int SPAN = 32 / CH;        // rows of a warp's read
+    const int dw = warp - 8, chunk = (lane >> 3) % CH, sub_row = (lane & 7) + 8 * ((lane >> 3) / CH);
+    uint4 raw[CH];
+    unsigned sc[CH];
+    // the row j of this lane in a tile: SPAN (4 j + dw) + sub_row
+    auto fetch = [&](int it, bool values) {
+      const int key0 = run.tile_at(it0 + it) * TA_BK;
+      // (a half tile past the last key that a row sees repeats the last page: masked, and NaN there is nobody's)
+      const unsigned char* rec0 = c4_page(c, seq, key0 / C4_PAGE, kv_head, HD);
+      const unsigned char* rec1 = c4_page(c, seq, min(key0 + C4_PAGE, run.pos_last) / C4_PAGE, kv_head, HD);
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const int r = SPAN * (4 * j + dw) + sub_row;
+        const unsigned char* rec = r < C4_PAGE ? rec0 : rec1;
+        raw[j] = *reinterpret_cast<const uint4*>(rec + (values ? c4_value_codes(HD) : 0) + (r % C4_PAGE) * (HD / 2) + chunk * 16);
+        sc[j] = rec[(values ? c4_value_scales(HD) : c4_key_scales(HD)) + (r % C4_PAGE) * CH + chunk];
+      }
+    };
+    auto place = [&](unsigned char* tile, bool values, bool whole, int edge) {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const int r = SPAN * (4 * j + dw) + sub_row;
+        unsigned s = c4_scale_bits(sc[j]);
+        if (values && !whole && sc[j] == 255u) {
+          s = 0u;
+          atomicOr(&s_nan[edge][chunk][r >> 5], 1u << (r & 31));
+        }
+        const unsigned s2 = s | s << 16, shift = c4_shift(s2);
+        unsigned char* dst = tile + chunk / 2 * (2 * TA_BOX_BYTES) + r * 128;
+        const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k]), s2, shift), c4_fma2(c4_pair<1>(w[k]), s2, shift),
+                                     c4_fma2(c4_pair<2>(w[k]), s2, shift), c4_fma2(c4_pair<3>(w[k]), s2, shift));
+          *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    };
+    uint4 ahead[CH];                     // the values' codes, while the keys' are in `raw`, and the other way round
+    unsigned ahead_sc[CH];
+    auto swap = [&] {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const uint4 x = raw[j];
+        const unsigned y = sc[j];
+        raw[j] = ahead[j];
+        sc[j] = ahead_sc[j];
+        ahead[j] = x;
+        ahead_sc[j] = y;
+      }
+    };
+    int edges = 0;
+    bool ok = true;
+    fetch(0, true);
+    swap();
+    fetch(0, false);
+#pragma unroll 1
+    for (int it = 0; it < n_tiles && ok; ++it) {
+      const int s = it & 1, key0 = run.tile_at(it0 + it) * TA_BK;
+      const bool whole = key0 + TA_BK - 1 <= run.pos_first && (p.window <= 0 || key0 > run.pos_last - p.window || key0 + TA_BK <= p.keep_first);
+      const int edge = min(edges, C4P_EDGES - 1);
+      if (!whole) {
+        if (tid == 256) {
+          s_edge_key[edge] = key0;
+          *(volatile int*)&s_edges = edge + 1;
+        }
+        ++edges;
+      }
+      if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&k_empty[s], ((it >> 1) - 1) & 1));
+      if (!ok) break;
+      place(Ks + s * TILE, false, whole, edge);
+      c4p_bar_arrive_warp(&k_full[s], lane);
+      if (it + 1 < n_tiles) fetch(it + 1, false);
+      swap();
+      if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&v_empty[s], ((it >> 1) - 1) & 1));
+      if (!ok) break;
+      place(Vs + s * TILE, true, whole, edge);
+      c4p_bar_arrive_warp(&v_full[s], lane);
+      if (it + 1 < n_tiles) fetch(it + 1, true);
+      swap();
+    }
+    if (!ok) s_failed = 1;
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    if (warp == 12) {
+      // ---- issuer.  Instruction descriptors: 32-bit accumulator, bfloat16 operands, M = 128; S: N = 128, both K-major;
+      // P V: N = HD, the first operand in tensor memory, the second MN-major ----
+      const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TA_BK >> 3) << 17) | ((unsigned)(TA_BQ >> 4) << 24);
+      const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(HD >> 3) << 17) | ((unsigned)(TA_BQ >> 4) << 24);
+      const unsigned long long desc_q = ta_desc(Qs, 16), desc_k = ta_desc(Ks, 16), desc_v = ta_desc(Vs, 2 * TA_BOX_BYTES);
+      auto scores = [&](int it, int sub) {
+        const int s = it & 1;
+        if (ta_elect()) {
+          const unsigned long long dq = desc_q + (unsigned long long)(sub * (TILE >> 4)), dk = desc_k + (unsigned long long)(s * (TILE >> 4));
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {      // 16 channels: 32 bytes further along the row, a box further every 64
+            const unsigned long long step = (k / 4) * (2 * TA_BOX_BYTES >> 4) + 2 * (k % 4);
+            ta_mma(tmem + (unsigned)(sub * TA_BK), dq + step, dk + step, idesc_s, k > 0 ? 1u : 0u);
+          }
+          ta_commit(&s_full[sub]);
+          if (sub == n_sub - 1) ta_commit(&k_empty[s]);
+        }
+        __syncwarp();
+      };
+      bool ok = __all_sync(0xffffffffu, ta_bar_wait(&k_full[0], 0));
+      ta_fence_after();
+      for (int sub = 0; sub < n_sub && ok; ++sub) scores(0, sub);
+      for (int it = 0; it < n_tiles && ok; ++it) {
+        const int s = it & 1;
+        ok = __all_sync(0xffffffffu, ta_bar_wait(&v_full[s], (it >> 1) & 1));
+        for (int sub = 0; sub < n_sub && ok; ++sub) {
+          ok = __all_sync(0xffffffffu, ta_bar_wait(&p_ready[sub], it & 1));
+          if (!ok) break;
+          ta_fence_after();
+          if (ta_elect()) {
+            const unsigned long long dv = desc_v + (unsigned long long)(s * (TILE >> 4));
+#pragma unroll
+            for (int j = 0; j < TA_BK / 16; ++j)     // 16 keys further: 8 columns of P, 16 rows of V
+              ta_mma_tmem(tmem_o + (unsigned)(sub * HD), tmem_p(sub) + 8u * j, dv + (unsigned long long)(j * (16 * 128 >> 4)), idesc_o,
+                          (it > 0 || j > 0) ? 1u : 0u);
+            ta_commit(&o_done[sub]);
+            if (sub == n_sub - 1) ta_commit(&v_empty[s]);
+          }
+          __syncwarp();
+          if (it + 1 < n_tiles) {
+            if (sub == 0) ok = __all_sync(0xffffffffu, ta_bar_wait(&k_full[(it + 1) & 1], ((it + 1) >> 1) & 1));
+            if (OVER) ok = __all_sync(0xffffffffu, ok && ta_bar_wait(&o_done[sub], it & 1));      // (the weights lie where the scores go)
+            if (!ok) break;
+            ta_fence_after();
+            scores(it + 1, sub);
+          }
+        }
+      }
+      if (!ok && lane == 0) s_failed = 1;
+    }
+  }
+  ta_fence_before();
+  __syncthreads();
+  if (s_failed) let_copies_land();
+  if (warp == 12) {
+    ta_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+  }
+  if (tid == 0 && s_failed && c.status) atomicExch(c.status, 10);
+}
+
+// Joins the runs of keys of 256 rows in their order: a block a row, a thread a channel.
+template <int HD>
+__global__ void __launch_bounds__(HD)
+cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, int n_splits) {
+  pdl_trigger();
+  pdl_wait();
+  const int kv_head = (int)blockIdx.y % n_kv_heads, seq = (int)blockIdx.y / n_kv_heads;
+  const int tile = (int)blockIdx.x / C4P_ROWS, r = (int)blockIdx.x % C4P_ROWS, row0 = (row_tiles - 1 - tile) * C4P_ROWS, row = row0 + r;
+  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  if (row >= n_new * p.group) return;
+  const C4pRun run(p.past_len[seq], n_new, row0, p.group, p.window, p.keep_first, n_splits);
+  const int used = (run.n_tiles + run.per - 1) / run.per;
+  float top = -INFINITY, sum = 0.f, o = 0.f;
+  for (int s = 0; s < used; ++s) {
+    const long long unit = (((long long)blockIdx.y * row_tiles + tile) * n_splits + s) * C4P_ROWS + r;
+    const float m = p.part[p.part_ml + 2 * unit], l = p.part[p.part_ml + 2 * unit + 1], x = p.part[unit * HD + threadIdx.x];
+    const float m_new = fmaxf(top, m), use = m_new == -INFINITY ? 0.f : m_new;
+    const float a = ta_exp2(top - use), b = ta_exp2(m - use);
+    sum = sum * a + l * b;
+    o = o * a + x * b;
+    top = m_new;
+  }
+  const int token = row / p.group, head = kv_head * p.group + row % p.group;
+  p.out[((long long)(t0 + token) * p.n_heads + head) * HD + threadIdx.x] = __float2bfloat16_rn(o / sum);
+}
+
+template <int HD>
+static int launch_c4p(const Cache4PromptParams& p, const Cache4View& c, int n_seqs, int row_tiles, int n_splits, cudaStream_t stream) {
+  constexpr size_t smem = C4pShape<HD>::SMEM;
+  auto kern = cache4_prompt_kernel<HD>;
+  static SharedMemoryAllowance allowed;
+  BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
+  BT_PDL_OK("cache4_prompt", launch_pdl(kern, dim3(n_seqs * c.n_kv_heads, row_tiles, n_splits), dim3(C4P_THREADS), smem, stream, 1, p, c));
+  if (n_splits > 1)
+    BT_PDL_OK("cache4_prompt_join", launch_pdl(cache4_prompt_join_kernel<HD>, dim3(row_tiles * C4P_ROWS, n_seqs * c.n_kv_heads), dim3(HD), 0, stream,
+                                               1, p, c.n_kv_heads, row_tiles, n_splits));
+  return 0;
+}
+
+}  // namespace bt
+
+// Arguments as bt_cache4_attention (bfloat16).  scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * row tiles (of 256 rows:
+// max_new * (n_heads / n_kv_heads)) * splits * 256 * (dim + 2).
+extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
+                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
+                                int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
+                                float* scratch, long long scratch_floats, cudaStream_t stream) {
+  using namespace bt;
+  BT_CHECK(dim == 64 || dim == 128, "cache4_attention: the kernel for many tokens takes heads of 64 or 128 channels, not %d", dim);
+  BT_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "cache4_attention: %d query heads cannot share %d key heads", n_heads, n_kv_heads);
+  BT_CHECK(n_pages > 0 && table != nullptr && table_len > 0 && n_seqs >= 0 && max_new >= 0 && window >= 0 && keep_first >= 0,
+           "cache4_attention: bad sizes pages=%lld table_len=%d sequences=%d window=%d kept=%d", n_pages, table_len, n_seqs, window, keep_first);
+  auto at16 = [](const void* x) { return (unsigned long long)x % 16 == 0; };
+  BT_CHECK(at16(pool) && at16(q) && at16(out) && q_row % 8 == 0, "cache4_attention: pool, queries and results must lie on 16-byte boundaries");
+  if (n_seqs == 0 || max_new == 0) return 0;
+  const int group = n_heads / n_kv_heads;
+  BT_CHECK((long long)max_new * group < (1ll << 30), "cache4_attention: %d new tokens of %d heads are too many", max_new, group);
+  const int row_tiles = (int)(((long long)max_new * group + C4P_ROWS - 1) / C4P_ROWS);
+  const long long units = (long long)n_seqs * n_kv_heads;
+  BT_CHECK(units <= 65535 && row_tiles <= 65535 && n_splits >= 1 && n_splits <= 65535, "cache4_attention: grid too large (%lld sequences' heads, %d tiles of rows)",
+           units, row_tiles);
+  const long long parts = units * row_tiles * n_splits * C4P_ROWS;
+  BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
+           "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
+  const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group,
+                             scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
+  const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
+  if (dim == 64) return launch_c4p<64>(p, c, n_seqs, row_tiles, n_splits, stream);
+  return launch_c4p<128>(p, c, n_seqs, row_tiles, n_splits, stream);
+}

@@ -1936,6 +1936,7 @@ _ARGUMENTS = {
     "bt_cache4_gather": "pllpllplpppiiipiiiip",
     "bt_cache4_attention": "plpplpiipppiiiiifiiip",
     "bt_cache4_decode": "plpplpiipppiiiiifiiiplp",
+    "bt_cache4_prompt": "plpplpiipppiiiiifiiiplp",
 }
 
 
@@ -2122,17 +2123,20 @@ def _sm_count() -> int:
 def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
     """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
 
-    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, blocks of 8 or 16 of them."""
-    columns = max_new * (n_heads // n_kv_heads)
-    if (head_dim != 64 and head_dim != 128) or columns > 16:
+    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, in blocks of 8 or 16; "many": blocks of 256 of them."""
+    if head_dim != 64 and head_dim != 128:
         return "any", 1, 0
-    wide = 8 if columns <= 8 else 16
+    columns = max_new * (n_heads // n_kv_heads)
     units = max(1, n_seqs * n_kv_heads)
     span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
-    pages = max(1, -(-span // PAGE_SIZE))
-    # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
-    splits = max(1, min(-(-6 * _sm_count() // units), -(-pages // 4)))
-    return "few", splits, units * splits * wide * (head_dim + 2) if splits > 1 else 0
+    if columns <= 16:
+        # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
+        splits = max(1, min(-(-6 * _sm_count() // units), -(-span // (4 * PAGE_SIZE))))
+        return "few", splits, units * splits * (8 if columns <= 8 else 16) * (head_dim + 2) if splits > 1 else 0
+    tiles = -(-columns // 256)
+    # a block a multiprocessor; pieces of eight tiles of 128 keys at least
+    splits = max(1, min(_sm_count() // (units * tiles), -(-span // 1024)))
+    return "many", splits, units * tiles * splits * 256 * (head_dim + 2) if splits > 1 else 0
 
 
 def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
@@ -2176,7 +2180,7 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
     kind, splits, floats = "any", 1, 0
-    if impl is None and code == 1 and q.data_ptr() % 16 == 0 and row % 8 == 0:
+    if impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0:
         kind, splits, floats = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
     partial = 0
     if floats:
@@ -2189,5 +2193,7 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
             _status_address(device), starts, pasts, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, window, keep_first)
     if kind == "few":
         _check(library().bt_cache4_decode(*head, splits, partial, floats, _raw_stream(device)))
+    elif kind == "many":
+        _check(library().bt_cache4_prompt(*head, splits, partial, floats, _raw_stream(device)))
     else:
         _check(library().bt_cache4_attention(*head, code, _raw_stream(device)))
