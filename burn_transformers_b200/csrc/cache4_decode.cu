@@ -31,7 +31,7 @@ struct Cache4DecodeParams {
   long long q_row;
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
-  int n_heads, group, col_blocks;
+  int n_heads, group, col_blocks, max_new;
   float scale_log2;
   int window, keep_first;
   float* part;                 // [unit][split][columns][HD], then [unit][split][columns][2]
@@ -48,6 +48,16 @@ __device__ __forceinline__ unsigned c4d_transpose(unsigned v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
   return d;
 }
+
+__device__ __forceinline__ float c4d_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <bool V>
+struct C4dFlag {
+  static constexpr bool value = V;
+};
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(C4D_WARPS * 32, NT == 1 ? 3 : 2)
@@ -89,6 +99,9 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   __syncthreads();
   unsigned char* ring = c4d_raw + warp * SLOTS * REC;
   const int count = mine > warp ? (mine - warp + C4D_WARPS - 1) / C4D_WARPS : 0;      // this warp's pages: first + warp + 4 i
+  // records of this warp's next 32 pages, one a lane
+  auto record_of = [&](int i) { return c4_page(c, seq, page_at(first + warp + C4D_WARPS * min(i, count - 1)), kv_head, HD); };
+  const unsigned char* next = count > 0 ? record_of(lane) : nullptr;
   auto ask = [&](int i, const unsigned char* rec) {      // (one lane)
     const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]);
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((unsigned)REC) : "memory");
@@ -97,7 +110,7 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
                  "l"(rec), "r"((unsigned)REC), "r"(bar)
                  : "memory");
   };
-  if (lane < min(SLOTS, count)) ask(lane, c4_page(c, seq, page_at(first + warp + C4D_WARPS * lane), kv_head, HD));
+  if (lane < min(SLOTS, count)) ask(lane, next);
 
   // the queries, column g (+ 8) of the second operand: this lane's channels in the order in which codes leave a word
   unsigned qf[NT][KW][4];
@@ -112,6 +125,14 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (t0 + token) * p.q_row + (long long)head * HD + q * (HD / 4));
 #pragma unroll
       for (int w = 0; w < KW; ++w) raw[w] = src[w];
+    }
+    if (p.scale_log2 <= 0.f) {        // from here on the largest product has the largest weight
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const unsigned f = p.scale_log2 < 0.f ? 0xbf80bf80u : 0u;      // -1 or 0
+        raw[w] = make_uint4(c4_fma2(raw[w].x, f, 0x80008000u), c4_fma2(raw[w].y, f, 0x80008000u), c4_fma2(raw[w].z, f, 0x80008000u),
+                            c4_fma2(raw[w].w, f, 0x80008000u));
+      }
     }
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
@@ -140,25 +161,13 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
   }
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   const int kg = (g >> 1) + 4 * (g & 1);      // the key on row g of a tile of 16 (row g + 8: 8 further)
-  bool ok = true;
-  for (int i = 0; i < count; ++i) {
-    const int key0 = page_at(first + warp + C4D_WARPS * i) * C4_PAGE;
-    const unsigned char* rec = ring + i % SLOTS * REC;
-    {
-      const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]), parity = (unsigned)(i / SLOTS) & 1u;
-      bool landed = false;
-      for (int t = 0; t < C4D_WAIT_LIMIT && !landed; ++t) {
-        unsigned done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        landed = done != 0;
-      }
-      ok = __all_sync(0xffffffffu, landed);
-      if (!ok) break;
-    }
-    // ---- scores of the page's 64 keys ----
+  const C4Bits bits;
+  // One page of keys and values.  PLAIN: every column sees all of it, and no scale stands for NaN.
+  auto page = [&](auto plain, const unsigned char* rec, int key0, bool whole) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    // ---- scores of its 64 keys ----
     float s[NT][4][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -178,8 +187,8 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
           const uint2 v = *reinterpret_cast<const uint2*>(row);
           w[h][0] = v.x; w[h][1] = v.y;
         }
-        const unsigned b = c4_scale_bits(rec[c4_key_scales(HD) + key * G + q * G / 4]);
-        s2[h] = b | b << 16;
+        const unsigned b = rec[c4_key_scales(HD) + key * G + q * G / 4];
+        s2[h] = PLAIN || b != 255u ? c4_scale_twice(b) : 0x7fc07fc0u;
         sh[h] = c4_shift(s2[h]);
       }
 #pragma unroll
@@ -187,10 +196,10 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
         unsigned x[2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x[h][0] = c4_fma2(c4_pair<0>(w[h][k]), s2[h], sh[h]);
-          x[h][1] = c4_fma2(c4_pair<1>(w[h][k]), s2[h], sh[h]);
-          x[h][2] = c4_fma2(c4_pair<2>(w[h][k]), s2[h], sh[h]);
-          x[h][3] = c4_fma2(c4_pair<3>(w[h][k]), s2[h], sh[h]);
+          x[h][0] = c4_fma2(c4_pair<0>(w[h][k], bits), s2[h], sh[h]);
+          x[h][1] = c4_fma2(c4_pair<1>(w[h][k], bits), s2[h], sh[h]);
+          x[h][2] = c4_fma2(c4_pair<2>(w[h][k], bits), s2[h], sh[h]);
+          x[h][3] = c4_fma2(c4_pair<3>(w[h][k], bits), s2[h], sh[h]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -200,45 +209,54 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
       }
     }
     // ---- which of them a column sees; maximum, weights ----
-    const bool whole = key0 + C4_PAGE - 1 <= pos_first &&
-                       (p.window <= 0 || key0 > pos_last - p.window || key0 + C4_PAGE <= p.keep_first);
     auto seen = [&](int key, int at) { return key <= at && (p.window <= 0 || key > at - p.window || key < p.keep_first); };
+    if (!PLAIN && !whole) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!seen(key0 + 16 * t + 8 * (e >> 1) + kg, pos[n][e & 1])) s[n][t][e] = -INFINITY;
+    }
     unsigned pt[NT][4][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = s[n][t][e] * p.scale_log2;
-          if (!whole && !seen(key0 + 16 * t + 8 * (e >> 1) + kg, pos[n][e & 1])) v = -INFINITY;
-          s[n][t][e] = v;
-          top[e & 1] = fmaxf(top[e & 1], v);
-        }
       float use[2];
+      bool grown = false;
+      float top[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(s[n][0][e], s[n][0][e + 2]);
+#pragma unroll
+        for (int t = 1; t < 4; ++t) top[e] = c4d_max3(top[e], s[n][t][e], s[n][t][e + 2]);
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
-        const float m_new = fmaxf(m[n][e], top[e]);
-        use[e] = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = ds_exp2(m[n][e] - use[e]);      // 0 for a column that had seen nothing yet
-        m[n][e] = m_new;
-        l[n][e] *= alpha;
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16)) * scale;
+        grown |= top[e] > m[n][e];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-        for (int k = 0; k < MT; ++k) {
-          acc[n][k][e] *= alpha;
-          acc[n][k][e + 2] *= alpha;
+        for (int e = 0; e < 2; ++e) {
+          const float m_new = fmaxf(m[n][e], top[e]);
+          const float alpha = ds_exp2(m[n][e] - (m_new == -INFINITY ? 0.f : m_new));      // 0 for a column that had seen nothing yet
+          m[n][e] = m_new;
+          l[n][e] *= alpha;
+#pragma unroll
+          for (int k = 0; k < MT; ++k) {
+            acc[n][k][e] *= alpha;
+            acc[n][k][e + 2] *= alpha;
+          }
         }
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) use[e] = m[n][e] == -INFINITY ? 0.f : -m[n][e];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = ds_exp2(s[n][t][e] - use[e & 1]);
+          w[e] = ds_exp2(fmaf(s[n][t][e], scale, use[e & 1]));
           l[n][e & 1] += w[e];
         }
         pt[n][t][0] = c4d_transpose(ds_pack(w[0], w[1]));
@@ -260,15 +278,23 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
         } else {
           w[j][0] = *reinterpret_cast<const unsigned*>(row);
         }
-        const unsigned raw = rec[c4_value_scales(HD) + key * G + g * G / 8];
-        b[j] = raw * 16u + 0x3580u;
-        const bool past_end = !whole && key0 + key > pos_last;
-        if (raw == 255u || past_end) {      // (NaN is seen to below; what lies past the end is not there)
-          b[j] = 0u;
-          odd |= !past_end;
-        }
+        b[j] = rec[c4_value_scales(HD) + key * G + g * G / 8];
       }
-      const unsigned s01 = b[0] | b[1] << 16, s23 = b[2] | b[3] << 16;
+      unsigned s01 = c4_scale_pair(b[0], b[1]), s23 = c4_scale_pair(b[2], b[3]);
+      if (!PLAIN) {
+        unsigned v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool past_end = !whole && key0 + 16 * t + q + 4 * j > pos_last;
+          v[j] = c4_scale_bits(b[j]);
+          if ((!whole && b[j] == 255u) || past_end) {      // (NaN is seen to below; what lies past the end is not there)
+            v[j] = 0u;
+            odd |= !past_end;
+          }
+        }
+        s01 = v[0] | v[1] << 16;
+        s23 = v[2] | v[3] << 16;
+      }
       const unsigned h01 = c4_shift(s01), h23 = c4_shift(s23);
 #pragma unroll
       for (int k = 0; k < VW; ++k)
@@ -276,14 +302,14 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
         for (int half = 0; half < 2; ++half) {
           const unsigned a = __byte_perm(w[0][k], w[1][k], half ? 0x7632 : 0x5410), d = __byte_perm(w[2][k], w[3][k], half ? 0x7632 : 0x5410);
           unsigned x[4], y[4];
-          x[0] = c4_fma2(c4_pair<0>(a), s01, h01);
-          x[1] = c4_fma2(c4_pair<1>(a), s01, h01);
-          x[2] = c4_fma2(c4_pair<2>(a), s01, h01);
-          x[3] = c4_fma2(c4_pair<3>(a), s01, h01);
-          y[0] = c4_fma2(c4_pair<0>(d), s23, h23);
-          y[1] = c4_fma2(c4_pair<1>(d), s23, h23);
-          y[2] = c4_fma2(c4_pair<2>(d), s23, h23);
-          y[3] = c4_fma2(c4_pair<3>(d), s23, h23);
+          x[0] = c4_fma2(c4_pair<0>(a, bits), s01, h01);
+          x[1] = c4_fma2(c4_pair<1>(a, bits), s01, h01);
+          x[2] = c4_fma2(c4_pair<2>(a, bits), s01, h01);
+          x[3] = c4_fma2(c4_pair<3>(a, bits), s01, h01);
+          y[0] = c4_fma2(c4_pair<0>(d, bits), s23, h23);
+          y[1] = c4_fma2(c4_pair<1>(d, bits), s23, h23);
+          y[2] = c4_fma2(c4_pair<2>(d, bits), s23, h23);
+          y[3] = c4_fma2(c4_pair<3>(d, bits), s23, h23);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             ds_mma(acc[n][4 * k + 2 * half], x[0], x[1], y[0], y[1], pt[n][t][0], pt[n][t][1]);
@@ -291,7 +317,7 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
           }
         }
     }
-    if (__any_sync(0xffffffffu, odd)) {      // the columns that see a key whose values are NaN
+    if (!PLAIN && !whole && __any_sync(0xffffffffu, odd)) {      // the columns that see a key whose values are NaN
       for (int key = 0; key < C4_PAGE; ++key) {
         if (rec[c4_value_scales(HD) + key * G + g * G / 8] != 255u) continue;
 #pragma unroll
@@ -304,10 +330,41 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
             }
       }
     }
-    __syncwarp();
-    if (lane == 0 && i + SLOTS < count) {
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      ask(i + SLOTS, c4_page(c, seq, page_at(first + warp + C4D_WARPS * (i + SLOTS)), kv_head, HD));
+  };
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    const int key0 = page_at(first + warp + C4D_WARPS * i) * C4_PAGE;
+    const unsigned char* rec = ring + i % SLOTS * REC;
+    {
+      const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]), parity = (unsigned)(i / SLOTS) & 1u;
+      bool landed = false;
+      for (int t = 0; t < C4D_WAIT_LIMIT && !landed; ++t) {
+        unsigned done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        landed = done != 0;
+      }
+      ok = __all_sync(0xffffffffu, landed);
+      if (!ok) break;
+    }
+    const bool whole = key0 + C4_PAGE - 1 <= pos_first &&
+                       (p.window <= 0 || key0 > pos_last - p.window || key0 + C4_PAGE <= p.keep_first);
+    bool nan = false;                       // among the page's scales?  (128 G bytes)
+#pragma unroll
+    for (int j = 0; j < G; ++j) nan |= c4_has_255(*reinterpret_cast<const unsigned*>(rec + c4_key_scales(HD) + 4 * (lane + 32 * j)));
+    if (whole && !__any_sync(0xffffffffu, nan))
+      page(C4dFlag<true>(), rec, key0, true);
+    else
+      page(C4dFlag<false>(), rec, key0, whole);
+    if (i + SLOTS < count) {
+      __syncwarp();
+      const unsigned long long rec_next = __shfl_sync(0xffffffffu, (unsigned long long)next, (i + SLOTS) & 31);
+      if (lane == 0) {
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        ask(i + SLOTS, reinterpret_cast<const unsigned char*>(rec_next));
+      }
+      if (((i + SLOTS) & 31) == 31) next = record_of(i + SLOTS + 1 + lane);
     }
   }
   if (!ok) {
@@ -370,11 +427,14 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   }
 }
 
-// Joins the pieces of a (sequence, key head, columns) in their order.  A block a unit, a thread a channel.
-template <int HD, int NT>
-__global__ void __launch_bounds__(HD)
+// Joins the pieces of a column of a (sequence, key head), in an order that the number of pieces alone sets.  A block a column: the pieces'
+// maxima and sums at once, then a thread a channel and every GROUPS-th piece, then the groups' sums.
+constexpr int C4J_MOST = 1024;      // pieces at most
+template <int HD, int NT, int GROUPS>
+__global__ void __launch_bounds__(HD * GROUPS)
 cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
-  constexpr int COLS = 8 * NT;
+  constexpr int COLS = 8 * NT, THREADS = HD * GROUPS;
+  __shared__ float s_weight[C4J_MOST], s_sum[GROUPS][HD], scratch[33];
   pdl_trigger();
   pdl_wait();
   const int seq = blockIdx.z, kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS, col = blockIdx.x;
@@ -386,19 +446,33 @@ cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
   const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
   const int n_pages = kept_only + pos_last / C4_PAGE - pg_lo + 1;
   const int per = max((n_pages + n_splits - 1) / n_splits, min(C4D_WARPS, n_pages)), used = (n_pages + per - 1) / per;
-  const long long unit = (long long)seq * gridDim.y + blockIdx.y;
-  float top = -INFINITY, sum = 0.f, o = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const long long at = (unit * n_splits + s) * COLS + col;
-    const float m = p.part[p.part_ml + 2 * at], l = p.part[p.part_ml + 2 * at + 1], x = p.part[at * HD + threadIdx.x];
-    const float m_new = fmaxf(top, m), use = m_new == -INFINITY ? 0.f : m_new;
-    const float a = ds_exp2(top - use), b = ds_exp2(m - use);
-    sum = sum * a + l * b;
-    o = o * a + x * b;
-    top = m_new;
+  const long long at0 = ((long long)seq * gridDim.y + blockIdx.y) * n_splits * COLS + col;
+  const int tid = threadIdx.x, d = tid % HD, group = tid / HD;
+  float top = -INFINITY;
+  for (int s = tid; s < used; s += THREADS) {
+    const float m = p.part[p.part_ml + 2 * (at0 + (long long)s * COLS)];
+    s_weight[s] = m;
+    top = fmaxf(top, m);
   }
+  top = block_max(top, scratch);
+  const float use = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int s = tid; s < used; s += THREADS) {
+    const float w = ds_exp2(s_weight[s] - use);
+    s_weight[s] = w;
+    sum += p.part[p.part_ml + 2 * (at0 + (long long)s * COLS) + 1] * w;
+  }
+  sum = block_sum(sum, scratch);      // (every weight is in shared memory when it returns)
+  float o = 0.f;
+#pragma unroll 4
+  for (int s = group; s < used; s += GROUPS) o += p.part[(at0 + (long long)s * COLS) * HD + d] * s_weight[s];
+  s_sum[group][d] = o;
+  __syncthreads();
+  if (group != 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) o += s_sum[i][d];
   const int token = (col0 + col) / p.group, head = kv_head * p.group + (col0 + col) % p.group;
-  p.out[((long long)(t0 + token) * p.n_heads + head) * HD + threadIdx.x] = __float2bfloat16_rn(o / sum);
+  p.out[((long long)(t0 + token) * p.n_heads + head) * HD + d] = __float2bfloat16_rn(o / sum);
 }
 
 template <int HD, int NT>
@@ -410,8 +484,13 @@ static int launch_c4d(const Cache4DecodeParams& p, const Cache4View& c, int n_se
   BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
   const dim3 grid(n_splits, c.n_kv_heads * p.col_blocks, n_seqs);
   BT_PDL_OK("cache4_decode", launch_pdl(kern, grid, dim3(C4D_WARPS * 32), smem, stream, 1, p, c));
-  if (n_splits > 1)
-    BT_PDL_OK("cache4_join", launch_pdl(cache4_join_kernel<HD, NT>, dim3(8 * NT, c.n_kv_heads * p.col_blocks, n_seqs), dim3(HD), 0, stream, 1, p, n_splits));
+  if (n_splits > 1) {
+    const dim3 columns(p.group * p.max_new < 8 * NT ? p.group * p.max_new : 8 * NT, c.n_kv_heads * p.col_blocks, n_seqs);
+    if (n_splits <= 16)
+      BT_PDL_OK("cache4_join", launch_pdl(cache4_join_kernel<HD, NT, 1>, columns, dim3(HD), 0, stream, 1, p, n_splits));
+    else
+      BT_PDL_OK("cache4_join", launch_pdl(cache4_join_kernel<HD, NT, 4>, columns, dim3(HD * 4), 0, stream, 1, p, n_splits));
+  }
   return 0;
 }
 
@@ -434,11 +513,12 @@ extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const
   const int group = n_heads / n_kv_heads;
   const long long cols = (long long)max_new * group;
   const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
-  BT_CHECK(n_seqs <= 65535 && (long long)n_kv_heads * blocks <= 65535 && n_splits >= 1 && n_splits <= 65535, "cache4_attention: grid too large");
+  BT_CHECK(n_seqs <= 65535 && (long long)n_kv_heads * blocks <= 65535 && n_splits >= 1 && n_splits <= C4J_MOST,
+           "cache4_attention: grid too large");
   const long long parts = (long long)n_seqs * n_kv_heads * blocks * n_splits * 8 * nt;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks,
+  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks, max_new,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, stream);

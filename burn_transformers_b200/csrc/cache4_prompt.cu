@@ -303,6 +303,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
     // a warp's 32 lanes read 16 bytes each of 8 (16) rows in a row; eight lanes of a store cover eight rows' same piece
     constexpr int SPAN = 32 / CH;        // rows of a warp's read
     const int dw = warp - 8, chunk = (lane >> 3) % CH, sub_row = (lane & 7) + 8 * ((lane >> 3) / CH);
+    const C4Bits bits;
     uint4 raw[CH];
     unsigned sc[CH];
     // the row j of this lane in a tile: SPAN (4 j + dw) + sub_row
@@ -333,8 +334,8 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k]), s2, shift), c4_fma2(c4_pair<1>(w[k]), s2, shift),
-                                     c4_fma2(c4_pair<2>(w[k]), s2, shift), c4_fma2(c4_pair<3>(w[k]), s2, shift));
+          const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k], bits), s2, shift), c4_fma2(c4_pair<1>(w[k], bits), s2, shift),
+                                     c4_fma2(c4_pair<2>(w[k], bits), s2, shift), c4_fma2(c4_pair<3>(w[k], bits), s2, shift));
           *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
         }
       }

@@ -2120,6 +2120,9 @@ def _sm_count() -> int:
     return _SM_COUNTS[device]
 
 
+SPLIT_X = 6
+
+
 def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
     """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
 
@@ -2130,8 +2133,8 @@ def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window
     units = max(1, n_seqs * n_kv_heads)
     span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
     if columns <= 16:
-        # blocks to fill the GPU twice over; a warp of a block's four takes a page at least
-        splits = max(1, min(-(-6 * _sm_count() // units), -(-span // (4 * PAGE_SIZE))))
+        # blocks to fill the GPU, three a multiprocessor; a warp of a block's four takes a page at least
+        splits = max(1, min(-(-SPLIT_X * _sm_count() // units), -(-span // (4 * PAGE_SIZE)), 1024))
         return "few", splits, units * splits * (8 if columns <= 8 else 16) * (head_dim + 2) if splits > 1 else 0
     tiles = -(-columns // 256)
     # a block a multiprocessor; pieces of eight tiles of 128 keys at least

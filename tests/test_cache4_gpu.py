@@ -194,6 +194,18 @@ def test_attention(dtype, heads, kv, dim, pasts, news, window, keep):
     assert torch.equal(got, attend(step, q, pool, heads, kv, dim, window, keep, scale))
 
 
+@pytest.mark.parametrize("heads, kv, dim", [(2, 2, 64), (5, 1, 128), (32, 2, 64)])
+@pytest.mark.parametrize("pasts, news", [([9001], [1]), ([5000, 17, 0], [1, 1, 1]), ([4500, 60], [3, 1]), ([6000, 300], [50, 41]), ([4000], [257])])
+@pytest.mark.parametrize("window, keep", [(0, 0), (2100, 70), (3000, 0)])
+def test_long_runs_in_pieces(heads, kv, dim, pasts, news, window, keep):
+    step, rng = Step(pasts, news), np.random.default_rng(heads + window)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, -0.2)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, -0.2)
+    assert torch.equal(got, attend(step, q, pool, heads, kv, dim, window, keep, -0.2))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads, kv, dim", [(4, 2, 64), (8, 1, 128)])
 @pytest.mark.parametrize("pasts, news", [([70, 300], [3, 2]), ([0, 100], [140, 1])])
