@@ -278,7 +278,7 @@ int bt_cache4_attention(const void* q, long long q_row, void* out, const void* p
                         int n_kv_heads, int dim, float scale, int window, int keep_first, int dtype, cudaStream_t stream);
 int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
                      int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,
-                     int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits, float* scratch,
+                     int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits, int n_warps, float* scratch,
                      long long scratch_floats, cudaStream_t stream);
 int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
                      int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,

@@ -57,14 +57,22 @@ __device__ __forceinline__ int c4_scale_byte(float top) {
   return b;
 }
 
-// round(x / s), ties to even, within -7..7.  The first guess is off by one at most; x - r s is exact (its bits lie between
-// x's last and s's first), so that it says which way.
-__device__ __forceinline__ int c4_code(float x, float s, float inv) {
-  float r = rintf(x * inv);
-  const float rest = fmaf(-r, s, x), half = 0.5f * s;
-  const bool odd = ((int)fminf(fmaxf(r, -8.f), 8.f)) & 1;
-  if (fabsf(rest) > half || (fabsf(rest) == half && odd)) r += rest > 0.f ? 1.f : -1.f;
-  return (int)fminf(fmaxf(r, -7.f), 7.f);
+// round(x / s) + 8, ties to even, in the last four bits.  `inv`: 1 / s rounded.
+// bfloat16 x: the corrected quotient is x / s rounded to 24 bits, which is no tie unless x / s is one (x and (k + 1/2) s have 8
+// significant bits each, so that they are equal or differ by more than 2^-9 of x).  32-bit x may lie closer to a tie than a quotient
+// tells: the rest x - r s, which is exact, says on which side.
+template <typename T>
+__device__ __forceinline__ unsigned c4_code(float x, float s, float inv) {
+  constexpr float kMagic = 12582912.f;         // 1.5 x 2^23: a sum with it rounds to whole numbers
+  float r = x * inv;
+  r = fmaf(fmaf(-r, s, x), inv, r);
+  if constexpr (sizeof(T) == 4) {
+    r = rintf(r);
+    const float rest = fmaf(-r, s, x), half = 0.5f * s;
+    const bool odd = (int)fminf(fmaxf(r, -8.f), 8.f) & 1;
+    if (fabsf(rest) > half || (fabsf(rest) == half && odd)) r += rest > 0.f ? 1.f : -1.f;
+  }
+  return __float_as_uint(r + (kMagic + 8.f)) & 15u;
 }
 
 // grid (blocks of tokens, pieces of a token's lanes); a lane: (head, key or value, 8 channels)
@@ -120,15 +128,20 @@ cache4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Cache4Row
     const bool fine = top < 0x7f800000u;
     const int b = fine ? c4_scale_byte(__uint_as_float(top)) : 255;
     const float s = c4_scale((unsigned)b), inv = 1.f / s;
+    if (b == 254) {                            // the largest scale: what its seventh multiple does not reach stays at it
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = fminf(fmaxf(x[i][j], -7.f * s), 7.f * s);
+    }
     unsigned word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word |= (unsigned)((fine ? c4_code(x[i][j], s, inv) : 0) + 8) << (4 * j);
+    for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(x[i][j], s, inv);
+    if (!fine) word = 0x88888888u;
     *reinterpret_cast<unsigned*>(rec[i] + which * c4_value_codes(dim) + in_page[i] * (dim / 2) + at * 4) = word;
     if ((at & 3) == 0) rec[i][c4_key_scales(dim) + which * (2 * dim) + in_page[i] * (dim / 32) + at / 4] = (unsigned char)b;
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(C4_THREADS)
 cache4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Cache4Rows rows, Cache4View c, const int* __restrict__ positions,
                      const int* __restrict__ token_seq, int n_tokens, int n_table, int dim) {
@@ -136,26 +149,38 @@ cache4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Cache4Rows rows, Cach
   pdl_wait();
   const int lane = blockIdx.y * C4_THREADS + threadIdx.x;
   const int eighths = dim / 8;
-  const int head = lane / (2 * eighths), t = blockIdx.x;
+  const int head = lane / (2 * eighths), t0 = blockIdx.x * TOKENS;
   if (head >= c.n_kv_heads) return;
   const int which = lane / eighths & 1, at = lane % eighths;
-  const int seq = token_seq[t], pos = positions[t];
-  int page = -1;
-  if (seq >= 0 && seq < n_table && pos >= 0) page = c.table[(long long)seq * c.table_stride + pos / C4_PAGE % c.table_len];
-  float x[8];
-  if (page < 0 || page >= c.n_pages) {
-    if (c.status) atomicExch(c.status, 9);
+  T* dst = (which ? v + head * rows.v_head : k + head * rows.k_head) + at * 8;
+  const long long row = which ? rows.v_row : rows.k_row;
+  unsigned word[TOKENS], b[TOKENS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = NAN;
-  } else {
+  for (int i = 0; i < TOKENS; ++i) {
+    word[i] = 0;
+    b[i] = 255u;
+    if (t0 + i >= n_tokens) continue;
+    const int seq = token_seq[t0 + i], pos = positions[t0 + i];
+    int page = -1;
+    if (seq >= 0 && seq < n_table && pos >= 0) page = c.table[(long long)seq * c.table_stride + pos / C4_PAGE % c.table_len];
+    if (page < 0 || page >= c.n_pages) {
+      if (c.status) atomicExch(c.status, 9);
+      continue;
+    }
     const int in_page = pos % C4_PAGE;
     const unsigned char* rec = c.pool + ((long long)page * c.n_kv_heads + head) * c4_record(dim);
-    const unsigned word = *reinterpret_cast<const unsigned*>(rec + which * c4_value_codes(dim) + in_page * (dim / 2) + at * 4);
-    const float s = c4_scale(rec[c4_key_scales(dim) + which * (2 * dim) + in_page * (dim / 32) + at / 4]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)((int)(word >> (4 * j) & 15u) - 8) * s;
+    word[i] = *reinterpret_cast<const unsigned*>(rec + which * c4_value_codes(dim) + in_page * (dim / 2) + at * 4);
+    b[i] = rec[c4_key_scales(dim) + which * (2 * dim) + in_page * (dim / 32) + at / 4];
   }
-  c4_store8<T, VEC>((which ? v + t * rows.v_row + head * rows.v_head : k + t * rows.k_row + head * rows.k_head) + at * 8, x);
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    if (t0 + i >= n_tokens) break;
+    const float s = c4_scale(b[i]);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)((int)(word[i] >> (4 * j) & 15u) - 8) * s;
+    c4_store8<T, VEC>(dst + (t0 + i) * row, x);
+  }
 }
 
 static int c4_check(const char* what, const void* pool, long long n_pages, const int* table, int table_len, int n_tokens, int n_kv_heads,
@@ -223,15 +248,24 @@ extern "C" int bt_cache4_gather(void* k, long long k_row, long long k_head, void
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   const int lanes = n_kv_heads * dim / 4;
   const bool vec = c4_whole(k, v, rows, dtype == kF32 ? 4 : 2);
-  const dim3 grid(n_tokens, (lanes + C4_THREADS - 1) / C4_THREADS);
-#define BT_C4_GATHER(T, VEC)                                                                                                   \
-  BT_PDL_OK("cache4_gather", launch_pdl(cache4_gather_kernel<T, VEC>, grid, dim3(C4_THREADS), 0, stream, 1, (T*)k, (T*)v, rows, c, \
+  const int pieces = (lanes + C4_THREADS - 1) / C4_THREADS;
+  const bool many = (long long)n_tokens * pieces > 4096;
+  const dim3 grid(many ? (n_tokens + 3) / 4 : n_tokens, pieces);
+#define BT_C4_GATHER(T, VEC, TOK)                                                                                                   \
+  BT_PDL_OK("cache4_gather", launch_pdl(cache4_gather_kernel<T, VEC, TOK>, grid, dim3(C4_THREADS), 0, stream, 1, (T*)k, (T*)v, rows, c, \
                                         positions, token_seq, n_tokens, n_table, dim))
-  if (dtype == kF32) {
-    if (vec) BT_C4_GATHER(float, true); else BT_C4_GATHER(float, false);
-  } else {
-    if (vec) BT_C4_GATHER(__nv_bfloat16, true); else BT_C4_GATHER(__nv_bfloat16, false);
+#define BT_C4_GATHER_T(T)                                                          \
+  if (vec) {                                                                       \
+    if (many) BT_C4_GATHER(T, true, 4); else BT_C4_GATHER(T, true, 1);             \
+  } else {                                                                         \
+    if (many) BT_C4_GATHER(T, false, 4); else BT_C4_GATHER(T, false, 1);           \
   }
+  if (dtype == kF32) {
+    BT_C4_GATHER_T(float)
+  } else {
+    BT_C4_GATHER_T(__nv_bfloat16)
+  }
+#undef BT_C4_GATHER_T
 #undef BT_C4_GATHER
   return 0;
 }

@@ -23,7 +23,7 @@
 
 namespace bt {
 
-constexpr int C4D_WARPS = 4;
+constexpr int C4D_MOST_WARPS = 12;        // of a block, by the registers of a multiprocessor (with 16 columns: 8)
 constexpr int C4D_WAIT_LIMIT = 1 << 20;
 
 struct Cache4DecodeParams {
@@ -31,17 +31,14 @@ struct Cache4DecodeParams {
   long long q_row;
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
-  int n_heads, group, col_blocks, max_new;
+  int n_heads, group, col_blocks, max_new, slots;
   float scale_log2;
   int window, keep_first;
   float* part;                 // [unit][split][columns][HD], then [unit][split][columns][2]
   long long part_ml;           // where the second begins
 };
 
-template <int HD>
-constexpr int c4d_slots() { return HD == 128 ? 2 : 3; }
-template <int HD, int NT>
-constexpr size_t c4d_smem() { return (size_t)C4D_WARPS * c4d_slots<HD>() * c4_record(HD); }
+constexpr int C4D_MOST_SLOTS = 8;        // pages of a warp's ring
 
 __device__ __forceinline__ unsigned c4d_transpose(unsigned v) {
   unsigned d;
@@ -60,20 +57,21 @@ struct C4dFlag {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(C4D_WARPS * 32, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(NT == 1 ? 384 : 256, 1)
 cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
-  constexpr int SLOTS = c4d_slots<HD>(), REC = c4_record(HD), G = HD / 32;
+  constexpr int REC = c4_record(HD), G = HD / 32;
   constexpr int KW = HD / 32;            // 32-bit words of a key row a lane holds
   constexpr int VW = HD / 64;            // of a value row
   constexpr int MT = HD / 16;
   constexpr int COLS = 8 * NT;
   extern __shared__ __align__(128) unsigned char c4d_raw[];
-  __shared__ __align__(8) unsigned long long s_full[C4D_WARPS][SLOTS];
-  __shared__ float s_ml[C4D_WARPS][COLS][2];
+  __shared__ __align__(8) unsigned long long s_full[C4D_MOST_WARPS][C4D_MOST_SLOTS];
+  __shared__ float s_ml[C4D_MOST_WARPS][COLS][2];
   __shared__ int s_failed;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int n_warps = (int)blockDim.x >> 5;
   const int split = blockIdx.x, n_splits = gridDim.x, seq = blockIdx.z;
   const int kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS;
   const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0, n_cols = n_new * p.group - col0;
@@ -85,32 +83,32 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   const int pg_lo = lo / C4_PAGE, pg_hi = pos_last / C4_PAGE;
   const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
   const int n_pages = kept_only + pg_hi - pg_lo + 1;
-  const int per = max((n_pages + n_splits - 1) / n_splits, min(C4D_WARPS, n_pages));      // (a page a warp at least)
+  const int per = (n_pages + n_splits - 1) / n_splits;
   const int first = split * per, mine = min(n_pages, first + per) - first;
   const long long unit = (long long)seq * gridDim.y + blockIdx.y;
   if (mine <= 0) return;                 // (the join counts the pieces in the same way)
   auto page_at = [&](int i) { return i < kept_only ? i : pg_lo + (i - kept_only); };
 
   if (lane == 0) {
-    for (int s = 0; s < SLOTS; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(ds_smem(&s_full[warp][s])));
+    for (int s = 0; s < p.slots; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(ds_smem(&s_full[warp][s])));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (tid == 0) s_failed = 0;
   __syncthreads();
-  unsigned char* ring = c4d_raw + warp * SLOTS * REC;
-  const int count = mine > warp ? (mine - warp + C4D_WARPS - 1) / C4D_WARPS : 0;      // this warp's pages: first + warp + 4 i
+  unsigned char* ring = c4d_raw + warp * p.slots * REC;
+  const int count = mine > warp ? (mine - warp + n_warps - 1) / n_warps : 0;      // this warp's pages: first + warp + n_warps i
   // records of this warp's next 32 pages, one a lane
-  auto record_of = [&](int i) { return c4_page(c, seq, page_at(first + warp + C4D_WARPS * min(i, count - 1)), kv_head, HD); };
+  auto record_of = [&](int i) { return c4_page(c, seq, page_at(first + warp + n_warps * min(i, count - 1)), kv_head, HD); };
   const unsigned char* next = count > 0 ? record_of(lane) : nullptr;
-  auto ask = [&](int i, const unsigned char* rec) {      // (one lane)
-    const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]);
+  auto ask = [&](int slot, const unsigned char* rec) {      // (one lane)
+    const unsigned bar = ds_smem(&s_full[warp][slot]);
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((unsigned)REC) : "memory");
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
-                     ds_smem(ring + i % SLOTS * REC)),
+                     ds_smem(ring + slot * REC)),
                  "l"(rec), "r"((unsigned)REC), "r"(bar)
                  : "memory");
   };
-  if (lane < min(SLOTS, count)) ask(lane, next);
+  if (lane < min(p.slots, count)) ask(lane, next);
 
   // the queries, column g (+ 8) of the second operand: this lane's channels in the order in which codes leave a word
   unsigned qf[NT][KW][4];
@@ -332,11 +330,13 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
     }
   };
   bool ok = true;
+  int slot = 0;
+  unsigned parity = 0;
   for (int i = 0; i < count; ++i) {
-    const int key0 = page_at(first + warp + C4D_WARPS * i) * C4_PAGE;
-    const unsigned char* rec = ring + i % SLOTS * REC;
+    const int key0 = page_at(first + warp + n_warps * i) * C4_PAGE;
+    const unsigned char* rec = ring + slot * REC;
     {
-      const unsigned bar = ds_smem(&s_full[warp][i % SLOTS]), parity = (unsigned)(i / SLOTS) & 1u;
+      const unsigned bar = ds_smem(&s_full[warp][slot]);
       bool landed = false;
       for (int t = 0; t < C4D_WAIT_LIMIT && !landed; ++t) {
         unsigned done;
@@ -357,14 +357,19 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
       page(C4dFlag<true>(), rec, key0, true);
     else
       page(C4dFlag<false>(), rec, key0, whole);
-    if (i + SLOTS < count) {
+    const int then = i + p.slots;           // the page that comes into this slot
+    if (then < count) {
       __syncwarp();
-      const unsigned long long rec_next = __shfl_sync(0xffffffffu, (unsigned long long)next, (i + SLOTS) & 31);
+      const unsigned long long rec_next = __shfl_sync(0xffffffffu, (unsigned long long)next, then & 31);
       if (lane == 0) {
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        ask(i + SLOTS, reinterpret_cast<const unsigned char*>(rec_next));
+        ask(slot, reinterpret_cast<const unsigned char*>(rec_next));
       }
-      if (((i + SLOTS) & 31) == 31) next = record_of(i + SLOTS + 1 + lane);
+      if ((then & 31) == 31) next = record_of(then + 1 + lane);
+    }
+    if (++slot == p.slots) {
+      slot = 0;
+      parity ^= 1u;
     }
   }
   if (!ok) {
@@ -399,15 +404,13 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
     }
   __syncthreads();
   if (s_failed && tid == 0 && c.status) atomicExch(c.status, 10);
-  for (int i = tid; i < COLS * HD; i += C4D_WARPS * 32) {
+  for (int i = tid; i < COLS * HD; i += (int)blockDim.x) {
     const int col = i / HD, d = i % HD;
     if (col >= n_cols) break;
     float top = -INFINITY, sum = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < C4D_WARPS; ++w) top = fmaxf(top, s_ml[w][col][0]);
+    for (int w = 0; w < n_warps; ++w) top = fmaxf(top, s_ml[w][col][0]);
     const float use = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < C4D_WARPS; ++w) {
+    for (int w = 0; w < n_warps; ++w) {
       const float weight = ds_exp2(s_ml[w][col][0] - use);
       sum += s_ml[w][col][1] * weight;
       o += s_acc[(w * COLS + col) * HD + d] * weight;
@@ -445,7 +448,7 @@ cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
   const int pg_lo = (p.window > 0 ? max(0, pos_first - p.window + 1) : 0) / C4_PAGE;
   const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
   const int n_pages = kept_only + pos_last / C4_PAGE - pg_lo + 1;
-  const int per = max((n_pages + n_splits - 1) / n_splits, min(C4D_WARPS, n_pages)), used = (n_pages + per - 1) / per;
+  const int per = (n_pages + n_splits - 1) / n_splits, used = (n_pages + per - 1) / per;
   const long long at0 = ((long long)seq * gridDim.y + blockIdx.y) * n_splits * COLS + col;
   const int tid = threadIdx.x, d = tid % HD, group = tid / HD;
   float top = -INFINITY;
@@ -476,14 +479,23 @@ cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
 }
 
 template <int HD, int NT>
-static int launch_c4d(const Cache4DecodeParams& p, const Cache4View& c, int n_seqs, int n_splits, cudaStream_t stream) {
-  constexpr size_t smem = c4d_smem<HD, NT>();
-  static_assert(smem >= sizeof(float) * C4D_WARPS * 8 * NT * HD, "the joined results outgrow the rings");
+static int launch_c4d(Cache4DecodeParams p, const Cache4View& c, int n_seqs, int n_splits, int n_warps, cudaStream_t stream) {
+  // the rings: the blocks that share a multiprocessor, as many as their registers allow and the call has, share its shared memory
+  constexpr int MOST = NT == 1 ? 12 : 8, WHOLE = 222 * 1024;
+  BT_CHECK(n_warps >= 1 && n_warps <= MOST, "cache4_attention: %d warps a block (1 to %d)", n_warps, MOST);
+  const long long blocks = (long long)n_splits * c.n_kv_heads * p.col_blocks * n_seqs;
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  int side = (int)(blocks <= sms ? 1 : blocks <= 2ll * sms ? 2 : 3);
+  if (side > MOST / n_warps) side = MOST / n_warps;
+  p.slots = (WHOLE / side - 2048) / (n_warps * c4_record(HD));
+  if (p.slots > C4D_MOST_SLOTS) p.slots = C4D_MOST_SLOTS;
+  const size_t smem = (size_t)n_warps * p.slots * c4_record(HD);
+  static_assert(2 * c4_record(HD) >= (int)sizeof(float) * 8 * NT * HD && WHOLE / 3 - 2048 >= 2 * 4 * c4_record(HD), "the joined results outgrow the rings");
   auto kern = cache4_decode_kernel<HD, NT>;
   static SharedMemoryAllowance allowed;
   BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
   const dim3 grid(n_splits, c.n_kv_heads * p.col_blocks, n_seqs);
-  BT_PDL_OK("cache4_decode", launch_pdl(kern, grid, dim3(C4D_WARPS * 32), smem, stream, 1, p, c));
+  BT_PDL_OK("cache4_decode", launch_pdl(kern, grid, dim3(n_warps * 32), smem, stream, 1, p, c));
   if (n_splits > 1) {
     const dim3 columns(p.group * p.max_new < 8 * NT ? p.group * p.max_new : 8 * NT, c.n_kv_heads * p.col_blocks, n_seqs);
     if (n_splits <= 16)
@@ -501,7 +513,7 @@ static int launch_c4d(const Cache4DecodeParams& p, const Cache4View& c, int n_se
 extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
                                 int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
                                 int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
-                                float* scratch, long long scratch_floats, cudaStream_t stream) {
+                                int n_warps, float* scratch, long long scratch_floats, cudaStream_t stream) {
   using namespace bt;
   BT_CHECK(dim == 64 || dim == 128, "cache4_attention: the kernel for few tokens takes heads of 64 or 128 channels, not %d", dim);
   BT_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "cache4_attention: %d query heads cannot share %d key heads", n_heads, n_kv_heads);
@@ -518,9 +530,9 @@ extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const
   const long long parts = (long long)n_seqs * n_kv_heads * blocks * n_splits * 8 * nt;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks, max_new,
+  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks, max_new, 0,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
-  if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, stream);
-  return nt == 1 ? launch_c4d<128, 1>(p, c, n_seqs, n_splits, stream) : launch_c4d<128, 2>(p, c, n_seqs, n_splits, stream);
+  if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, n_warps, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, n_warps, stream);
+  return nt == 1 ? launch_c4d<128, 1>(p, c, n_seqs, n_splits, n_warps, stream) : launch_c4d<128, 2>(p, c, n_seqs, n_splits, n_warps, stream);
 }

@@ -37,16 +37,23 @@ __device__ __forceinline__ float2 qn_turn(int pos, float f, float size) {
   return make_float2(c * size, s * size);
 }
 
+// 8 channels as they lie in memory, and as numbers.
 template <typename T>
-__device__ __forceinline__ void qn_load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    unpack16(*reinterpret_cast<const uint4*>(p), x);
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+struct QnRaw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      unpack16(v[0], x);
+    } else {
+      x[0] = __uint_as_float(v[0].x); x[1] = __uint_as_float(v[0].y); x[2] = __uint_as_float(v[0].z); x[3] = __uint_as_float(v[0].w);
+      x[4] = __uint_as_float(v[1].x); x[5] = __uint_as_float(v[1].y); x[6] = __uint_as_float(v[1].z); x[7] = __uint_as_float(v[1].w);
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void qn_store8(T* p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 2) {
@@ -72,13 +79,25 @@ qk_norm_rotary_kernel(QnParams p) {
   const int token = (int)(job / p.warps_per_token), part = (int)(job % p.warps_per_token);
   if (token >= p.n_tokens) return;
   const int pos = p.positions[token];
-  float2* turn = s_turn[warp];
-  for (int i = lane; i < p.rot / 2; i += 32) turn[i] = qn_turn(pos, p.freq[i], p.size);
-  __syncwarp();
   // this lane's two pieces of 8 channels: pieces that turn into one another, or (past the turned ones, and for neighbours) in a row
   const int c = lane % LANES, sub = lane / LANES, pairs = p.interleaved ? 0 : p.rot / 16;
   const bool mine = 16 * c < p.dim, turned = 16 * c < p.rot;
   const int a = c < pairs ? 8 * c : 16 * c, b = c < pairs ? 8 * (c + pairs) : 16 * c + 8;
+  const int first = part * p.vecs_per_warp, last = min(p.n_vecs, first + p.vecs_per_warp);
+  const T* src = reinterpret_cast<const T*>(p.src) + token * p.src_row;
+  T* dst = reinterpret_cast<T*>(p.dst) + token * p.dst_row;
+  // the next heads are asked for before the ones at hand are worked on (the first before the angles)
+  QnRaw<T> next_x, next_y;
+  auto fetch = [&](int v) {
+    if (mine && v < last) {
+      next_x.load(src + (long long)v * p.dim + a);
+      next_y.load(src + (long long)v * p.dim + b);
+    }
+  };
+  fetch(first + sub);
+  float2* turn = s_turn[warp];
+  for (int i = lane; i < p.rot / 2; i += 32) turn[i] = qn_turn(pos, p.freq[i], p.size);
+  __syncwarp();
   float cs[8], sn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -86,9 +105,6 @@ qk_norm_rotary_kernel(QnParams p) {
     cs[i] = w.x;
     sn[i] = w.y;
   }
-  const int first = part * p.vecs_per_warp, last = min(p.n_vecs, first + p.vecs_per_warp);
-  const T* src = reinterpret_cast<const T*>(p.src) + token * p.src_row;
-  T* dst = reinterpret_cast<T*>(p.dst) + token * p.dst_row;
   float wa[8], wb[8];
   const float* held = nullptr;
   for (int v0 = first; v0 < last; v0 += 32 / LANES) {
@@ -96,9 +112,10 @@ qk_norm_rotary_kernel(QnParams p) {
     const bool here = mine && v < last;
     float x[8], y[8];
     if (here) {
-      qn_load8<T>(src + (long long)v * p.dim + a, x);
-      qn_load8<T>(src + (long long)v * p.dim + b, y);
+      next_x.unpack(x);
+      next_y.unpack(y);
     }
+    fetch(v + 32 / LANES);
     if (p.normed) {
       float sum = 0.f;
       if (here) {
@@ -110,8 +127,11 @@ qk_norm_rotary_kernel(QnParams p) {
       const float r = rsqrtf(sum / (float)p.dim + p.eps);
       const float* weight = v < p.n_heads ? p.q_weight : p.k_weight;
       if (here && weight != held) {
-        qn_load8<float>(weight + a, wa);
-        qn_load8<float>(weight + b, wb);
+        QnRaw<float> w;
+        w.load(weight + a);
+        w.unpack(wa);
+        w.load(weight + b);
+        w.unpack(wb);
         held = weight;
       }
 #pragma unroll

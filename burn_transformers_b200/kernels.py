@@ -7,6 +7,8 @@ so that a kernel never sees a size it was not written for.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -1935,7 +1937,7 @@ _ARGUMENTS = {
     "bt_cache4_append": "pllpllplppppiiipiiiip",
     "bt_cache4_gather": "pllpllplpppiiipiiiip",
     "bt_cache4_attention": "plpplpiipppiiiiifiiip",
-    "bt_cache4_decode": "plpplpiipppiiiiifiiiplp",
+    "bt_cache4_decode": "plpplpiipppiiiiifiiiiplp",
     "bt_cache4_prompt": "plpplpiipppiiiiifiiiplp",
 }
 
@@ -2120,26 +2122,57 @@ def _sm_count() -> int:
     return _SM_COUNTS[device]
 
 
-SPLIT_X = 6
+@functools.lru_cache(maxsize=4096)
+def _cache4_few(sms, units, pages, wide, head_dim):
+    """(warps a block, pieces of the keys) for `units` blocks' worth of columns over `pages` pages each, at most.
+
+    By a model of what was measured, in us: a page keeps a warp 1.45 (heads of 128 channels; 1.0 for 64), or a multiprocessor 0.27
+    (0.16) once it has more warps than that; a call costs 4 from end to end, joining pieces 3 more, and a block 1.2 of its
+    multiprocessor's time.  More warps a block serve calls that do not fill the GPU without joining anything; pieces serve those with
+    few sequences and heads, and cut the tail of those with many."""
+    alone, shared = (1.45, 0.27) if head_dim == 128 else (1.0, 0.16)
+    most = 12 if wide == 8 else 8
+    best = (math.inf, 4, 1)
+    for warps in (4, 6, 8, 12):
+        if warps > most:
+            continue
+        room = sms * (most // warps)
+        for pieces in {1, 2, 3, room // units, sms // units}:
+            if pieces < 1 or (pieces > 1 and (pieces - 1) * 4 >= pages) or pieces > 1024:
+                continue
+            blocks, rounds = units * pieces, -(-(-(-pages // pieces)) // warps)
+            join = 3.0 if pieces > 1 else 0.0
+            if blocks <= room:
+                cost = 4.0 + join + rounds * max(alone, shared * warps * -(-blocks // sms))
+            else:
+                cost = 4.0 + join + (units * pages * shared + blocks * 1.2) / sms + 0.25 * rounds * max(alone, shared * most)
+            best = min(best, (cost, warps, pieces))
+    return best[1], best[2]
 
 
 def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
-    """Which kernel takes a step of these sizes in bfloat16, its pieces of the keys, and the scratch that joining them takes.
+    """Which kernel takes a step of these sizes in bfloat16, its warps a block (few tokens), its pieces of the keys, and the scratch
+    that joining them takes: for the step itself, and for any of the same heads with fewer sequences or shorter ones.
 
     "few": up to 16 columns (query heads of a key head, times new tokens) a key head, in blocks of 8 or 16; "many": blocks of 256 of them."""
     if head_dim != 64 and head_dim != 128:
-        return "any", 1, 0
+        return "any", 0, 1, 0, 0
     columns = max_new * (n_heads // n_kv_heads)
     units = max(1, n_seqs * n_kv_heads)
     span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
+    sms = _sm_count()
     if columns <= 16:
-        # blocks to fill the GPU, three a multiprocessor; a warp of a block's four takes a page at least
-        splits = max(1, min(-(-SPLIT_X * _sm_count() // units), -(-span // (4 * PAGE_SIZE)), 1024))
-        return "few", splits, units * splits * (8 if columns <= 8 else 16) * (head_dim + 2) if splits > 1 else 0
+        wide = 8 if columns <= 8 else 16
+        pages = max(1, -(-span // PAGE_SIZE))
+        warps, pieces = _cache4_few(sms, units, pages, wide, head_dim)
+        one = wide * (head_dim + 2)
+        most = min(max(3 * sms, 3 * units), units * -(-pages // 4))
+        return "few", warps, pieces, units * pieces * one if pieces > 1 else 0, most * one
     tiles = -(-columns // 256)
     # a block a multiprocessor; pieces of eight tiles of 128 keys at least
-    splits = max(1, min(_sm_count() // (units * tiles), -(-span // 1024)))
-    return "many", splits, units * tiles * splits * 256 * (head_dim + 2) if splits > 1 else 0
+    pieces = max(1, min(sms // (units * tiles), -(-span // 1024)))
+    one = 256 * (head_dim + 2)
+    return "many", 0, pieces, units * tiles * pieces * one if pieces > 1 else 0, min(sms, units * tiles * -(-span // 1024)) * one
 
 
 def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
@@ -2151,9 +2184,10 @@ def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, windo
 
 
 def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window=0, keep_first=0) -> int:
-    """32-bit words of `scratch` that cache4_attention wants for a step of these sizes."""
+    """32-bit words of `scratch` that cache4_attention wants for a step of these sizes, and at most for one of fewer or shorter
+    sequences with as many new tokens."""
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
-    return _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)[2]
+    return _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)[4]
 
 
 def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads,
@@ -2182,9 +2216,9 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
-    kind, splits, floats = "any", 1, 0
+    kind, warps, splits, floats = "any", 0, 1, 0
     if impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0:
-        kind, splits, floats = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
+        kind, warps, splits, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
     partial = 0
     if floats:
         if scratch is None:
@@ -2195,7 +2229,7 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     head = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
             _status_address(device), starts, pasts, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, window, keep_first)
     if kind == "few":
-        _check(library().bt_cache4_decode(*head, splits, partial, floats, _raw_stream(device)))
+        _check(library().bt_cache4_decode(*head, splits, warps, partial, floats, _raw_stream(device)))
     elif kind == "many":
         _check(library().bt_cache4_prompt(*head, splits, partial, floats, _raw_stream(device)))
     else:
