@@ -4,48 +4,59 @@
 // round(x / s), ties to even, at most 7 in size: all decided exactly, so that the result does not depend on how a division rounds.
 // A group that holds an infinity or NaN is filed as NaN.  Values beyond what the format holds (25,088) are held as its largest.
 //
-// Both are bound by memory and, for a decode step, by latency: four lanes share a group, a lane moves 8 channels in 16-byte pieces
-// (32-bit inputs: two), and the four bytes of codes beside its neighbours'.  A block takes several tokens, a thread the same 8
-// channels of each, so that their loads are in flight together.
+// Both are bound by memory and, for a decode step, by latency.  Four lanes share a group, a lane moves 8 channels in 16-byte pieces (32-bit
+// inputs: two) and the four bytes of their codes beside its neighbours'.  A block takes several tokens, a thread the same 8 channels of each,
+// four of them in flight; where a token's records lie is looked up once a block, while the first rows come.
 #include "cache4.cuh"
+#include "cache4_codes.cuh"
 
 namespace bt {
 
-constexpr int C4_THREADS = 256;
+constexpr int C4_THREADS = 256, C4_AHEAD = 4;
 
 struct Cache4Rows {
   long long k_row, k_head, v_row, v_head;      // elements between tokens and between heads
 };
+struct Cache4Where {
+  const int *positions, *token_seq, *ctx_len;
+  int n_tokens, n_table;
+};
 
+// 8 channels as they lie in memory, and as numbers.
 template <typename T, bool VEC>
-__device__ __forceinline__ void c4_load8(const T* p, float (&x)[8]) {
-  if constexpr (!VEC) {
+struct C4Row {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float(p[i]);
-  } else if constexpr (sizeof(T) == 2) {
-    unpack16(*reinterpret_cast<const uint4*>(p), x);
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      T* x = reinterpret_cast<T*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
   }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void c4_store8(T* p, const float (&x)[8]) {
-  if constexpr (!VEC) {
+  // the largest of the 8 without their signs, as a 32-bit number's bits (above 0x7f800000: NaN)
+  __device__ __forceinline__ unsigned top() const {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned m = 0x7fff7fffu, a = __vmaxu2(__vmaxu2(v[0].x & m, v[0].y & m), __vmaxu2(v[0].z & m, v[0].w & m));
+      return max(a << 16, a & 0xffff0000u);
+    } else {
+      unsigned t = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = from_float<T>(x[i]);
-  } else if constexpr (sizeof(T) == 2) {
-    __nv_bfloat162 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);      // (exact: the values have 7 bits)
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-  } else {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      for (int i = 0; i < 8; ++i) t = max(t, reinterpret_cast<const unsigned*>(v)[i] & 0x7fffffffu);
+      return t;
+    }
   }
-}
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned w = reinterpret_cast<const unsigned*>(v)[i >> 1];
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    } else {
+      return __uint_as_float(reinterpret_cast<const unsigned*>(v)[i]);
+    }
+  }
+};
 
 // The smallest scale byte with 7 s >= top (finite, not negative); 254 where none has.
 __device__ __forceinline__ int c4_scale_byte(float top) {
@@ -57,13 +68,13 @@ __device__ __forceinline__ int c4_scale_byte(float top) {
   return b;
 }
 
-// round(x / s) + 8, ties to even, in the last four bits.  `inv`: 1 / s rounded.
+// round(x / s), ties to even, plus a constant: the bits of a sum that rounds to whole numbers.  `inv`: 1 / s, nearly.
 // bfloat16 x: the corrected quotient is x / s rounded to 24 bits, which is no tie unless x / s is one (x and (k + 1/2) s have 8
 // significant bits each, so that they are equal or differ by more than 2^-9 of x).  32-bit x may lie closer to a tie than a quotient
 // tells: the rest x - r s, which is exact, says on which side.
+constexpr unsigned kC4Whole = 0x4b400000u;       // 1.5 x 2^23
 template <typename T>
 __device__ __forceinline__ unsigned c4_code(float x, float s, float inv) {
-  constexpr float kMagic = 12582912.f;         // 1.5 x 2^23: a sum with it rounds to whole numbers
   float r = x * inv;
   r = fmaf(fmaf(-r, s, x), inv, r);
   if constexpr (sizeof(T) == 4) {
@@ -72,116 +83,143 @@ __device__ __forceinline__ unsigned c4_code(float x, float s, float inv) {
     const bool odd = (int)fminf(fmaxf(r, -8.f), 8.f) & 1;
     if (fabsf(rest) > half || (fabsf(rest) == half && odd)) r += rest > 0.f ? 1.f : -1.f;
   }
-  return __float_as_uint(r + (kMagic + 8.f)) & 15u;
+  return __float_as_uint(r + __uint_as_float(kC4Whole + 8u));
 }
 
-// grid (blocks of tokens, pieces of a token's lanes); a lane: (head, key or value, 8 channels)
-template <typename T, bool VEC, int TOKENS>
-__global__ void __launch_bounds__(C4_THREADS)
-cache4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Cache4Rows rows, Cache4View c, const int* __restrict__ positions,
-                     const int* __restrict__ token_seq, const int* __restrict__ ctx_len, int n_tokens, int n_table, int dim) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = blockIdx.y * C4_THREADS + threadIdx.x;
-  const int eighths = dim / 8;
-  const int head = lane / (2 * eighths);
-  if (head >= c.n_kv_heads) return;            // (whole groups of four lanes: dim / 8 is a multiple of 4)
-  const int which = lane / eighths & 1, at = lane % eighths;
-  const unsigned quad = 0xfu << (threadIdx.x & 28);
-  const T* src = which ? v + head * rows.v_head : k + head * rows.k_head;
-  const long long row = which ? rows.v_row : rows.k_row;
-  const int t0 = blockIdx.x * TOKENS;
-  float x[TOKENS][8];
-  unsigned char* rec[TOKENS];                  // null: not filed
-  int in_page[TOKENS];
-#pragma unroll
-  for (int i = 0; i < TOKENS; ++i)
-    if (t0 + i < n_tokens) c4_load8<T, VEC>(src + (t0 + i) * row + at * 8, x[i]);
-#pragma unroll
-  for (int i = 0; i < TOKENS; ++i) {
-    rec[i] = nullptr;
-    in_page[i] = 0;
-    if (t0 + i >= n_tokens) continue;
-    const int seq = token_seq[t0 + i], pos = positions[t0 + i];
-    if (seq < 0 || seq >= n_table || pos < 0) {
-      if (c.status) atomicExch(c.status, 9);
-      continue;
-    }
+// Where the tokens t0 .. of a block lie: the byte offset of their page in the pool and their place in it, -1 for one that is not there.
+template <int TOKENS>
+__device__ __forceinline__ void c4_look_up(const Cache4View& c, const Cache4Where& at, int t0, int dim, bool ring, long long* s_page, int* s_row) {
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  if (tid < TOKENS && t0 + tid < at.n_tokens) {
+    const int seq = at.token_seq[t0 + tid], pos = at.positions[t0 + tid];
+    long long page = -1;
+    bool bad = seq < 0 || seq >= at.n_table || pos < 0;
     // (in a ring only the newest positions that it holds are written, so that no two tokens of a step meet)
-    if ((long long)pos < (long long)ctx_len[seq] - (long long)c.table_len * C4_PAGE) continue;
-    const int page = c.table[(long long)seq * c.table_stride + pos / C4_PAGE % c.table_len];
-    if (page < 0 || page >= c.n_pages) {
-      if (c.status) atomicExch(c.status, 9);
-      continue;
+    if (!bad && !(ring && (long long)pos < (long long)at.ctx_len[seq] - (long long)c.table_len * C4_PAGE)) {
+      int entry = pos / C4_PAGE;
+      if (entry >= c.table_len) entry %= c.table_len;
+      page = c.table[(long long)seq * c.table_stride + entry];
+      if (page < 0 || page >= c.n_pages) {
+        bad = true;
+        page = -1;
+      }
     }
-    in_page[i] = pos % C4_PAGE;
-    rec[i] = c.pool + ((long long)page * c.n_kv_heads + head) * c4_record(dim);
+    if (bad && c.status) atomicExch(c.status, 9);
+    s_page[tid] = page < 0 ? -1 : page * c.n_kv_heads * c4_record(dim);
+    s_row[tid] = pos % C4_PAGE;
   }
+}
+
+// block (lanes of a head: keys' pieces of 8 channels, then values'; heads); grid (blocks of tokens, blocks of heads)
+template <typename T, bool VEC, int TOKENS>
+__global__ void __launch_bounds__(C4_THREADS)
+cache4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Cache4Rows rows, Cache4View c, Cache4Where where, int dim) {
+  __shared__ long long s_page[TOKENS];
+  __shared__ int s_row[TOKENS];
+  pdl_trigger();
+  pdl_wait();
+  const int eighths = dim / 8, which = (int)threadIdx.x >= eighths, at = (int)threadIdx.x - which * eighths;
+  const int head = blockIdx.y * blockDim.y + threadIdx.y, t0 = blockIdx.x * TOKENS;
+  const bool mine = head < c.n_kv_heads;
+  const long long row = which ? rows.v_row : rows.k_row;
+  const T* src = (which ? v + head * rows.v_head : k + head * rows.k_head) + at * 8;
+  constexpr int AHEAD = TOKENS < C4_AHEAD ? TOKENS : C4_AHEAD;
+  C4Row<T, VEC> x[AHEAD];
+  auto fetch = [&](int first) {
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i) {
-    if (rec[i] == nullptr) continue;           // (the same in the four lanes)
-    unsigned top = 0;
+    for (int i = 0; i < AHEAD; ++i)
+      if (mine && t0 + first + i < where.n_tokens) x[i].load(src + (t0 + first + i) * row);
+  };
+  fetch(0);
+  c4_look_up<TOKENS>(c, where, t0, dim, true, s_page, s_row);
+  __syncthreads();
+  if (!mine) return;                           // (whole groups of four lanes: dim / 8 is a multiple of 4)
+  const unsigned quad = 0xfu << ((threadIdx.y * blockDim.x + threadIdx.x) & 28);
+  unsigned char* const codes = c.pool + (long long)head * c4_record(dim) + which * c4_value_codes(dim) + at * 4;
+  unsigned char* const scales = c.pool + (long long)head * c4_record(dim) + c4_key_scales(dim) + which * (2 * dim) + at / 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[i][j]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(quad, top, 1));
-    top = max(top, __shfl_xor_sync(quad, top, 2));
-    const bool fine = top < 0x7f800000u;
-    const int b = fine ? c4_scale_byte(__uint_as_float(top)) : 255;
-    const float s = c4_scale((unsigned)b), inv = 1.f / s;
-    if (b == 254) {                            // the largest scale: what its seventh multiple does not reach stays at it
+  for (int first = 0; first < TOKENS; first += AHEAD) {
+    if (first > 0) fetch(first);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = fminf(fmaxf(x[i][j], -7.f * s), 7.f * s);
+    for (int i = 0; i < AHEAD; ++i) {
+      const int t = first + i;
+      if (t0 + t >= where.n_tokens || s_page[t] < 0) continue;      // (the same in the four lanes)
+      unsigned top = x[i].top();
+      top = max(top, __shfl_xor_sync(quad, top, 1));
+      top = max(top, __shfl_xor_sync(quad, top, 2));
+      const bool fine = top < 0x7f800000u;
+      const int b = fine ? c4_scale_byte(__uint_as_float(top)) : 255;
+      const float s = c4_scale((unsigned)b), inv = __frcp_rn(s);
+      const float most = b == 254 ? 7.f * s : INFINITY;      // the largest scale: what its seventh multiple does not reach stays at it
+      unsigned word = 0;
+      if (b == 254) {
+#pragma unroll
+        for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(fminf(fmaxf(x[i].at(j), -most), most), s, inv);
+      } else {
+#pragma unroll
+        for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(x[i].at(j), s, inv);
+      }
+      word = fine ? word - 0x11111111u * kC4Whole : 0x88888888u;
+      *reinterpret_cast<unsigned*>(codes + s_page[t] + s_row[t] * (dim / 2)) = word;
+      if ((at & 3) == 0) scales[s_page[t] + s_row[t] * (dim / 32)] = (unsigned char)b;
     }
-    unsigned word = 0;
-#pragma unroll
-    for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(x[i][j], s, inv);
-    if (!fine) word = 0x88888888u;
-    *reinterpret_cast<unsigned*>(rec[i] + which * c4_value_codes(dim) + in_page[i] * (dim / 2) + at * 4) = word;
-    if ((at & 3) == 0) rec[i][c4_key_scales(dim) + which * (2 * dim) + in_page[i] * (dim / 32) + at / 4] = (unsigned char)b;
   }
 }
 
 template <typename T, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(C4_THREADS)
-cache4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Cache4Rows rows, Cache4View c, const int* __restrict__ positions,
-                     const int* __restrict__ token_seq, int n_tokens, int n_table, int dim) {
+cache4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Cache4Rows rows, Cache4View c, Cache4Where where, int dim) {
+  __shared__ long long s_page[TOKENS];
+  __shared__ int s_row[TOKENS];
   pdl_trigger();
   pdl_wait();
-  const int lane = blockIdx.y * C4_THREADS + threadIdx.x;
-  const int eighths = dim / 8;
-  const int head = lane / (2 * eighths), t0 = blockIdx.x * TOKENS;
+  const int eighths = dim / 8, which = (int)threadIdx.x >= eighths, at = (int)threadIdx.x - which * eighths;
+  const int head = blockIdx.y * blockDim.y + threadIdx.y, t0 = blockIdx.x * TOKENS;
+  c4_look_up<TOKENS>(c, where, t0, dim, false, s_page, s_row);
+  __syncthreads();
   if (head >= c.n_kv_heads) return;
-  const int which = lane / eighths & 1, at = lane % eighths;
-  T* dst = (which ? v + head * rows.v_head : k + head * rows.k_head) + at * 8;
+  const unsigned char* const codes = c.pool + (long long)head * c4_record(dim) + which * c4_value_codes(dim) + at * 4;
+  const unsigned char* const scales = c.pool + (long long)head * c4_record(dim) + c4_key_scales(dim) + which * (2 * dim) + at / 4;
   const long long row = which ? rows.v_row : rows.k_row;
+  T* dst = (which ? v + head * rows.v_head : k + head * rows.k_head) + at * 8 + t0 * row;
+  const C4Bits bits;
   unsigned word[TOKENS], b[TOKENS];
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i) {
-    word[i] = 0;
-    b[i] = 255u;
-    if (t0 + i >= n_tokens) continue;
-    const int seq = token_seq[t0 + i], pos = positions[t0 + i];
-    int page = -1;
-    if (seq >= 0 && seq < n_table && pos >= 0) page = c.table[(long long)seq * c.table_stride + pos / C4_PAGE % c.table_len];
-    if (page < 0 || page >= c.n_pages) {
-      if (c.status) atomicExch(c.status, 9);
-      continue;
+  for (int t = 0; t < TOKENS; ++t) {
+    word[t] = 0;
+    b[t] = 255u;
+    if (t0 + t < where.n_tokens && s_page[t] >= 0) {
+      word[t] = *reinterpret_cast<const unsigned*>(codes + s_page[t] + s_row[t] * (dim / 2));
+      b[t] = scales[s_page[t] + s_row[t] * (dim / 32)];
     }
-    const int in_page = pos % C4_PAGE;
-    const unsigned char* rec = c.pool + ((long long)page * c.n_kv_heads + head) * c4_record(dim);
-    word[i] = *reinterpret_cast<const unsigned*>(rec + which * c4_value_codes(dim) + in_page * (dim / 2) + at * 4);
-    b[i] = rec[c4_key_scales(dim) + which * (2 * dim) + in_page * (dim / 32) + at / 4];
   }
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i) {
-    if (t0 + i >= n_tokens) break;
-    const float s = c4_scale(b[i]);
-    float x[8];
+  for (int t = 0; t < TOKENS; ++t) {
+    if (t0 + t >= where.n_tokens) break;
+    const unsigned s = c4_scale_bits(b[t]), s2 = s | s << 16, shift = c4_shift(s2);
+    const unsigned p0 = c4_fma2(c4_pair<0>(word[t], bits), s2, shift), p1 = c4_fma2(c4_pair<1>(word[t], bits), s2, shift);
+    const unsigned p2 = c4_fma2(c4_pair<2>(word[t], bits), s2, shift), p3 = c4_fma2(c4_pair<3>(word[t], bits), s2, shift);
+    // a pair is channels i and i + 4
+    const uint4 y = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+    if constexpr (sizeof(T) == 2 && VEC) {
+      *reinterpret_cast<uint4*>(dst) = y;
+    } else {
+      float x[8];
+      unpack16(y, x);
+      if constexpr (VEC) {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)((int)(word[i] >> (4 * j) & 15u) - 8) * s;
-    c4_store8<T, VEC>(dst + (t0 + i) * row, x);
+        for (int j = 0; j < 8; ++j) dst[j] = from_float<T>(x[j]);
+      }
+    }
+    dst += row;
   }
 }
+
+// Blocks of one token up to here, of eight above: fewer would leave multiprocessors idle.
+constexpr int C4_MANY = 2048;
 
 static int c4_check(const char* what, const void* pool, long long n_pages, const int* table, int table_len, int n_tokens, int n_kv_heads,
                     int dim) {
@@ -211,20 +249,19 @@ extern "C" int bt_cache4_append(const void* k, long long k_row, long long k_head
   if (n_tokens == 0) return 0;
   const Cache4Rows rows{k_row, k_head, v_row, v_head};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
-  const int lanes = n_kv_heads * dim / 4, pieces = (lanes + C4_THREADS - 1) / C4_THREADS;
+  const Cache4Where where{positions, token_seq, ctx_len, n_tokens, n_table};
   const bool vec = c4_whole(k, v, rows, dtype == kF32 ? 4 : 2);
-  // several tokens a block once there are enough of them to fill the GPU
-  const bool many = (long long)n_tokens * pieces > 4096;
-  const int per = many ? 4 : 1;
-  const dim3 grid((n_tokens + per - 1) / per, pieces);
-#define BT_C4_APPEND(T, VEC, TOK)                                                                                                     \
-  BT_PDL_OK("cache4_append", launch_pdl(cache4_append_kernel<T, VEC, TOK>, grid, dim3(C4_THREADS), 0, stream, 1, (const T*)k, (const T*)v, \
-                                        rows, c, positions, token_seq, ctx_len, n_tokens, n_table, dim))
+  const dim3 block(dim / 4, C4_THREADS / (dim / 4));
+  const int pieces = (n_kv_heads + (int)block.y - 1) / (int)block.y;
+  const bool many = (long long)n_tokens * pieces > C4_MANY;
+#define BT_C4_APPEND(T, VEC, TOK)                                                                                                         \
+  BT_PDL_OK("cache4_append", launch_pdl(cache4_append_kernel<T, VEC, TOK>, dim3((n_tokens + TOK - 1) / TOK, pieces), block, 0, stream, 1, \
+                                        (const T*)k, (const T*)v, rows, c, where, dim))
 #define BT_C4_APPEND_T(T)                                                          \
   if (vec) {                                                                       \
-    if (many) BT_C4_APPEND(T, true, 4); else BT_C4_APPEND(T, true, 1);             \
+    if (many) BT_C4_APPEND(T, true, 8); else BT_C4_APPEND(T, true, 1);             \
   } else {                                                                         \
-    if (many) BT_C4_APPEND(T, false, 4); else BT_C4_APPEND(T, false, 1);           \
+    if (many) BT_C4_APPEND(T, false, 8); else BT_C4_APPEND(T, false, 1);           \
   }
   if (dtype == kF32) {
     BT_C4_APPEND_T(float)
@@ -246,19 +283,19 @@ extern "C" int bt_cache4_gather(void* k, long long k_row, long long k_head, void
   if (n_tokens == 0) return 0;
   const Cache4Rows rows{k_row, k_head, v_row, v_head};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
-  const int lanes = n_kv_heads * dim / 4;
+  const Cache4Where where{positions, token_seq, nullptr, n_tokens, n_table};
   const bool vec = c4_whole(k, v, rows, dtype == kF32 ? 4 : 2);
-  const int pieces = (lanes + C4_THREADS - 1) / C4_THREADS;
-  const bool many = (long long)n_tokens * pieces > 4096;
-  const dim3 grid(many ? (n_tokens + 3) / 4 : n_tokens, pieces);
-#define BT_C4_GATHER(T, VEC, TOK)                                                                                                   \
-  BT_PDL_OK("cache4_gather", launch_pdl(cache4_gather_kernel<T, VEC, TOK>, grid, dim3(C4_THREADS), 0, stream, 1, (T*)k, (T*)v, rows, c, \
-                                        positions, token_seq, n_tokens, n_table, dim))
+  const dim3 block(dim / 4, C4_THREADS / (dim / 4));
+  const int pieces = (n_kv_heads + (int)block.y - 1) / (int)block.y;
+  const bool many = (long long)n_tokens * pieces > C4_MANY;
+#define BT_C4_GATHER(T, VEC, TOK)                                                                                                         \
+  BT_PDL_OK("cache4_gather", launch_pdl(cache4_gather_kernel<T, VEC, TOK>, dim3((n_tokens + TOK - 1) / TOK, pieces), block, 0, stream, 1, \
+                                        (T*)k, (T*)v, rows, c, where, dim))
 #define BT_C4_GATHER_T(T)                                                          \
   if (vec) {                                                                       \
-    if (many) BT_C4_GATHER(T, true, 4); else BT_C4_GATHER(T, true, 1);             \
+    if (many) BT_C4_GATHER(T, true, 8); else BT_C4_GATHER(T, true, 1);             \
   } else {                                                                         \
-    if (many) BT_C4_GATHER(T, false, 4); else BT_C4_GATHER(T, false, 1);           \
+    if (many) BT_C4_GATHER(T, false, 8); else BT_C4_GATHER(T, false, 1);           \
   }
   if (dtype == kF32) {
     BT_C4_GATHER_T(float)

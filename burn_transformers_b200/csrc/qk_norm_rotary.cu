@@ -6,9 +6,9 @@
 // there, so that far positions lose nothing (a 32-bit product is off by pos * f / 2^24: 0.06 at position 10^6).
 //
 // Bound by memory: every channel is read and written once.  A warp takes one token and some of its heads.  Its lanes form the token's cosines
-// and sines once, in shared memory, and keep the eight pairs that a lane turns in registers; a lane holds 16 channels of a head (the
-// two pieces of 8 that turn into one another, or 16 in a row), so that nothing but the norm's sum goes between lanes.  How many heads
-// a warp takes: all of them when there are enough tokens to fill the GPU, as few as fit its lanes when there are not.
+// and sines once, in shared memory, and a lane keeps what its eight pairs are multiplied by in registers; it holds 16 channels of a head
+// (the two pieces of 8 that turn into one another, or 16 in a row), so that nothing but the norm's sum goes between lanes.  How many
+// heads a warp takes: all of them when there are enough tokens to fill the GPU, as few as fit its lanes when there are not.
 #include "common.cuh"
 
 namespace bt {
@@ -37,39 +37,66 @@ __device__ __forceinline__ float2 qn_turn(int pos, float f, float size) {
   return make_float2(c * size, s * size);
 }
 
-// 8 channels as they lie in memory, and as numbers.
+// 16 channels of a lane, in two pieces of 8 as they lie in memory.
 template <typename T>
 struct QnRaw {
-  uint4 v[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+  uint4 v[sizeof(T)];
+  __device__ __forceinline__ void load(const T* a, const T* b) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      v[i] = reinterpret_cast<const uint4*>(a)[i];
+      v[i + sizeof(T) / 2] = reinterpret_cast<const uint4*>(b)[i];
+    }
   }
-  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+  __device__ __forceinline__ void store(T* a, T* b) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      reinterpret_cast<uint4*>(a)[i] = v[i];
+      reinterpret_cast<uint4*>(b)[i] = v[i + sizeof(T) / 2];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {      // i: 0 .. 15
     if constexpr (sizeof(T) == 2) {
-      unpack16(v[0], x);
+      const unsigned w = reinterpret_cast<const unsigned*>(v)[i >> 1];
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     } else {
-      x[0] = __uint_as_float(v[0].x); x[1] = __uint_as_float(v[0].y); x[2] = __uint_as_float(v[0].z); x[3] = __uint_as_float(v[0].w);
-      x[4] = __uint_as_float(v[1].x); x[5] = __uint_as_float(v[1].y); x[6] = __uint_as_float(v[1].z); x[7] = __uint_as_float(v[1].w);
+      return __uint_as_float(reinterpret_cast<const unsigned*>(v)[i]);
+    }
+  }
+  __device__ __forceinline__ void set(int i, float x, float y) {      // channels i (even), i + 1
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      reinterpret_cast<unsigned*>(v)[i >> 1] = *reinterpret_cast<const unsigned*>(&h);
+    } else {
+      reinterpret_cast<unsigned*>(v)[i] = __float_as_uint(x);
+      reinterpret_cast<unsigned*>(v)[i + 1] = __float_as_uint(y);
     }
   }
 };
-template <typename T>
-__device__ __forceinline__ void qn_store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    __nv_bfloat162 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-  } else {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  }
+
+// Pairs of 32-bit numbers in one register pair: one instruction for two multiply-adds, each rounded as by itself.
+__device__ __forceinline__ unsigned long long qn_two(float a, float b) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void qn_halves(unsigned long long v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long qn_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long qn_mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
-// LANES: lanes a head (a power of two, 16 channels each; those past the head's channels idle).
-template <typename T, int LANES>
-__global__ void __launch_bounds__(QN_WARPS * 32)
+// LANES: lanes a head (a power of two, 16 channels each; those past the head's channels idle).  NEAR: neighbours turn into one another.
+// A lane's 16 channels are 8 pairs (u, v) that turn: u' = r (u w_u c - v w_v s), v' = r (v w_v c + u w_u s), r the norm's factor; the products
+// of weights with cosines and sines are the same for all heads of a token (queries, then keys).
+template <typename T, int LANES, bool NEAR>
+__global__ void __launch_bounds__(QN_WARPS * 32, 3)
 qk_norm_rotary_kernel(QnParams p) {
   __shared__ float2 s_turn[QN_WARPS][128];
   pdl_trigger();
@@ -80,86 +107,94 @@ qk_norm_rotary_kernel(QnParams p) {
   if (token >= p.n_tokens) return;
   const int pos = p.positions[token];
   // this lane's two pieces of 8 channels: pieces that turn into one another, or (past the turned ones, and for neighbours) in a row
-  const int c = lane % LANES, sub = lane / LANES, pairs = p.interleaved ? 0 : p.rot / 16;
+  const int c = lane % LANES, sub = lane / LANES, pairs = NEAR ? 0 : p.rot / 16;
   const bool mine = 16 * c < p.dim, turned = 16 * c < p.rot;
   const int a = c < pairs ? 8 * c : 16 * c, b = c < pairs ? 8 * (c + pairs) : 16 * c + 8;
   const int first = part * p.vecs_per_warp, last = min(p.n_vecs, first + p.vecs_per_warp);
   const T* src = reinterpret_cast<const T*>(p.src) + token * p.src_row;
   T* dst = reinterpret_cast<T*>(p.dst) + token * p.dst_row;
   // the next heads are asked for before the ones at hand are worked on (the first before the angles)
-  QnRaw<T> next_x, next_y;
+  QnRaw<T> next;
   auto fetch = [&](int v) {
-    if (mine && v < last) {
-      next_x.load(src + (long long)v * p.dim + a);
-      next_y.load(src + (long long)v * p.dim + b);
-    }
+    if (mine && v < last) next.load(src + v * p.dim + a, src + v * p.dim + b);
   };
   fetch(first + sub);
   float2* turn = s_turn[warp];
   for (int i = lane; i < p.rot / 2; i += 32) turn[i] = qn_turn(pos, p.freq[i], p.size);
   __syncwarp();
-  float cs[8], sn[8];
+  // w_u c, -w_v s, w_v c, w_u s of two pairs each
+  unsigned long long uc[4], vs[4], vc[4], us[4];
+  auto weigh = [&](const float* weight) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 w = turned ? turn[8 * c + i] : make_float2(1.f, 0.f);
-    cs[i] = w.x;
-    sn[i] = w.y;
-  }
-  float wa[8], wb[8];
-  const float* held = nullptr;
+    for (int j = 0; j < 8; j += 2) {
+      float f[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = j + e, u = NEAR ? 16 * c + 2 * i : a + i, v = NEAR ? 16 * c + 2 * i + 1 : b + i;
+        const float2 w = turned ? turn[8 * c + i] : make_float2(1.f, 0.f);
+        const float wu = p.normed ? weight[u] : 1.f, wv = p.normed ? weight[v] : 1.f;
+        f[e][0] = wu * w.x;
+        f[e][1] = -wv * w.y;
+        f[e][2] = wv * w.x;
+        f[e][3] = wu * w.y;
+      }
+      uc[j / 2] = qn_two(f[0][0], f[1][0]);
+      vs[j / 2] = qn_two(f[0][1], f[1][1]);
+      vc[j / 2] = qn_two(f[0][2], f[1][2]);
+      us[j / 2] = qn_two(f[0][3], f[1][3]);
+    }
+  };
+  const float per_channel = 1.f / (float)p.dim;
+  int kind = -1;                       // whose weights those are
   for (int v0 = first; v0 < last; v0 += 32 / LANES) {
     const int v = v0 + sub;
     const bool here = mine && v < last;
-    float x[8], y[8];
-    if (here) {
-      next_x.unpack(x);
-      next_y.unpack(y);
-    }
+    const QnRaw<T> at = next;
     fetch(v + 32 / LANES);
-    if (p.normed) {
-      float sum = 0.f;
-      if (here) {
+    unsigned long long u2[4], v2[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
-      }
+    for (int j = 0; j < 4; ++j) {
+      u2[j] = NEAR ? qn_two(at.at(4 * j), at.at(4 * j + 2)) : qn_two(at.at(2 * j), at.at(2 * j + 1));
+      v2[j] = NEAR ? qn_two(at.at(4 * j + 1), at.at(4 * j + 3)) : qn_two(at.at(8 + 2 * j), at.at(8 + 2 * j + 1));
+    }
+    float r = 1.f;
+    if (p.normed) {
+      unsigned long long sum2 = 0ull;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum2 = qn_fma2(u2[j], u2[j], qn_fma2(v2[j], v2[j], sum2));
+      float x, y;
+      qn_halves(sum2, x, y);
+      float sum = here ? x + y : 0.f;
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(sum / (float)p.dim + p.eps);
-      const float* weight = v < p.n_heads ? p.q_weight : p.k_weight;
-      if (here && weight != held) {
-        QnRaw<float> w;
-        w.load(weight + a);
-        w.unpack(wa);
-        w.load(weight + b);
-        w.unpack(wb);
-        held = weight;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= r * wa[i];
-        y[i] *= r * wb[i];
-      }
+      r = rsqrtf(fmaf(sum, per_channel, p.eps));
     }
     if (!here) continue;
-    if (p.interleaved) {
+    if (kind != (v >= p.n_heads)) {
+      kind = v >= p.n_heads;
+      weigh(kind ? p.k_weight : p.q_weight);
+    }
+    const unsigned long long r2 = qn_two(r, r);
+    QnRaw<T> done;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = x[2 * i], w = x[2 * i + 1], g = y[2 * i], h = y[2 * i + 1];
-        x[2 * i] = u * cs[i] - w * sn[i];
-        x[2 * i + 1] = w * cs[i] + u * sn[i];
-        y[2 * i] = g * cs[4 + i] - h * sn[4 + i];
-        y[2 * i + 1] = h * cs[4 + i] + g * sn[4 + i];
+    for (int j = 0; j < 4; ++j) {
+      unsigned long long u = qn_mul2(u2[j], uc[j]), w = qn_mul2(v2[j], vc[j]);
+      if (turned) {                    // (elsewhere an infinity beside a zero would become NaN)
+        u = qn_fma2(v2[j], vs[j], u);
+        w = qn_fma2(u2[j], us[j], w);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float u = x[i], w = y[i];
-        x[i] = u * cs[i] - w * sn[i];
-        y[i] = w * cs[i] + u * sn[i];
+      float x0, x1, y0, y1;
+      qn_halves(qn_mul2(u, r2), x0, x1);
+      qn_halves(qn_mul2(w, r2), y0, y1);
+      if (NEAR) {
+        done.set(4 * j, x0, y0);
+        done.set(4 * j + 2, x1, y1);
+      } else {
+        done.set(2 * j, x0, x1);
+        done.set(8 + 2 * j, y0, y1);
       }
     }
-    qn_store8<T>(dst + (long long)v * p.dim + a, x);
-    qn_store8<T>(dst + (long long)v * p.dim + b, y);
+    done.store(dst + v * p.dim + a, dst + v * p.dim + b);
   }
 }
 
@@ -221,13 +256,20 @@ static int launch_qn(QnParams p, bool whole, cudaStream_t stream) {
     const long long blocks = ((long long)p.n_tokens * p.warps_per_token + QN_WARPS - 1) / QN_WARPS;
     BT_CHECK(blocks < (1ll << 31), "qk_norm_rotary: %d tokens of %d heads are too many for one launch", p.n_tokens, p.n_vecs);
     const dim3 grid((unsigned)blocks), block(QN_WARPS * 32);
+#define BT_QN(LANES)                                                                                                                  \
+  if (p.interleaved)                                                                                                                  \
+    BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, LANES, true>, grid, block, 0, stream, 1, p));                     \
+  else                                                                                                                                \
+    BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, LANES, false>, grid, block, 0, stream, 1, p));                    \
+  break
     switch (lanes) {
-      case 1: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 1>, grid, block, 0, stream, 1, p)); break;
-      case 2: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 2>, grid, block, 0, stream, 1, p)); break;
-      case 4: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 4>, grid, block, 0, stream, 1, p)); break;
-      case 8: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 8>, grid, block, 0, stream, 1, p)); break;
-      default: BT_PDL_OK("qk_norm_rotary", launch_pdl(qk_norm_rotary_kernel<T, 16>, grid, block, 0, stream, 1, p));
+      case 1: BT_QN(1);
+      case 2: BT_QN(2);
+      case 4: BT_QN(4);
+      case 8: BT_QN(8);
+      default: BT_QN(16);
     }
+#undef BT_QN
     return 0;
   }
   const long long blocks = ((long long)p.n_tokens * p.n_vecs + QN_WARPS - 1) / QN_WARPS;

@@ -2126,26 +2126,28 @@ def _sm_count() -> int:
 def _cache4_few(sms, units, pages, wide, head_dim):
     """(warps a block, pieces of the keys) for `units` blocks' worth of columns over `pages` pages each, at most.
 
-    By a model of what was measured, in us: a page keeps a warp 1.45 (heads of 128 channels; 1.0 for 64), or a multiprocessor 0.27
-    (0.16) once it has more warps than that; a call costs 4 from end to end, joining pieces 3 more, and a block 1.2 of its
-    multiprocessor's time.  More warps a block serve calls that do not fill the GPU without joining anything; pieces serve those with
-    few sequences and heads, and cut the tail of those with many."""
-    alone, shared = (1.45, 0.27) if head_dim == 128 else (1.0, 0.16)
+    By a model of what was measured, in us: with n warps on its multiprocessor a page keeps a warp 0.75 + 0.2 n (0.5 + 0.11 n with heads of
+    64 channels); a call costs 4 from end to end, joining pieces 3 more.  Calls that more than fill the GPU go by what a multiprocessor gets
+    done, a page in 0.27 (0.16), and by what a block's beginning and end take of it: 4 by itself, 1.6 beside one other, 1.2 beside two.  More
+    warps a block serve calls that do not fill the GPU without joining anything; pieces serve those with few sequences and heads."""
+    base, step, shared = (0.75, 0.2, 0.27) if head_dim == 128 else (0.5, 0.11, 0.16)
     most = 12 if wide == 8 else 8
     best = (math.inf, 4, 1)
     for warps in (4, 6, 8, 12):
         if warps > most:
             continue
-        room = sms * (most // warps)
+        side = most // warps
+        room = sms * side
         for pieces in {1, 2, 3, room // units, sms // units}:
             if pieces < 1 or (pieces > 1 and (pieces - 1) * 4 >= pages) or pieces > 1024:
                 continue
             blocks, rounds = units * pieces, -(-(-(-pages // pieces)) // warps)
-            join = 3.0 if pieces > 1 else 0.0
-            if blocks <= room:
-                cost = 4.0 + join + rounds * max(alone, shared * warps * -(-blocks // sms))
+            cost = 4.0 + (3.0 if pieces > 1 else 0.0)
+            if blocks <= 2 * room:
+                beside = min(side, -(-blocks // sms)) * warps
+                cost += -(-blocks // room) * rounds * (base + step * beside)
             else:
-                cost = 4.0 + join + (units * pages * shared + blocks * 1.2) / sms + 0.25 * rounds * max(alone, shared * most)
+                cost += units * pages * shared / sms + blocks * (4.0, 1.6, 1.2)[side - 1] / sms + 0.25 * rounds * (base + step * most)
             best = min(best, (cost, warps, pieces))
     return best[1], best[2]
 
