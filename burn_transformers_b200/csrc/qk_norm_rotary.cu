@@ -246,9 +246,9 @@ static int launch_qn(QnParams p, bool whole, cudaStream_t stream) {
   if (whole) {
     const int lanes = p.dim <= 16 ? 1 : p.dim <= 32 ? 2 : p.dim <= 64 ? 4 : p.dim <= 128 ? 8 : 16;
     const int side = 32 / lanes, rounds = (p.n_vecs + side - 1) / side;
-    // rounds a warp: all of them once the tokens alone give every multiprocessor 64 warps
-    const long long wanted = 64ll * (sm_count() > 0 ? sm_count() : 148);
-    long long split = (wanted + p.n_tokens - 1) / p.n_tokens;
+    // rounds a warp: as many as leave no more warps than run at once (three blocks a multiprocessor)
+    long long split = 3ll * QN_WARPS * (sm_count() > 0 ? sm_count() : 148) / p.n_tokens;
+    if (split < 1) split = 1;
     if (split > rounds) split = rounds;
     const int per = (int)((rounds + split - 1) / split);
     p.vecs_per_warp = per * side;

@@ -2126,8 +2126,8 @@ def _sm_count() -> int:
 def _cache4_few(sms, units, pages, wide, head_dim):
     """(warps a block, pieces of the keys) for `units` blocks' worth of columns over `pages` pages each, at most.
 
-    By a model of what was measured, in us: with n warps on its multiprocessor a page keeps a warp 0.75 + 0.2 n (0.5 + 0.11 n with heads of
-    64 channels); a call costs 4 from end to end, joining pieces 3 more.  Calls that more than fill the GPU go by what a multiprocessor gets
+    By a model of what was measured, in us: with n warps on its multiprocessor, in fours, a page keeps a warp 0.75 + 0.2 n (0.5 + 0.11 n with
+    heads of 64 channels); a call costs 4 from end to end, joining pieces 3 more.  Calls that more than fill the GPU go by what a multiprocessor gets
     done, a page in 0.27 (0.16), and by what a block's beginning and end take of it: 4 by itself, 1.6 beside one other, 1.2 beside two.  More
     warps a block serve calls that do not fill the GPU without joining anything; pieces serve those with few sequences and heads."""
     base, step, shared = (0.75, 0.2, 0.27) if head_dim == 128 else (0.5, 0.11, 0.16)
@@ -2145,7 +2145,7 @@ def _cache4_few(sms, units, pages, wide, head_dim):
             cost = 4.0 + (3.0 if pieces > 1 else 0.0)
             if blocks <= 2 * room:
                 beside = min(side, -(-blocks // sms)) * warps
-                cost += -(-blocks // room) * rounds * (base + step * beside)
+                cost += -(-blocks // room) * rounds * (base + step * 4 * -(-beside // 4))
             else:
                 cost += units * pages * shared / sms + blocks * (4.0, 1.6, 1.2)[side - 1] / sms + 0.25 * rounds * (base + step * most)
             best = min(best, (cost, warps, pieces))
