@@ -7,10 +7,10 @@
 //   0, 1  softmax, a thread a row of tile 0 or 1: scores from tensor memory into registers, running maximum and sum in 32-bit, weights
 //         as bfloat16 back into tensor memory, from where P V takes them.  The output accumulates there and is rescaled only when a
 //         row's maximum has outgrown the one its weights are formed with by more than 2^8;
-//   2     takes the codes apart: a lane reads 16 bytes (32 channels, one scale) of the next tile's keys and values ahead, turns them into
-//         the exact bfloat16 values (cache4_decode.cu says how) and stores them where the products read them.  A word of eight codes
-//         leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers are renamed;
-//   3     one warp issues S = Q K^T and O += P V of both tiles in turn: while one tile's products run the other's weights are formed.
+//   2, 3  one warp issues S = Q K^T and O += P V of both tiles in turn: while one tile's products run the other's weights are formed.  The
+//         other seven take the codes apart, four the keys', three the values': a lane reads 16 bytes (32 channels, one scale) of the next
+//         tile ahead, turns them into the exact bfloat16 values (cache4_codes.cuh) and stores them where the products read them.  A word
+//         of eight codes leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers renamed.
 // Keys and values are taken apart once for both tiles.  With heads of 128 channels the weights lie over the scores they were made of
 // (the tensor memory is full), so that a tile's next scores wait for its last product; heads of 64 have room for both.
 // Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of tiles, whose results a second kernel joins in order.
@@ -105,7 +105,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
     for (int s = 0; s < 2; ++s) {
       ta_bar_init(&k_full[s], 4);
       ta_bar_init(&k_empty[s], 1);
-      ta_bar_init(&v_full[s], 4);
+      ta_bar_init(&v_full[s], 3);
       ta_bar_init(&v_empty[s], 1);
       ta_bar_init(&s_full[s], 1);
       ta_bar_init(&p_ready[s], 4);
@@ -192,7 +192,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) t4[q] = ta_max3(t4[q], __uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1]));
         const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * scale;
-        if (it > 0) {                    // (the product before still reads its weights and adds to O)
+        if (!OVER && it > 0) {           // (the product before still reads its weights and adds to O; OVER: the scores came after it)
           ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[sub], (it - 1) & 1));
           if (!ok) break;
           ta_fence_after();
@@ -297,96 +297,86 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         }
       }
     }
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
-    // ---- takes the codes apart ----
-    // a warp's 32 lanes read 16 bytes each of 8 (16) rows in a row; eight lanes of a store cover eight rows' same piece
-    constexpr int SPAN = 32 / CH;        // rows of a warp's read
-    const int dw = warp - 8, chunk = (lane >> 3) % CH, sub_row = (lane & 7) + 8 * ((lane >> 3) / CH);
-    const C4Bits bits;
-    uint4 raw[CH];
-    unsigned sc[CH];
-    // the row j of this lane in a tile: SPAN (4 j + dw) + sub_row
-    auto fetch = [&](int it, bool values) {
-      const int key0 = run.tile_at(it0 + it) * TA_BK;
-      // (a half tile past the last key that a row sees repeats the last page: masked, and NaN there is nobody's)
-      const unsigned char* rec0 = c4_page(c, seq, key0 / C4_PAGE, kv_head, HD);
-      const unsigned char* rec1 = c4_page(c, seq, min(key0 + C4_PAGE, run.pos_last) / C4_PAGE, kv_head, HD);
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        const int r = SPAN * (4 * j + dw) + sub_row;
-        const unsigned char* rec = r < C4_PAGE ? rec0 : rec1;
-        raw[j] = *reinterpret_cast<const uint4*>(rec + (values ? c4_value_codes(HD) : 0) + (r % C4_PAGE) * (HD / 2) + chunk * 16);
-        sc[j] = rec[(values ? c4_value_scales(HD) : c4_key_scales(HD)) + (r % C4_PAGE) * CH + chunk];
-      }
-    };
-    auto place = [&](unsigned char* tile, bool values, bool whole, int edge) {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        const int r = SPAN * (4 * j + dw) + sub_row;
-        unsigned s = c4_scale_bits(sc[j]);
-        if (values && !whole && sc[j] == 255u) {
-          s = 0u;
-          atomicOr(&s_nan[edge][chunk][r >> 5], 1u << (r & 31));
-        }
-        const unsigned s2 = s | s << 16, shift = c4_shift(s2);
-        unsigned char* dst = tile + chunk / 2 * (2 * TA_BOX_BYTES) + r * 128;
-        const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k], bits), s2, shift), c4_fma2(c4_pair<1>(w[k], bits), s2, shift),
-                                     c4_fma2(c4_pair<2>(w[k], bits), s2, shift), c4_fma2(c4_pair<3>(w[k], bits), s2, shift));
-          *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    };
-    uint4 ahead[CH];                     // the values' codes, while the keys' are in `raw`, and the other way round
-    unsigned ahead_sc[CH];
-    auto swap = [&] {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        const uint4 x = raw[j];
-        const unsigned y = sc[j];
-        raw[j] = ahead[j];
-        sc[j] = ahead_sc[j];
-        ahead[j] = x;
-        ahead_sc[j] = y;
-      }
-    };
-    int edges = 0;
-    bool ok = true;
-    fetch(0, true);
-    swap();
-    fetch(0, false);
-#pragma unroll 1
-    for (int it = 0; it < n_tiles && ok; ++it) {
-      const int s = it & 1, key0 = run.tile_at(it0 + it) * TA_BK;
-      const bool whole = key0 + TA_BK - 1 <= run.pos_first && (p.window <= 0 || key0 > run.pos_last - p.window || key0 + TA_BK <= p.keep_first);
-      const int edge = min(edges, C4P_EDGES - 1);
-      if (!whole) {
-        if (tid == 256) {
-          s_edge_key[edge] = key0;
-          *(volatile int*)&s_edges = edge + 1;
-        }
-        ++edges;
-      }
-      if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&k_empty[s], ((it >> 1) - 1) & 1));
-      if (!ok) break;
-      place(Ks + s * TILE, false, whole, edge);
-      c4p_bar_arrive_warp(&k_full[s], lane);
-      if (it + 1 < n_tiles) fetch(it + 1, false);
-      swap();
-      if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&v_empty[s], ((it >> 1) - 1) & 1));
-      if (!ok) break;
-      place(Vs + s * TILE, true, whole, edge);
-      c4p_bar_arrive_warp(&v_full[s], lane);
-      if (it + 1 < n_tiles) fetch(it + 1, true);
-      swap();
-    }
-    if (!ok) s_failed = 1;
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    if (warp != 12) {
+      // ---- takes the codes apart: warps 8-11 the keys', 13-15 the values'.  A warp's read is 16 bytes a lane of SPAN rows in a row (a
+      // unit); eight lanes of a store cover eight rows' same piece ----
+      constexpr int SPAN = 32 / CH, UNITS = TA_BK / SPAN;
+      const bool values = warp > 12;
+      const int who = values ? warp - 13 : warp - 8, step = values ? 3 : 4;
+      constexpr int MOST = (UNITS + 2) / 3;      // units of a warp
+      const int chunk = (lane >> 3) % CH, sub_row = (lane & 7) + 8 * ((lane >> 3) / CH);
+      unsigned char* const stage0 = values ? Vs : Ks;
+      unsigned long long *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
+      const int codes_at = (values ? c4_value_codes(HD) : 0) + chunk * 16, scales_at = (values ? c4_value_scales(HD) : c4_key_scales(HD)) + chunk;
+      const C4Bits bits;
+      // the records of the next 32 half tiles, one a lane.  (A half tile past the last key that a row sees repeats the last page: masked, and
+      // NaN there is nobody's)
+      auto record_of = [&](int half) {
+        const int it = min(half >> 1, n_tiles - 1), key = min(run.tile_at(it0 + it) * TA_BK + (half & 1) * C4_PAGE, run.pos_last);
+        return (unsigned long long)c4_page(c, seq, key / C4_PAGE, kv_head, HD);
+      };
+      unsigned long long records = record_of(lane);
+      uint4 raw[MOST];
+      unsigned sc[MOST];
+      auto fetch = [&](int it) {
+        const unsigned char* rec0 = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, records, (2 * it) & 31));
+        const unsigned char* rec1 = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, records, (2 * it + 1) & 31));
+        if ((it & 15) == 15) records = record_of(2 * it + 2 + lane);
+#pragma unroll
+        for (int j = 0; j < MOST; ++j) {
+          const int unit = j * step + who;
+          if (unit >= UNITS) continue;           // (the same in the warp)
+          const int r = SPAN * unit + sub_row, in_page = r % C4_PAGE;
+          const unsigned char* rec = SPAN * unit < C4_PAGE ? rec0 : rec1;
+          raw[j] = *reinterpret_cast<const uint4*>(rec + codes_at + in_page * (HD / 2));
+          sc[j] = rec[scales_at + in_page * CH];
+        }
+      };
+      int edges = 0;
+      bool ok = true;
+      fetch(0);
+#pragma unroll 1
+      for (int it = 0; it < n_tiles; ++it) {
+        const int s = it & 1, key0 = run.tile_at(it0 + it) * TA_BK;
+        const bool whole = key0 + TA_BK - 1 <= run.pos_first && (p.window <= 0 || key0 > run.pos_last - p.window || key0 + TA_BK <= p.keep_first);
+        const int edge = min(edges, C4P_EDGES - 1);
+        if (!whole) {
+          if (values && who == 0 && lane == 0) {
+            s_edge_key[edge] = key0;
+            *(volatile int*)&s_edges = edge + 1;
+          }
+          ++edges;
+        }
+        if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&empty[s], ((it >> 1) - 1) & 1));
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < MOST; ++j) {
+          const int unit = j * step + who;
+          if (unit >= UNITS) continue;
+          const int r = SPAN * unit + sub_row;
+          unsigned sb = c4_scale_bits(sc[j]);
+          if (values && !whole && sc[j] == 255u) {
+            sb = 0u;
+            atomicOr(&s_nan[edge][chunk][r >> 5], 1u << (r & 31));
+          }
+          const unsigned s2 = sb | sb << 16, shift = c4_shift(s2);
+          unsigned char* dst = stage0 + s * TILE + chunk / 2 * (2 * TA_BOX_BYTES) + r * 128;
+          const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k], bits), s2, shift), c4_fma2(c4_pair<1>(w[k], bits), s2, shift),
+                                       c4_fma2(c4_pair<2>(w[k], bits), s2, shift), c4_fma2(c4_pair<3>(w[k], bits), s2, shift));
+            *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        c4p_bar_arrive_warp(&full[s], lane);
+        if (it + 1 < n_tiles) fetch(it + 1);
+      }
+      if (!ok) s_failed = 1;
+    }
     if (warp == 12) {
       // ---- issuer.  Instruction descriptors: 32-bit accumulator, bfloat16 operands, M = 128; S: N = 128, both K-major;
       // P V: N = HD, the first operand in tensor memory, the second MN-major ----
