@@ -3,16 +3,21 @@
 //
 // A block serves one (sequence, key head) and 256 rows: row r is query head r % group of new token r / group, so that heads which
 // share a key head share its keys, however many new tokens there are.  The rows are two tiles of 128 (rows of the tensor memory), and the
-// visible keys go by in tiles of 128.  Four warpgroups:
-//   0, 1  softmax, a thread a row of tile 0 or 1: scores from tensor memory into registers, running maximum and sum in 32-bit, weights
-//         as bfloat16 back into tensor memory, from where P V takes them.  The output accumulates there and is rescaled only when a
-//         row's maximum has outgrown the one its weights are formed with by more than 2^8;
-//   2, 3  one warp issues S = Q K^T and O += P V of both tiles in turn: while one tile's products run the other's weights are formed.  The
-//         other seven take the codes apart, four the keys', three the values': a lane reads 16 bytes (32 channels, one scale) of the next
-//         tile ahead, turns them into the exact bfloat16 values (cache4_codes.cuh) and stores them where the products read them.  A word
-//         of eight codes leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers renamed.
-// Keys and values are taken apart once for both tiles.  With heads of 128 channels the weights lie over the scores they were made of
-// (the tensor memory is full), so that a tile's next scores wait for its last product; heads of 64 have room for both.
+// visible keys go by in tiles of 128, in steps of 64.  Sixteen warps:
+//   0-3, 4-7  softmax, a thread a row of tile 0 or 1: a step's scores from tensor memory into registers, running maximum and sum in
+//         32-bit, weights as bfloat16 back over the scores they were made of, from where P V takes them.  The output accumulates in
+//         tensor memory and is rescaled only when a row's maximum has outgrown the one its weights are formed with by more than 2^8;
+//   12, 13  issue S = Q K^T and O += P V, each for its tile of rows.  Scores lie in two sets of columns: a step's are formed while the
+//         softmax is at the step before;
+//   8-10, 11, 14 and 15  take the keys' and the values' codes apart: a lane reads 16 bytes (32 channels, one scale) of the next tile ahead,
+//         turns them into the exact bfloat16 values (cache4_codes.cuh) and stores them where the products read them.  A word of eight
+//         codes leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers renamed.
+// What bounds it is the products of 64 columns: they take a tensor core as long as ones of 128 (69 cycles for 16 channels, measured), so that a
+// step of 256 rows takes it 1,500 cycles of the 1,860 it lasts; the exponentials take 1,024 of the special-function units'.  Whole tiles of 128
+// keys have cheaper products, but their scores and weights fill the tensor memory: each tile's next scores then wait for its last product
+// and the softmax for both, which came to the same for long prompts (2 x 4,096 tokens, 32 heads over 8 of 128: 328 us, 333 here) and is
+// slower for short ones (8 x 257 behind a window of 1,024: 82 us, 77 here).  One issuer for both tiles of rows: 376.  Taking the tiles apart
+// beforehand, for all blocks of rows at once: 316, but 91 for the short ones.
 // Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of tiles, whose results a second kernel joins in order.
 //
 // Masked keys get the weight 0 exactly.  A value filed as NaN reaches the rows that see its key and no other: in a tile that every row
@@ -45,7 +50,6 @@ template <int HD>
 struct C4pShape {
   static constexpr int TILE = HD / 64 * 2 * TA_BOX_BYTES;        // 128 rows of a head
   static constexpr size_t SMEM = (size_t)6 * TILE;               // two tiles of queries, two stages of keys and of values
-  static constexpr bool OVER = 2 * (TA_BK + HD + 64) > 512;      // the weights lie over the scores
 };
 
 // The tiles of keys that a block's rows see, and how they are cut: the same for the attention and the kernel that joins.
@@ -63,6 +67,19 @@ struct C4pRun {
   __device__ int tile_at(int i) const { return i < kept_only ? i : kt_lo + (i - kept_only); }
 };
 
+// 32 channels of a row of keys or values (16 bytes of codes, one scale) as bfloat16, to their places in a tile.
+__device__ __forceinline__ void c4p_place(unsigned char* tile, int r, int chunk, const uint4& raw, unsigned scale, const C4Bits& bits) {
+  const unsigned s2 = scale | scale << 16, shift = c4_shift(s2);
+  unsigned char* dst = tile + chunk / 2 * (2 * TA_BOX_BYTES) + r * 128;
+  const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k], bits), s2, shift), c4_fma2(c4_pair<1>(w[k], bits), s2, shift),
+                               c4_fma2(c4_pair<2>(w[k], bits), s2, shift), c4_fma2(c4_pair<3>(w[k], bits), s2, shift));
+    *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
+  }
+}
+
 __device__ __forceinline__ void c4p_bar_arrive_warp(unsigned long long* bar, int lane) {
   __syncwarp();
   if (lane == 0) ta_bar_arrive(bar);
@@ -71,18 +88,16 @@ __device__ __forceinline__ void c4p_bar_arrive_warp(unsigned long long* bar, int
 template <int HD>
 __global__ void __launch_bounds__(C4P_THREADS, 1)
 cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
-  using Shape = C4pShape<HD>;
-  constexpr int TILE = Shape::TILE, CH = HD / 32;
-  constexpr bool OVER = Shape::OVER;
+  constexpr int TILE = C4pShape<HD>::TILE, CH = HD / 32, ISSUER = 12;
   extern __shared__ __align__(1024) unsigned char c4p_raw[];
-  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ __align__(8) unsigned long long bars[20];
   __shared__ unsigned s_nan[C4P_EDGES][CH][4];      // a bit a key of a tile that not every row sees
   __shared__ int s_edge_key[C4P_EDGES], s_edges;
   __shared__ unsigned s_tmem;
   __shared__ int s_failed;
   unsigned char *Qs = c4p_raw, *Ks = Qs + 2 * TILE, *Vs = Ks + 2 * TILE;
   unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // [stage]
-  unsigned long long *s_full = bars + 8, *p_ready = bars + 10, *o_done = bars + 12;                     // [tile of rows], one phase a tile of keys
+  unsigned long long *s_full = bars + 8, *p_ready = bars + 12, *o_done = bars + 16;      // [tile of rows][step parity]
 
   const int kv_head = (int)blockIdx.x % c.n_kv_heads, seq = (int)blockIdx.x / c.n_kv_heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -103,10 +118,12 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
 
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      ta_bar_init(&k_full[s], 4);
-      ta_bar_init(&k_empty[s], 1);
+      ta_bar_init(&k_full[s], 3);
+      ta_bar_init(&k_empty[s], n_sub);
       ta_bar_init(&v_full[s], 3);
-      ta_bar_init(&v_empty[s], 1);
+      ta_bar_init(&v_empty[s], n_sub);
+    }
+    for (int s = 0; s < 4; ++s) {
       ta_bar_init(&s_full[s], 1);
       ta_bar_init(&p_ready[s], 4);
       ta_bar_init(&o_done[s], 1);
@@ -116,7 +133,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (tid < C4P_EDGES * CH * 4) (&s_nan[0][0][0])[tid] = 0u;
-  if (warp == 12) {
+  if (warp == ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(ta_smem(&s_tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
@@ -137,10 +154,12 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   ta_fence_before();
   __syncthreads();
   ta_fence_after();
-  const unsigned tmem = s_tmem, tmem_o = tmem + 2 * TA_BK;      // S of both tiles, O of both, (P of both)
-  auto tmem_p = [&](int sub) { return OVER ? tmem + (unsigned)(sub * TA_BK) : tmem_o + (unsigned)(2 * HD + sub * 64); };
+  const unsigned tmem = s_tmem, tmem_o = tmem + 256;      // S of both tiles of rows, two steps each (64 columns, the weights over the first 32); O
+  // steps of 64 keys: the last tile's second half may lie past every row's last key
+  const bool ends_early = run.tile_at(it0 + n_tiles - 1) * TA_BK + 64 > run.pos_last;
+  const int n_steps = 2 * n_tiles - (ends_early ? 1 : 0);
 
-  // registers: 512 threads x 128 at launch; 2 x 128 x 176 + 2 x 128 x 80 is the same
+  // registers: 512 threads x 128 at launch are 2 x 128 x 176 + 2 x 128 x 80
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
     // ---- softmax: a thread a row; warp w reaches the lanes of quarter w % 4 ----
@@ -150,34 +169,32 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       const int at_first = run.past + (row0 + sub * TA_BQ) / p.group;
       const int at_last = run.past + min(n_new * p.group - 1, row0 + sub * TA_BQ + TA_BQ - 1) / p.group;
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned my_s = tmem + (unsigned)(sub * TA_BK) + lanes, my_o = tmem_o + (unsigned)(sub * HD) + lanes, my_p = tmem_p(sub) + lanes;
+      const unsigned my_s = tmem + (unsigned)(sub * TA_BK) + lanes, my_o = tmem_o + (unsigned)(sub * HD) + lanes;
       const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
       float m = -INFINITY, l = 0.f;      // the reference maximum (base 2, scaled) and the sum of weights formed with it
       bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_tiles; ++it) {
-        const int key0 = run.tile_at(it0 + it) * TA_BK;
-        ok = __all_sync(0xffffffffu, ta_bar_wait(&s_full[sub], it & 1));
+      for (int j = 0; j < n_steps; ++j) {
+        const int key0 = run.tile_at(it0 + (j >> 1)) * TA_BK + 64 * (j & 1);
+        const bool whole = key0 + 63 <= at_first && (p.window <= 0 || key0 > at_last - p.window || key0 + 64 <= p.keep_first);
+        ok = __all_sync(0xffffffffu, ta_bar_wait(&s_full[2 * sub + (j & 1)], (j >> 1) & 1));
         if (!ok) break;                  // (uniform in the warp; the others run into their own bounds)
         ta_fence_after();
-        unsigned a[4][32];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ta_ld32_issue(my_s + 32u * q, a[q]);
+        unsigned a[2][32];
+        ta_ld32_issue(my_s + 64u * (j & 1), a[0]);
+        ta_ld32_issue(my_s + 64u * (j & 1) + 32u, a[1]);
         ta_ld_wait(a[0], a[1]);
-        ta_ld_wait(a[2], a[3]);
-        // from here on the largest score has the largest weight
-        if (p.scale_log2 <= 0.f) {
+        if (p.scale_log2 <= 0.f) {       // from here on the largest score has the largest weight
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int i = 0; i < 32; ++i) a[q][i] = p.scale_log2 < 0.f ? a[q][i] ^ 0x80000000u : __float_as_uint(__uint_as_float(a[q][i]) * 0.f);
         }
-        const bool whole = key0 + TA_BK - 1 <= at_first && (p.window <= 0 || key0 > at_last - p.window || key0 + TA_BK <= p.keep_first);
         if (!whole) {                    // a bit a key
           const int lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) - key0, hi = pos - key0;
           const int kept = p.window > 0 ? min(p.keep_first, pos + 1) - key0 : 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             const int first = lo - 32 * q, last = hi - 32 * q, below = kept - 32 * q;
             unsigned seen = last >= 31 ? 0xffffffffu : last < 0 ? 0u : (2u << last) - 1u;
             seen &= first <= 0 ? 0xffffffffu : first > 31 ? 0u : 0xffffffffu << first;
@@ -188,22 +205,21 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         }
         float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains side by side)
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
+        for (int i = 0; i < 16; i += 2)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) t4[q] = ta_max3(t4[q], __uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1]));
+          for (int q = 0; q < 4; ++q)
+            t4[q] = ta_max3(t4[q], __uint_as_float(a[q >> 1][(q & 1) * 16 + i]), __uint_as_float(a[q >> 1][(q & 1) * 16 + i + 1]));
         const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * scale;
-        if (!OVER && it > 0) {           // (the product before still reads its weights and adds to O; OVER: the scores came after it)
-          ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[sub], (it - 1) & 1));
-          if (!ok) break;
-          ta_fence_after();
-        }
         const bool grown = top > m + TS_GROWTH || (m == -INFINITY && top > -INFINITY);
         if (__any_sync(0xffffffffu, grown)) {
           const float m_new = grown ? top : m;
           const float alpha = grown ? ta_exp2(m - m_new) : 1.f;      // 0 for a row that had seen nothing yet
           l *= alpha;
           m = m_new;
-          if (it > 0) {
+          if (j > 0) {                   // the products before must have been added
+            ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[2 * sub + ((j - 1) & 1)], ((j - 1) >> 1) & 1));
+            if (!ok) break;
+            ta_fence_after();
 #pragma unroll 1
             for (int q = 0; q < HD; q += 32) {
               unsigned o[32];
@@ -219,22 +235,19 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         const unsigned long long scale2 = ta_two(__float_as_uint(scale), __float_as_uint(scale));
         const unsigned long long shift2 = ta_two(__float_as_uint(-m_use), __float_as_uint(-m_use));
         unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
+        unsigned w[32];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          unsigned w[32];
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              unsigned x, y;
-              ta_halves(ta_fma2(ta_two(a[2 * h + q][i], a[2 * h + q][i + 1]), scale2, shift2), x, y);
-              x = __float_as_uint(ta_exp2(__uint_as_float(x)));
-              y = __float_as_uint(ta_exp2(__uint_as_float(y)));
-              sum[(i >> 1) & 3] = ta_add2(sum[(i >> 1) & 3], ta_two(x, y));
-              w[q * 16 + (i >> 1)] = ta_pack(__uint_as_float(x), __uint_as_float(y));
-            }
-          ta_st32(my_p + 32u * h, w);
-        }
+          for (int i = 0; i < 32; i += 2) {
+            unsigned x, y;
+            ta_halves(ta_fma2(ta_two(a[q][i], a[q][i + 1]), scale2, shift2), x, y);
+            x = __float_as_uint(ta_exp2(__uint_as_float(x)));
+            y = __float_as_uint(ta_exp2(__uint_as_float(y)));
+            sum[(i >> 1) & 3] = ta_add2(sum[(i >> 1) & 3], ta_two(x, y));
+            w[q * 16 + (i >> 1)] = ta_pack(__uint_as_float(x), __uint_as_float(y));
+          }
+        ta_st32(my_s + 64u * (j & 1), w);
         {
           unsigned x, y;
           ta_halves(ta_add2(ta_add2(sum[0], sum[1]), ta_add2(sum[2], sum[3])), x, y);
@@ -242,27 +255,25 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         }
         ta_st_wait();
         ta_fence_before();
-        c4p_bar_arrive_warp(&p_ready[sub], lane);
+        c4p_bar_arrive_warp(&p_ready[2 * sub + (j & 1)], lane);
       }
-      if (ok) ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[sub], (n_tiles - 1) & 1));
+      if (ok) ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[2 * sub + ((n_steps - 1) & 1)], ((n_steps - 1) >> 1) & 1));
       ta_fence_after();
       if (!ok) {
         s_failed = 1;
       } else {
-        // channels whose values are NaN for a key that this row sees in a tile that others do not
+        // channels whose values are NaN for a key that this row sees, but were multiplied as 0
         unsigned lost = 0;
-        const int edges = *(volatile int*)&s_edges;
-        for (int e = 0; e < edges; ++e) {
-          const int key0 = s_edge_key[e];
-          for (int j = 0; j < CH * 4; ++j) {
-            unsigned bits = s_nan[e][j >> 2][j & 3];
-            while (bits) {
-              const int key = key0 + 32 * (j & 3) + __ffs(bits) - 1;
-              bits &= bits - 1;
-              if (key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first)) lost |= 1u << (j >> 2);
-            }
+        auto look = [&](int key0, int word, unsigned bits) {
+          while (bits) {
+            const int key = key0 + 32 * (word & 3) + __ffs(bits) - 1;
+            bits &= bits - 1;
+            if (key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first)) lost |= 1u << (word >> 2);
           }
-        }
+        };
+        const int edges = *(volatile int*)&s_edges;
+        for (int e = 0; e < edges; ++e)
+          for (int j = 0; j < CH * 4; ++j) look(s_edge_key[e], j, s_nan[e][j >> 2][j & 3]);
         const bool mine = sub * TA_BQ + r < n_rows;
         const bool cut = gridDim.z > 1;
         const float inv = cut ? 1.f : 1.f / l;
@@ -299,12 +310,13 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
-    if (warp != 12) {
-      // ---- takes the codes apart: warps 8-11 the keys', 13-15 the values'.  A warp's read is 16 bytes a lane of SPAN rows in a row (a
+    if (warp != ISSUER && warp != ISSUER + 1) {
+      // ---- takes the codes apart: warps 8-10 the keys', 11, 14 and 15 the values'.  A warp's read is 16 bytes a lane of SPAN rows in a row (a
       // unit); eight lanes of a store cover eight rows' same piece ----
       constexpr int SPAN = 32 / CH, UNITS = TA_BK / SPAN;
-      const bool values = warp > 12;
-      const int who = values ? warp - 13 : warp - 8, step = values ? 3 : 4;
+      constexpr int step = 3;
+      const bool values = warp > 10;
+      const int who = !values ? warp - 8 : warp == 11 ? 0 : warp - 13;
       constexpr int MOST = (UNITS + 2) / 3;      // units of a warp
       const int chunk = (lane >> 3) % CH, sub_row = (lane & 7) + 8 * ((lane >> 3) / CH);
       unsigned char* const stage0 = values ? Vs : Ks;
@@ -361,15 +373,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
             sb = 0u;
             atomicOr(&s_nan[edge][chunk][r >> 5], 1u << (r & 31));
           }
-          const unsigned s2 = sb | sb << 16, shift = c4_shift(s2);
-          unsigned char* dst = stage0 + s * TILE + chunk / 2 * (2 * TA_BOX_BYTES) + r * 128;
-          const unsigned w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 v = make_uint4(c4_fma2(c4_pair<0>(w[k], bits), s2, shift), c4_fma2(c4_pair<1>(w[k], bits), s2, shift),
-                                       c4_fma2(c4_pair<2>(w[k], bits), s2, shift), c4_fma2(c4_pair<3>(w[k], bits), s2, shift));
-            *reinterpret_cast<uint4*>(dst + ((((chunk & 1) * 4 + k) ^ (r & 7)) << 4)) = v;
-          }
+          c4p_place(stage0 + s * TILE, r, chunk, raw[j], sb, bits);
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         c4p_bar_arrive_warp(&full[s], lane);
@@ -377,53 +381,56 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       }
       if (!ok) s_failed = 1;
     }
-    if (warp == 12) {
-      // ---- issuer.  Instruction descriptors: 32-bit accumulator, bfloat16 operands, M = 128; S: N = 128, both K-major;
+    if (warp == ISSUER || (warp == ISSUER + 1 && n_sub > 1)) {
+      // ---- issuers, one a tile of rows.  Instruction descriptors: 32-bit accumulator, bfloat16 operands, M = 128; S: N = 64, both K-major;
       // P V: N = HD, the first operand in tensor memory, the second MN-major ----
-      const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TA_BK >> 3) << 17) | ((unsigned)(TA_BQ >> 4) << 24);
+      const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(64 >> 3) << 17) | ((unsigned)(TA_BQ >> 4) << 24);
       const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(HD >> 3) << 17) | ((unsigned)(TA_BQ >> 4) << 24);
       const unsigned long long desc_q = ta_desc(Qs, 16), desc_k = ta_desc(Ks, 16), desc_v = ta_desc(Vs, 2 * TA_BOX_BYTES);
-      auto scores = [&](int it, int sub) {
-        const int s = it & 1;
+      const int sub = warp - ISSUER;
+      // S of step j's 64 keys (half j % 2 of their tile's rows) into the columns of its parity
+      auto scores = [&](int j) {
         if (ta_elect()) {
-          const unsigned long long dq = desc_q + (unsigned long long)(sub * (TILE >> 4)), dk = desc_k + (unsigned long long)(s * (TILE >> 4));
+          const unsigned long long dq = desc_q + (unsigned long long)(sub * (TILE >> 4));
+          const unsigned long long dk = desc_k + (unsigned long long)(((j >> 1) & 1) * (TILE >> 4) + (j & 1) * (TA_BOX_BYTES >> 4));
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {      // 16 channels: 32 bytes further along the row, a box further every 64
             const unsigned long long step = (k / 4) * (2 * TA_BOX_BYTES >> 4) + 2 * (k % 4);
-            ta_mma(tmem + (unsigned)(sub * TA_BK), dq + step, dk + step, idesc_s, k > 0 ? 1u : 0u);
+            ta_mma(tmem + (unsigned)(sub * TA_BK + (j & 1) * 64), dq + step, dk + step, idesc_s, k > 0 ? 1u : 0u);
           }
-          ta_commit(&s_full[sub]);
-          if (sub == n_sub - 1) ta_commit(&k_empty[s]);
+          ta_commit(&s_full[2 * sub + (j & 1)]);
+          if ((j & 1) || j + 1 == n_steps) ta_commit(&k_empty[(j >> 1) & 1]);
         }
         __syncwarp();
       };
-      bool ok = __all_sync(0xffffffffu, ta_bar_wait(&k_full[0], 0));
-      ta_fence_after();
-      for (int sub = 0; sub < n_sub && ok; ++sub) scores(0, sub);
-      for (int it = 0; it < n_tiles && ok; ++it) {
-        const int s = it & 1;
-        ok = __all_sync(0xffffffffu, ta_bar_wait(&v_full[s], (it >> 1) & 1));
-        for (int sub = 0; sub < n_sub && ok; ++sub) {
-          ok = __all_sync(0xffffffffu, ta_bar_wait(&p_ready[sub], it & 1));
+      auto mix = [&](int j) {             // P V: 16 keys further are 8 columns of P, 16 rows of V
+        if (ta_elect()) {
+          const unsigned long long dv = desc_v + (unsigned long long)(((j >> 1) & 1) * (TILE >> 4) + (j & 1) * (TA_BOX_BYTES >> 4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            ta_mma_tmem(tmem_o + (unsigned)(sub * HD), tmem + (unsigned)(sub * TA_BK + (j & 1) * 64) + 8u * i,
+                        dv + (unsigned long long)(i * (16 * 128 >> 4)), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+          ta_commit(&o_done[2 * sub + (j & 1)]);
+          if ((j & 1) || j + 1 == n_steps) ta_commit(&v_empty[(j >> 1) & 1]);
+        }
+        __syncwarp();
+      };
+      // P V of a step when its weights are there (and the values); then, when that product is done, the scores two steps ahead, whose
+      // columns its weights held (and their keys are there).  The softmax has the step between to work on meanwhile.
+      bool ok = true;
+      for (int j = -2; j < n_steps && ok; ++j) {
+        if (j >= 0) {
+          ok = __all_sync(0xffffffffu, ta_bar_wait(&v_full[(j >> 1) & 1], (j >> 2) & 1) && ta_bar_wait(&p_ready[2 * sub + (j & 1)], (j >> 1) & 1));
           if (!ok) break;
           ta_fence_after();
-          if (ta_elect()) {
-            const unsigned long long dv = desc_v + (unsigned long long)(s * (TILE >> 4));
-#pragma unroll
-            for (int j = 0; j < TA_BK / 16; ++j)     // 16 keys further: 8 columns of P, 16 rows of V
-              ta_mma_tmem(tmem_o + (unsigned)(sub * HD), tmem_p(sub) + 8u * j, dv + (unsigned long long)(j * (16 * 128 >> 4)), idesc_o,
-                          (it > 0 || j > 0) ? 1u : 0u);
-            ta_commit(&o_done[sub]);
-            if (sub == n_sub - 1) ta_commit(&v_empty[s]);
-          }
-          __syncwarp();
-          if (it + 1 < n_tiles) {
-            if (sub == 0) ok = __all_sync(0xffffffffu, ta_bar_wait(&k_full[(it + 1) & 1], ((it + 1) >> 1) & 1));
-            if (OVER) ok = __all_sync(0xffffffffu, ok && ta_bar_wait(&o_done[sub], it & 1));      // (the weights lie where the scores go)
-            if (!ok) break;
-            ta_fence_after();
-            scores(it + 1, sub);
-          }
+          mix(j);
+        }
+        if (j + 2 < n_steps) {
+          ok = __all_sync(0xffffffffu, ta_bar_wait(&k_full[((j + 2) >> 1) & 1], ((j + 2) >> 2) & 1) &&
+                                           (j < 0 || ta_bar_wait(&o_done[2 * sub + (j & 1)], (j >> 1) & 1)));
+          if (!ok) break;
+          ta_fence_after();
+          scores(j + 2);
         }
       }
       if (!ok && lane == 0) s_failed = 1;
@@ -432,7 +439,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   ta_fence_before();
   __syncthreads();
   if (s_failed) let_copies_land();
-  if (warp == 12) {
+  if (warp == ISSUER) {
     ta_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
   }
