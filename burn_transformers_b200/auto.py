@@ -27,6 +27,7 @@ class AutoLoadOptions:
     max_tokens: int | None = None     # cache size in tokens; default: one sequence of the longest length
     max_slots: int | None = None
     max_context: int | None = None
+    cache_bits: int | None = None     # 4: softmax attention keeps keys and values in 4-bit codes; None: in `dtype`
 
 
 @dataclasses.dataclass
@@ -46,7 +47,7 @@ class AutoCausalLm:
     def load_local(root, options: AutoLoadOptions | None = None) -> LoadedModel:
         options = options or AutoLoadOptions()
         engine = Engine.from_folder(root, options.dtype, max_tokens=options.max_tokens, max_slots=options.max_slots,
-                                    max_context=options.max_context, device=options.device)
+                                    max_context=options.max_context, device=options.device, cache_bits=options.cache_bits)
         return LoadedModel(engine, GenerationConfig.from_model_folder(root), str(root), engine.load_report)
 
 

@@ -2,7 +2,8 @@
 layers, fixed-size state per sequence.
 
 Layer calls with the same key/value needs (heads, head size, window) form a group with a page
-pool of its own, `k[layer][page][kv_head][PAGE_SIZE][head_dim]`; a sequence holds one page per
+pool of its own, `k[layer][page][kv_head][PAGE_SIZE][head_dim]` (in 4 bits `k[layer][page][kv_head][68 * head_dim]` bytes, keys and
+values); a sequence holds one page per
 64 positions in every group (a windowed group cycles through as many pages as its window spans),
 so one page id addresses the same rows in every layer of the group.  This mirrors the reference's
 bank of homogeneous cache groups (src/cache/tensor/state.rs:36-60, src/cache/tensor/kv.rs:65-86 of
@@ -70,7 +71,7 @@ class KvGroup:
     entries: list[int]            # cache entry ids, in layer order inside the group
     table_len: int                # pages a sequence may hold (all keys) or cycles through (window)
     pool: _PageBooks
-    k: torch.Tensor               # [layers, pages, kv_heads, PAGE_SIZE, head_dim]
+    k: torch.Tensor               # [layers, pages, kv_heads, PAGE_SIZE, head_dim], in 4 bits [layers, pages, kv_heads, bytes]
     v: torch.Tensor
     whole: bool = False           # the table reaches the longest sequence: its pages never come round
 
@@ -111,9 +112,12 @@ class CacheBank:
             shape = (len(entries), n_pages, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
             # (a group without values keeps an empty value pool, so that every group has the same two fields)
             v_shape = shape if spec.has_values else (len(entries), 0, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
+            dtype = kv_dtype
+            if spec.bits is not None:      # a record of bytes a page and head: codes and scales of keys and values
+                dtype, shape, v_shape = torch.uint8, (*shape[:3], 68 * spec.head_dim), (len(entries), 0, spec.n_kv_heads, 0)
             group = KvGroup(spec, entries, table_len, _PageBooks(self, len(self.groups), n_pages),
-                            torch.zeros(shape, dtype=kv_dtype, device=self.device),
-                            torch.zeros(v_shape, dtype=kv_dtype, device=self.device),
+                            torch.zeros(shape, dtype=dtype, device=self.device),
+                            torch.zeros(v_shape, dtype=dtype, device=self.device),
                             whole=table_len >= self.table_width)
             for layer, entry in enumerate(entries):
                 self._entry_group[entry] = (len(self.groups), layer)

@@ -12,17 +12,22 @@ PAGE_SIZE = 64  # tokens per page; the kernels' page_size
 class KvSpec:
     """Keys and values per position: all of them (`window` None) or the last `window`.  `has_values` False: one row
     per position and key head only (a layer whose values are read out of the same rows, such as a latent that is both
-    key and value); the group then has no value pool."""
+    key and value); the group then has no value pool.  `bits` 4: keys and values in 4-bit codes with a scale for every 32
+    channels (csrc/cache4.cuh), side by side in the group's one pool; None: in the model's type."""
     n_kv_heads: int
     head_dim: int
     window: int | None = None
     has_values: bool = True
+    bits: int | None = None
 
     def __post_init__(self):
         if self.n_kv_heads <= 0 or self.head_dim <= 0:
             raise ValueError("KvSpec: heads and head_dim must be positive")
         if self.window is not None and self.window <= 0:
             raise ValueError("KvSpec: window must be positive")
+        if self.bits is not None and (self.bits != 4 or not self.has_values or self.head_dim % 32 or self.head_dim > 256):
+            raise ValueError(f"KvSpec: {self.bits} bits for heads of {self.head_dim}: a cache of codes has 4 bits, keys and values, and "
+                             f"heads of a multiple of 32 channels up to 256")
 
 
 @dataclasses.dataclass(frozen=True)

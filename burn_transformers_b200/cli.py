@@ -30,6 +30,8 @@ def main(argv=None) -> int:
     parser.add_argument("prompt_ids", nargs="?", default="464,1115,4165,7577,389")
     parser.add_argument("max_new_tokens", nargs="?", type=int, default=32)
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    parser.add_argument("--cache-bits", type=int, choices=[4], default=None,
+                        help="4: softmax attention keeps keys and values in 4-bit codes (default: in --dtype)")
     parser.add_argument("--strategy", choices=["greedy", "sample"], default=None)
     parser.add_argument("--temperature", type=float, default=None)
     parser.add_argument("--top-k", type=int, default=None)
@@ -62,7 +64,8 @@ def main(argv=None) -> int:
         return 2
     try:
         tokens = cache_tokens_for([len(p) for p in prompts], args.max_new_tokens)
-        loaded = AutoCausalLm.load_local(args.model_dir, AutoLoadOptions(dtype=args.dtype, max_tokens=tokens))
+        loaded = AutoCausalLm.load_local(args.model_dir, AutoLoadOptions(dtype=args.dtype, max_tokens=tokens,
+                                                                            cache_bits=args.cache_bits))
         generation = loaded.generation_defaults
         generation.max_new_tokens = args.max_new_tokens
         for name in ("strategy", "temperature", "top_k", "top_p", "min_p", "repetition_penalty", "presence_penalty",

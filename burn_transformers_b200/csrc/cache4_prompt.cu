@@ -1,7 +1,7 @@
 // Attention over a 4-bit cache (cache4.cuh) for steps that bring many tokens a sequence, on the fifth-generation tensor cores:
 // bfloat16 queries, heads of 64 or 128 channels.
 //
-// A block serves one (sequence, key head) and 256 rows: row r is query head r % group of new token r / group, so that heads which
+// A block serves one (sequence, key head) and 256 rows (or 128): row r is query head r % group of new token r / group, so that heads which
 // share a key head share its keys, however many new tokens there are.  The rows are two tiles of 128 (rows of the tensor memory), and the
 // visible keys go by in tiles of 128, in steps of 64.  Sixteen warps:
 //   0-3, 4-7  softmax, a thread a row of tile 0 or 1: a step's scores from tensor memory into registers, running maximum and sum in
@@ -31,7 +31,6 @@
 namespace bt {
 
 constexpr int C4P_THREADS = 512;
-constexpr int C4P_ROWS = 256;
 constexpr int C4P_EDGES = 8;            // tiles that not every row of a block sees: at most 7
 
 struct Cache4PromptParams {
@@ -39,10 +38,10 @@ struct Cache4PromptParams {
   long long q_row;
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
-  int n_heads, group;
+  int n_heads, group, rows;     // rows a block: 128 or 256
   float scale_log2;
   int window, keep_first;
-  float* part;                 // [unit][split][256][HD], then [unit][split][256][2]
+  float* part;                 // [unit][split][rows][HD], then [unit][split][rows][2]
   long long part_ml;
 };
 
@@ -55,9 +54,9 @@ struct C4pShape {
 // The tiles of keys that a block's rows see, and how they are cut: the same for the attention and the kernel that joins.
 struct C4pRun {
   int past, pos_first, pos_last, kept_only, kt_lo, n_tiles, per;
-  __device__ C4pRun(int past_, int n_new, int row0, int group, int window, int keep_first, int n_splits) : past(past_) {
+  __device__ C4pRun(int past_, int n_new, int row0, int rows, int group, int window, int keep_first, int n_splits) : past(past_) {
     pos_first = past + row0 / group;
-    pos_last = past + min(n_new * group - 1, row0 + C4P_ROWS - 1) / group;
+    pos_last = past + min(n_new * group - 1, row0 + rows - 1) / group;
     const int lo = window > 0 ? max(0, pos_first - window + 1) : 0;
     kt_lo = lo / TA_BK;
     kept_only = window > 0 ? min((min(keep_first, pos_last + 1) + TA_BK - 1) / TA_BK, kt_lo) : 0;
@@ -104,10 +103,10 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   pdl_trigger();
   pdl_wait();
   const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
-  const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * C4P_ROWS;      // (the longest blocks first)
-  const int n_rows = min(C4P_ROWS, n_new * p.group - row0);
+  const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * p.rows;      // (the longest blocks first)
+  const int n_rows = min(p.rows, n_new * p.group - row0);
   if (n_rows <= 0) return;
-  const C4pRun run(p.past_len[seq], n_new, row0, p.group, p.window, p.keep_first, (int)gridDim.z);
+  const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, (int)gridDim.z);
   const int it0 = (int)blockIdx.z * run.per, n_tiles = min(run.n_tiles, it0 + run.per) - it0;
   if (n_tiles <= 0) return;
   if ((ta_smem(c4p_raw) & 1023u) != 0) {      // the swizzled layouts need the alignment: refuse rather than compute nonsense
@@ -279,7 +278,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         const float inv = cut ? 1.f : 1.f / l;
         const int token = row / p.group, head = kv_head * p.group + row % p.group;
         __nv_bfloat16* dst = p.out + ((long long)(t0 + token) * p.n_heads + head) * HD;
-        const long long unit = (((long long)blockIdx.x * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * C4P_ROWS + sub * TA_BQ + r;
+        const long long unit = (((long long)blockIdx.x * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * p.rows + sub * TA_BQ + r;
         float* part = p.part + unit * HD;
 #pragma unroll 1
         for (int q = 0; q < CH; ++q) {
@@ -446,21 +445,21 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   if (tid == 0 && s_failed && c.status) atomicExch(c.status, 10);
 }
 
-// Joins the runs of keys of 256 rows in their order: a block a row, a thread a channel.
+// Joins the runs of keys of a block's rows in their order: a block a row, a thread a channel.
 template <int HD>
 __global__ void __launch_bounds__(HD)
 cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, int n_splits) {
   pdl_trigger();
   pdl_wait();
   const int kv_head = (int)blockIdx.y % n_kv_heads, seq = (int)blockIdx.y / n_kv_heads;
-  const int tile = (int)blockIdx.x / C4P_ROWS, r = (int)blockIdx.x % C4P_ROWS, row0 = (row_tiles - 1 - tile) * C4P_ROWS, row = row0 + r;
+  const int tile = (int)blockIdx.x / p.rows, r = (int)blockIdx.x % p.rows, row0 = (row_tiles - 1 - tile) * p.rows, row = row0 + r;
   const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
   if (row >= n_new * p.group) return;
-  const C4pRun run(p.past_len[seq], n_new, row0, p.group, p.window, p.keep_first, n_splits);
+  const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
   const int used = (run.n_tiles + run.per - 1) / run.per;
   float top = -INFINITY, sum = 0.f, o = 0.f;
   for (int s = 0; s < used; ++s) {
-    const long long unit = (((long long)blockIdx.y * row_tiles + tile) * n_splits + s) * C4P_ROWS + r;
+    const long long unit = (((long long)blockIdx.y * row_tiles + tile) * n_splits + s) * p.rows + r;
     const float m = p.part[p.part_ml + 2 * unit], l = p.part[p.part_ml + 2 * unit + 1], x = p.part[unit * HD + threadIdx.x];
     const float m_new = fmaxf(top, m), use = m_new == -INFINITY ? 0.f : m_new;
     const float a = ta_exp2(top - use), b = ta_exp2(m - use);
@@ -480,20 +479,21 @@ static int launch_c4p(const Cache4PromptParams& p, const Cache4View& c, int n_se
   BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
   BT_PDL_OK("cache4_prompt", launch_pdl(kern, dim3(n_seqs * c.n_kv_heads, row_tiles, n_splits), dim3(C4P_THREADS), smem, stream, 1, p, c));
   if (n_splits > 1)
-    BT_PDL_OK("cache4_prompt_join", launch_pdl(cache4_prompt_join_kernel<HD>, dim3(row_tiles * C4P_ROWS, n_seqs * c.n_kv_heads), dim3(HD), 0, stream,
+    BT_PDL_OK("cache4_prompt_join", launch_pdl(cache4_prompt_join_kernel<HD>, dim3(row_tiles * p.rows, n_seqs * c.n_kv_heads), dim3(HD), 0, stream,
                                                1, p, c.n_kv_heads, row_tiles, n_splits));
   return 0;
 }
 
 }  // namespace bt
 
-// Arguments as bt_cache4_attention (bfloat16).  scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * row tiles (of 256 rows:
-// max_new * (n_heads / n_kv_heads)) * splits * 256 * (dim + 2).
+// Arguments as bt_cache4_attention (bfloat16).  scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * row tiles (of `rows` rows:
+// max_new * (n_heads / n_kv_heads)) * splits * rows * (dim + 2).
 extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
                                 int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
                                 int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
-                                float* scratch, long long scratch_floats, cudaStream_t stream) {
+                                int rows, float* scratch, long long scratch_floats, cudaStream_t stream) {
   using namespace bt;
+  BT_CHECK(rows == 128 || rows == 256, "cache4_attention: %d rows a block (128 or 256)", rows);
   BT_CHECK(dim == 64 || dim == 128, "cache4_attention: the kernel for many tokens takes heads of 64 or 128 channels, not %d", dim);
   BT_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "cache4_attention: %d query heads cannot share %d key heads", n_heads, n_kv_heads);
   BT_CHECK(n_pages > 0 && table != nullptr && table_len > 0 && n_seqs >= 0 && max_new >= 0 && window >= 0 && keep_first >= 0,
@@ -503,14 +503,14 @@ extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const
   if (n_seqs == 0 || max_new == 0) return 0;
   const int group = n_heads / n_kv_heads;
   BT_CHECK((long long)max_new * group < (1ll << 30), "cache4_attention: %d new tokens of %d heads are too many", max_new, group);
-  const int row_tiles = (int)(((long long)max_new * group + C4P_ROWS - 1) / C4P_ROWS);
+  const int row_tiles = (int)(((long long)max_new * group + rows - 1) / rows);
   const long long units = (long long)n_seqs * n_kv_heads;
   BT_CHECK(units <= 65535 && row_tiles <= 65535 && n_splits >= 1 && n_splits <= 65535, "cache4_attention: grid too large (%lld sequences' heads, %d tiles of rows)",
            units, row_tiles);
-  const long long parts = units * row_tiles * n_splits * C4P_ROWS;
+  const long long parts = units * row_tiles * n_splits * rows;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group,
+  const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, rows,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   if (dim == 64) return launch_c4p<64>(p, c, n_seqs, row_tiles, n_splits, stream);

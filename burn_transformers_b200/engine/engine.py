@@ -60,11 +60,15 @@ class Engine:
     # ---- construction ------------------------------------------------------------------
     @classmethod
     def from_folder(cls, folder, dtype: str = "bfloat16", *, max_tokens: int | None = None,
-                    max_slots: int | None = None, max_context: int | None = None, device="cuda:0") -> "Engine":
-        """Reads config.json, picks the architecture by `model_type`, loads model.safetensors strictly."""
+                    max_slots: int | None = None, max_context: int | None = None, device="cuda:0",
+                    cache_bits: int | None = None) -> "Engine":
+        """Reads config.json, picks the architecture by `model_type`, loads model.safetensors strictly.  `cache_bits` 4: softmax attention
+        keeps its keys and values in 4-bit codes (parts.CausalSelfAttention.hold_cache_in)."""
         from .. import models  # noqa: F401  (registers the architectures)
         arch, config = config_from_folder(Path(folder))
         plan = arch.build(config)
+        if cache_bits is not None:
+            plan.hold_cache_in(cache_bits)
         tensors, report = load_weights(folder, plan.weights, dtype, torch.device(device))
         if max_context is None and plan.max_context >= UNBOUNDED_CONTEXT:
             # a model without a position table: no sequence outgrows the cache, so the page tables need be no longer

@@ -11,6 +11,7 @@ import torch
 
 from ..cache.spec import CacheNeed
 from ..config.base import ModelConfig
+from ..errors import CacheError, ShapeError
 from ..parts.base import Block, Norm, Part, PositionEncoding
 from ..weights.spec import TensorSpec, WeightPlan
 
@@ -76,6 +77,17 @@ class ModelPlan:
         for name, (part, local) in self.names.items():
             tensors[name] = part.specs()[local]
         return WeightPlan(tensors, self.namespaces, self.probe, self.ignored, dict(self.tied), dict(self.sources))
+
+    def hold_cache_in(self, bits: int) -> None:
+        """Has every mixer that can hold its keys and values in `bits` bits do so; before an engine makes its cache."""
+        able = [part for part in self.all_parts() if hasattr(part, "hold_cache_in")]
+        if not able:
+            raise CacheError(f"cache_bits {bits}: no attention of this model has a cache that can be held in fewer bits")
+        for part in able:
+            try:
+                part.hold_cache_in(bits)
+            except ShapeError as error:
+                raise CacheError(f"cache_bits {bits}: {error}") from None
 
     def cache_needs(self) -> list[CacheNeed]:
         """One entry per call of the schedule; readers of another call's cache need nothing."""

@@ -1938,7 +1938,7 @@ _ARGUMENTS = {
     "bt_cache4_gather": "pllpllplpppiiipiiiip",
     "bt_cache4_attention": "plpplpiipppiiiiifiiip",
     "bt_cache4_decode": "plpplpiipppiiiiifiiiiplp",
-    "bt_cache4_prompt": "plpplpiipppiiiiifiiiplp",
+    "bt_cache4_prompt": "plpplpiipppiiiiifiiiiplp",
 }
 
 
@@ -2153,10 +2153,10 @@ def _cache4_few(sms, units, pages, wide, head_dim):
 
 
 def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
-    """Which kernel takes a step of these sizes in bfloat16, its warps a block (few tokens), its pieces of the keys, and the scratch
-    that joining them takes: for the step itself, and for any of the same heads with fewer sequences or shorter ones.
+    """Which kernel takes a step of these sizes in bfloat16, its warps a block ("few") or rows a block ("many"), its pieces of the keys,
+    and the scratch that joining them takes: for the step itself, and for any of the same heads with fewer sequences or shorter ones.
 
-    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, in blocks of 8 or 16; "many": blocks of 256 of them."""
+    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, in blocks of 8 or 16; "many": the same as rows."""
     if head_dim != 64 and head_dim != 128:
         return "any", 0, 1, 0, 0
     columns = max_new * (n_heads // n_kv_heads)
@@ -2170,11 +2170,15 @@ def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window
         one = wide * (head_dim + 2)
         most = min(max(3 * sms, 3 * units), units * -(-pages // 4))
         return "few", warps, pieces, units * pieces * one if pieces > 1 else 0, most * one
-    tiles = -(-columns // 256)
-    # a block a multiprocessor; pieces of eight tiles of 128 keys at least
+    # a block a multiprocessor; pieces of eight tiles of 128 keys at least.  Blocks of 128 rows where 256 would leave a quarter of them
+    # idle and the keys are too few to cut (two prompts of 1,024, 12 heads of 64: 23.6 us and 18.0; 8 of 512, 16 heads: 24.6 and 33.1)
+    rows = 256
+    tiles = -(-columns // rows)
     pieces = max(1, min(sms // (units * tiles), -(-span // 1024)))
-    one = 256 * (head_dim + 2)
-    return "many", 0, pieces, units * tiles * pieces * one if pieces > 1 else 0, min(sms, units * tiles * -(-span // 1024)) * one
+    if pieces == 1 and 4 * units * tiles <= 3 * sms:
+        rows = 128
+    one = rows * (head_dim + 2)
+    return "many", rows, pieces, units * tiles * pieces * one if pieces > 1 else 0, min(sms, units * tiles * -(-span // 1024)) * one
 
 
 def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
@@ -2218,9 +2222,9 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
-    kind, warps, splits, floats = "any", 0, 1, 0
+    kind, wide, splits, floats = "any", 0, 1, 0
     if impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0:
-        kind, warps, splits, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
+        kind, wide, splits, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
     partial = 0
     if floats:
         if scratch is None:
@@ -2231,8 +2235,8 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     head = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
             _status_address(device), starts, pasts, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, window, keep_first)
     if kind == "few":
-        _check(library().bt_cache4_decode(*head, splits, warps, partial, floats, _raw_stream(device)))
+        _check(library().bt_cache4_decode(*head, splits, wide, partial, floats, _raw_stream(device)))
     elif kind == "many":
-        _check(library().bt_cache4_prompt(*head, splits, partial, floats, _raw_stream(device)))
+        _check(library().bt_cache4_prompt(*head, splits, wide, partial, floats, _raw_stream(device)))
     else:
         _check(library().bt_cache4_attention(*head, code, _raw_stream(device)))

@@ -29,6 +29,14 @@ class CausalSelfAttention(Mixer):
     result is added to the residual stream (src/models/gpt2/model.rs:114-142, 218-261;
     src/attention/dispatch.rs:277-430 of the reference).  `n_kv_heads` < `n_heads` shares each key
     head among consecutive query heads.
+
+    `qk_norm_eps`: every query and key head is normed, x / sqrt(mean(x^2) + eps) * weight ("q_norm.weight" and "k_norm.weight",
+    [head_dim]), before `positions` turns it, in the same pass where `positions` offers it.
+
+    `cache_bits` 4 (or `hold_cache_in(4)`): the cache holds keys and values in 4-bit codes (csrc/cache4.cuh).  Every query then attends over
+    what the cache holds, the step's own keys and values too, so that a sequence's results do not depend on the portions that it
+    came in.  With a `window`, positions below `keep_first` stay visible beside it (of a cache in 4 bits only), and the cache keeps
+    every position.
     """
 
     accepts_lazy_norm = True
@@ -37,7 +45,8 @@ class CausalSelfAttention(Mixer):
 
     def __init__(self, width: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, *,
                  causal: bool = True, window: int | None = None, bias: bool = True,
-                 init_std: float = 0.02, out_init_std: float | None = None, positions=None, out_scale: float = 1.0):
+                 init_std: float = 0.02, out_init_std: float | None = None, positions=None, out_scale: float = 1.0,
+                 qk_norm_eps: float | None = None, cache_bits: int | None = None, keep_first: int = 0):
         if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
             raise ShapeError(f"{n_heads} query heads cannot share {n_kv_heads} key heads")
         if not 1 <= head_dim <= self.MAX_HEAD_DIM:
@@ -56,8 +65,26 @@ class CausalSelfAttention(Mixer):
         # the mixer's result times this as it enters the residual stream: folded into the output projection when the
         # weights are bound (in 32-bit, rounded once to the compute type)
         self.out_scale = float(out_scale)
+        self.qk_norm_eps = None if qk_norm_eps is None else float(qk_norm_eps)
+        if keep_first < 0 or (keep_first and (window is None or cache_bits is None)):
+            raise ShapeError(f"{keep_first} kept positions need a window and a cache in 4 bits")
+        self.keep_first = int(keep_first)
+        self.cache_bits = None
+        if cache_bits is not None:
+            self.hold_cache_in(cache_bits)
+
+    def hold_cache_in(self, bits: int) -> None:
+        """Has the cache hold this layer's keys and values in `bits` (4) bits; before the engine makes its cache."""
+        if bits != 4:
+            raise ShapeError(f"a cache holds keys and values in the model's type or in 4 bits, not in {bits}")
+        if self.head_dim % 32 or not self.causal:
+            raise ShapeError(f"a cache in 4 bits takes causal attention over heads of a multiple of 32 channels, not of {self.head_dim}")
+        self.cache_bits = 4
 
     def bind(self, tensors):
+        if self.positions is not None and hasattr(self.positions, "inv_freq"):
+            for t in tensors.values():
+                self.positions.inv_freq(t.device)
         if self.out_scale != 1.0:
             tensors = dict(tensors)
             for name in ("out.weight", "out.bias"):
@@ -72,9 +99,14 @@ class CausalSelfAttention(Mixer):
         if self.has_bias:
             specs["qkv.bias"] = TensorSpec((self.proj_width,), VECTOR, ("zeros",))
             specs["out.bias"] = TensorSpec((self.width,), VECTOR, ("zeros",))
+        if self.qk_norm_eps is not None:
+            specs["q_norm.weight"] = TensorSpec((self.head_dim,), VECTOR, ("ones",))
+            specs["k_norm.weight"] = TensorSpec((self.head_dim,), VECTOR, ("ones",))
         return specs
 
     def cache_need(self):
+        if self.cache_bits is not None:
+            return CacheNeed(kv=KvSpec(self.n_kv_heads, self.head_dim, bits=self.cache_bits))
         return CacheNeed(kv=KvSpec(self.n_kv_heads, self.head_dim, self.window))
 
     def _splits(self, ctx) -> int:
@@ -87,6 +119,39 @@ class CausalSelfAttention(Mixer):
         by_fill = -(-2 * _sm_count(ctx.ws.device) // units)
         return int(max(1, min(by_fill, pages, 8)))
 
+    def _turn(self, ctx, proj) -> None:
+        """Norms and turns the step's query and key heads in place."""
+        heads = (self.n_heads, self.n_kv_heads, self.head_dim)
+        if self.qk_norm_eps is None:
+            if self.positions is not None:
+                self.positions.rotate(ctx, proj, *heads)
+            return
+        norm = dict(q_weight=self.t_q_norm_weight, k_weight=self.t_k_norm_weight, eps=self.qk_norm_eps)
+        if hasattr(self.positions, "norm_rotate"):
+            self.positions.norm_rotate(ctx, proj, *heads, **norm)
+            return
+        kernels.qk_norm_rotary(proj, ctx.positions, None, n_tokens=ctx.n_tokens, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
+                               head_dim=self.head_dim, rot_dims=0, **norm)
+        if self.positions is not None:
+            self.positions.rotate(ctx, proj, *heads)
+
+    def _forward_4_bits(self, ctx, proj, residual, entry, owns_cache) -> None:
+        n = ctx.n_tokens
+        pool, _, group, g = ctx.cache.layer_pools(entry)
+        table = ctx.tables[g]
+        if owns_cache:
+            k = proj[:n, self.q_width:self.q_width + self.kv_width].view(n, self.n_kv_heads, self.head_dim)
+            v = proj[:n, self.q_width + self.kv_width:].view(n, self.n_kv_heads, self.head_dim)
+            kernels.cache4_append(k, v, pool, ctx.positions, ctx.token_seq, ctx.ctx_len, table, group.table_len, n_tokens=n)
+        sizes = dict(n_tokens=n, n_seqs=ctx.n_seqs, max_new=1 if ctx.is_decode else ctx.max_new, max_ctx=ctx.ctx_bound, n_heads=self.n_heads,
+                     n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, window=self.window or 0, keep_first=self.keep_first)
+        floats = kernels.cache4_attention_scratch_floats(**sizes)
+        scratch = ctx.ws.take((floats,), torch.float32) if floats else None
+        mixed = ctx.ws.take((n, self.q_width), ctx.dtype)
+        kernels.cache4_attention(proj, mixed, pool, table, group.table_len, ctx.seq_start, ctx.past_len, scale=self.scale, scratch=scratch, **sizes)
+        linear(ctx, mixed, self.t_out_weight, self.t_out_bias if self.has_bias else None, residual, m=n,
+               residual=residual, w_is_nk=self.nk_out_weight)
+
     def forward(self, ctx, x, residual, entry, owns_cache=True):
         n = ctx.n_tokens
         dtype = ctx.dtype
@@ -94,11 +159,14 @@ class CausalSelfAttention(Mixer):
         linear(ctx, x, self.t_qkv_weight, self.t_qkv_bias if self.has_bias else None, proj, m=n,
                w_is_nk=self.nk_qkv_weight)
         program = getattr(ctx, "program", None)
-        if self.positions is not None:
+        if self.positions is not None or self.qk_norm_eps is not None or self.cache_bits is not None:
             if program is not None:
                 from ..engine.program import ProgramUnsupported
-                raise ProgramUnsupported("a rotating position encoding has no phase in the fused step")
-            self.positions.rotate(ctx, proj, self.n_heads, self.n_kv_heads, self.head_dim)
+                raise ProgramUnsupported("a rotating position encoding, a norm of heads or a cache in 4 bits has no phase in the fused step")
+            self._turn(ctx, proj)
+        if self.cache_bits is not None:
+            self._forward_4_bits(ctx, proj, residual, entry, owns_cache)
+            return
         k_pool, v_pool, group, g = ctx.cache.layer_pools(entry)
         table = ctx.tables[g]
         window = self.window or 0

@@ -109,15 +109,30 @@ class InterleavedRotary(PositionEncoding):
 
     def rotate(self, ctx, proj, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
         n = ctx.n_tokens
+        if self.size != 1.0:
+            self.norm_rotate(ctx, proj, n_heads, n_kv_heads, head_dim)
+            return
         heads = n_heads + n_kv_heads              # queries and keys lie side by side, values after them
         view = proj[:n, :heads * head_dim].view(n, heads, head_dim)
         self.rotate_vectors(ctx, view, view)
 
 
+    # the pairs that turn: neighbours, or channels half of `dims` apart
+    neighbours = True
+
+    def norm_rotate(self, ctx, proj, n_heads: int, n_kv_heads: int, head_dim: int, *, q_weight=None, k_weight=None, eps: float = 0.0) -> None:
+        """`rotate` with the norm of every query and key head before it (x / sqrt(mean(x^2) + eps) * weight, where weights are given) in one
+        pass over the projections; the angles are formed in 64-bit, and cosine and sine are scaled by `size`."""
+        kernels.qk_norm_rotary(proj, ctx.positions, self.inv_freq(proj.device), n_tokens=ctx.n_tokens, n_heads=n_heads, n_kv_heads=n_kv_heads,
+                               head_dim=head_dim, rot_dims=self.dims, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                               interleaved=self.neighbours, size=self.size)
+
+
 class HalfSplitRotary(InterleavedRotary):
     """The same turn with the other pairing: channel i < dims/2 of a vector goes with channel i + dims/2.  Its kernel
     writes 32-bit vectors (a recurrence reads them), can scale the vectors from one index on afterwards (keys), and
-    copies the channels that follow the vectors in a row."""
+    copies the channels that follow the vectors in a row; a step's own projections are turned in place (`rotate`)."""
+    neighbours = False
 
     def rotate_rows(self, ctx, src, dst, *, n_vecs: int, length: int, scaled_from=None, scale: float = 1.0,
                     tail: int = 0) -> None:
@@ -129,5 +144,5 @@ class HalfSplitRotary(InterleavedRotary):
     def rotate_vectors(self, ctx, src, dst) -> None:
         raise NotImplementedError("the half-split rotation writes 32-bit rows: use rotate_rows")
 
-    def rotate(self, ctx, proj, n_heads, n_kv_heads, head_dim) -> None:
-        raise NotImplementedError("the half-split rotation writes 32-bit rows: use rotate_rows")
+    def rotate(self, ctx, proj, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+        self.norm_rotate(ctx, proj, n_heads, n_kv_heads, head_dim)

@@ -1,0 +1,63 @@
+"""What holds its keys and values in 4 bits, and what refuses to, without a device."""
+import pytest
+import torch
+
+from burn_transformers_b200.cache import CacheBank, CacheConfig, CacheNeed, KvSpec
+from burn_transformers_b200.config import Gpt2Config
+from burn_transformers_b200.errors import CacheError, ShapeError
+from burn_transformers_b200.models.gpt2 import build_gpt2
+from burn_transformers_b200.parts import CausalSelfAttention
+
+
+def test_a_group_in_4_bits_is_one_pool_of_bytes():
+    needs = [CacheNeed(kv=KvSpec(2, 64)), CacheNeed(kv=KvSpec(2, 64, bits=4)), CacheNeed(kv=KvSpec(2, 64, bits=4))]
+    bank = CacheBank(needs, CacheConfig(64 * 6, 3, 64 * 5), torch.bfloat16, "cpu")
+    plain, packed = bank.groups
+    assert plain.k.dtype == torch.bfloat16 and packed.k.dtype == torch.uint8
+    assert list(packed.k.shape) == [2, 6, 2, 68 * 64] and packed.v.numel() == 0
+    assert packed.k[0].nbytes * 256 == (plain.k[0].nbytes + plain.v[0].nbytes) * 68
+    slot = bank.acquire()
+    bank.reserve([(slot, 130)])
+    assert len(bank.table_row(1, slot)) == 3
+    bank.check()
+
+
+@pytest.mark.parametrize("spec", [dict(head_dim=48, bits=4), dict(head_dim=288, bits=4), dict(head_dim=64, bits=8),
+                                  dict(head_dim=64, bits=4, has_values=False)])
+def test_specs_that_are_refused(spec):
+    with pytest.raises(ValueError):
+        KvSpec(2, **spec)
+
+
+def test_a_plan_holds_its_softmax_attention_in_4_bits():
+    config = dict(model_type="gpt2", n_layer=3, n_embd=128, n_head=2, vocab_size=64, n_positions=128)
+    plan = build_gpt2(Gpt2Config.from_dict(config))
+    assert all(need.kv.bits is None for need in plan.cache_needs())
+    plan.hold_cache_in(4)
+    assert [need.kv for need in plan.cache_needs()] == [KvSpec(2, 64, bits=4)] * 3
+    with pytest.raises(CacheError, match="not in 8"):
+        plan.hold_cache_in(8)
+    odd = build_gpt2(Gpt2Config.from_dict(dict(config, n_head=8)))
+    with pytest.raises(CacheError, match="multiple of 32 channels, not of 16"):
+        odd.hold_cache_in(4)
+
+
+def test_a_model_without_softmax_attention_refuses(monkeypatch):
+    plan = build_gpt2(Gpt2Config.from_dict(dict(model_type="gpt2", n_layer=1, n_embd=128, n_head=2, vocab_size=64, n_positions=128)))
+    monkeypatch.setattr(plan, "all_parts", lambda: [plan.embedding, plan.final_norm])
+    with pytest.raises(CacheError, match="fewer bits"):
+        plan.hold_cache_in(4)
+
+
+@pytest.mark.parametrize("kw, words", [(dict(keep_first=2), "kept positions"), (dict(keep_first=2, window=8), "kept positions"),
+                                       (dict(keep_first=-1), "kept positions"), (dict(cache_bits=3), "not in 3"),
+                                       (dict(cache_bits=4, causal=False), "causal")])
+def test_an_attention_that_is_refused(kw, words):
+    with pytest.raises(ShapeError, match=words):
+        CausalSelfAttention(128, 2, 2, 64, 0.125, **kw)
+
+
+def test_norms_of_heads_are_tensors_of_the_part():
+    part = CausalSelfAttention(128, 4, 2, 32, 0.125, qk_norm_eps=1e-6, cache_bits=4, window=100, keep_first=4)
+    assert part.specs()["q_norm.weight"].shape == (32,) and part.specs()["k_norm.weight"].shape == (32,)
+    assert part.cache_need().kv == KvSpec(2, 32, bits=4)
