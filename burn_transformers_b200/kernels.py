@@ -1963,14 +1963,14 @@ def _fault(t, name, device, dtype, shape, note="contiguous") -> None:
 
 def _int_list(t, name, device, count) -> int:
     """The address of a contiguous list of at least `count` int32."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.shape[0] >= count
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.numel() >= count
             and t.is_contiguous()):
         _fault(t, name, device, torch.int32, f"a list of at least {count}")
     return t.data_ptr()
 
 
 def _float_list(t, name, device, count) -> int:
-    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.dim() == 1 and t.shape[0] >= count
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.dim() == 1 and t.numel() >= count
             and t.is_contiguous()):
         _fault(t, name, device, torch.float32, f"a list of at least {count}")
     return t.data_ptr()
@@ -1978,8 +1978,8 @@ def _float_list(t, name, device, count) -> int:
 
 def _row_stride(t, name, device, dtype, count, width, written=False) -> int:
     """Elements between the rows of `t`: at least `count` rows of at least `width` contiguous elements (apart, if they are written)."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.shape[0] >= count
-            and t.shape[1] >= width and (t.stride(1) == 1 or width == 1) and (not written or count < 2 or t.stride(0) >= width)):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.size(0) >= count
+            and t.size(1) >= width and (t.stride(1) == 1 or width == 1) and (not written or count < 2 or t.stride(0) >= width)):
         _fault(t, name, device, dtype, f"at least {count} rows of at least {width} elements", "contiguous within a row, rows apart")
     return t.stride(0)
 
