@@ -274,14 +274,15 @@ int bt_cache4_gather(void* k, long long k_row, long long k_head, void* v, long l
                      long long n_pages, const int* positions, const int* token_seq, const int* table, int n_table, int table_stride,
                      int table_len, int* status, int n_tokens, int n_kv_heads, int dim, int dtype, cudaStream_t stream);
 int bt_cache4_attention(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
-                        int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,
-                        int n_kv_heads, int dim, float scale, int window, int keep_first, int dtype, cudaStream_t stream);
+                        int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs, int max_new, int n_heads,
+                        int n_kv_heads, int dim, float scale, int window, int keep_first, int pieces, int rows,
+                        float* scratch, long long scratch_floats, int dtype, cudaStream_t stream);
 int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
-                     int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,
+                     int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs, int max_new, int n_heads,
                      int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits, int n_warps, float* scratch,
                      long long scratch_floats, cudaStream_t stream);
 int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
-                     int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs, int max_new, int n_heads,
+                     int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs, int max_new, int n_heads,
                      int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits, int rows, float* scratch,
                      long long scratch_floats, cudaStream_t stream);
 int bt_qk_norm_rotary(const void* src, long long src_row, void* dst, long long dst_row, const int* positions, const float* freq,

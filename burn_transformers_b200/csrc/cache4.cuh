@@ -44,6 +44,12 @@ __device__ __forceinline__ const unsigned char* c4_page(const Cache4View& c, int
   return c.pool + ((long long)page * c.n_kv_heads + kv_head) * c4_record(dim);
 }
 
+// A sequence's new tokens: rows t0 .. t0 + n_new - 1 of the step, which has n_tokens.
+__device__ __forceinline__ void c4_new_tokens(const int* seq_start, int seq, int n_tokens, int& t0, int& n_new) {
+  t0 = max(0, seq_start[seq]);
+  n_new = min(seq_start[seq + 1], n_tokens) - t0;
+}
+
 // Which keys the query at `pos` sees: `kept` first ones (0 .. kept - 1) and the run lo .. pos, which does not overlap them.
 __device__ __forceinline__ void c4_seen(int pos, int window, int keep_first, int& kept, int& lo) {
   lo = window > 0 ? max(0, pos - window + 1) : 0;

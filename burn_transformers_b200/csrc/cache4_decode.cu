@@ -1,7 +1,7 @@
 // Attention over a 4-bit cache (cache4.cuh) for steps that bring few tokens a sequence: bfloat16 queries, heads of 64 or 128 channels.
 //
 // A block serves one (sequence, key head) and 8 or 16 columns: the query heads that share the key head, for each new token.  Each of its
-// four warps takes pages of the visible run by itself, through a ring of its own (a page of a key head is one record: one bulk copy), so
+// warps takes pages of the visible run by itself, through a ring of its own (a page of a key head is one record: one bulk copy), so
 // that no barrier stands between pages.  With the keys on the 16 rows of an mma.sync tile and the columns on its 8:
 //   S^T = K q^T   a lane's 16 (8) bytes of a key row are 32 (16) channels in a row; the contraction may take the channels in any order, so
 //                 that the codes go to the tensor cores as they come out of the word (nibbles i and i + 4), and the queries are put in
@@ -12,9 +12,11 @@
 // Maximum, sum and products are 32-bit; the weights are rounded to bfloat16 for the second product, as the other attention kernels of
 // this library do.
 //
-// What bounds it: the integer pipe, which takes the codes apart (about 7 operations a key and key head of 128 channels and warp), close
-// to the memory behind it (136 bytes).  The run is cut into `n_splits` pieces where sequences and heads do not fill the GPU; their
-// partial results (maximum, sum, weighted values) are joined in order by a second kernel.
+// What bounds it: a page takes a warp a chain of dependent steps (1.45 us by itself, 3.2 beside eleven others, 0.27 a page and
+// multiprocessor), and 168 registers allow 12 warps; the integer pipe, which takes the codes apart (7 operations for a word of eight), is
+// active 64 % of the time, memory 61 % (64 sequences of 1,000 to 8,000 tokens, 32 heads over 8 of 128: 77 us, 4.1 TB/s).  Half precision,
+// which needs 5 operations for a word, came to the same.  A block has 4 to 12 warps and the run is cut into `n_splits` pieces as the caller's
+// model of their cost says (kernels.py); the pieces' results (maximum, sum, weighted values) are joined in order by a second kernel.
 // Keys that a column does not see get the weight 0 exactly, and what lies in a page past the sequence's end (any bytes) is never
 // multiplied; a value filed as NaN reaches the columns that see its key and no other.
 #include "cache4.cuh"
@@ -31,7 +33,7 @@ struct Cache4DecodeParams {
   long long q_row;
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
-  int n_heads, group, col_blocks, max_new, slots;
+  int n_tokens, n_heads, group, col_blocks, max_new, slots;
   float scale_log2;
   int window, keep_first;
   float* part;                 // [unit][split][columns][HD], then [unit][split][columns][2]
@@ -74,7 +76,9 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   const int n_warps = (int)blockDim.x >> 5;
   const int split = blockIdx.x, n_splits = gridDim.x, seq = blockIdx.z;
   const int kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS;
-  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0, n_cols = n_new * p.group - col0;
+  int t0, n_new;
+  c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
+  const int n_cols = n_new * p.group - col0;
   if (n_cols <= 0) return;
   const int past = p.past_len[seq];
   const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
@@ -441,7 +445,8 @@ cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
   pdl_trigger();
   pdl_wait();
   const int seq = blockIdx.z, kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS, col = blockIdx.x;
-  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  int t0, n_new;
+  c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (col0 + col >= n_new * p.group) return;
   const int past = p.past_len[seq];
   const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
@@ -511,7 +516,7 @@ static int launch_c4d(Cache4DecodeParams p, const Cache4View& c, int n_seqs, int
 // Arguments as bt_cache4_attention (bfloat16).  max_new * (n_heads / n_kv_heads) columns a key head go in blocks of 8 or 16.
 // scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * column blocks * splits * columns * (dim + 2).
 extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
-                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
+                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs,
                                 int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
                                 int n_warps, float* scratch, long long scratch_floats, cudaStream_t stream) {
   using namespace bt;
@@ -521,7 +526,7 @@ extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const
            "cache4_attention: bad sizes pages=%lld table_len=%d sequences=%d window=%d kept=%d", n_pages, table_len, n_seqs, window, keep_first);
   auto at16 = [](const void* x) { return (unsigned long long)x % 16 == 0; };
   BT_CHECK(at16(pool) && at16(q) && q_row % 8 == 0, "cache4_attention: pool and query rows must lie on 16-byte boundaries");
-  if (n_seqs == 0 || max_new == 0) return 0;
+  if (n_seqs == 0 || max_new == 0 || n_tokens == 0) return 0;
   const int group = n_heads / n_kv_heads;
   const long long cols = (long long)max_new * group;
   const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
@@ -530,7 +535,7 @@ extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const
   const long long parts = (long long)n_seqs * n_kv_heads * blocks * n_splits * 8 * nt;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, blocks, max_new, 0,
+  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_tokens, n_heads, group, blocks, max_new, 0,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, n_warps, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, n_warps, stream);

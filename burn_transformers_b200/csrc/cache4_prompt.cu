@@ -38,7 +38,7 @@ struct Cache4PromptParams {
   long long q_row;
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
-  int n_heads, group, rows;     // rows a block: 128 or 256
+  int n_tokens, n_heads, group, rows;     // rows a block: 128 or 256
   float scale_log2;
   int window, keep_first;
   float* part;                 // [unit][split][rows][HD], then [unit][split][rows][2]
@@ -102,7 +102,8 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   pdl_trigger();
   pdl_wait();
-  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  int t0, n_new;
+  c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * p.rows;      // (the longest blocks first)
   const int n_rows = min(p.rows, n_new * p.group - row0);
   if (n_rows <= 0) return;
@@ -453,7 +454,8 @@ cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, i
   pdl_wait();
   const int kv_head = (int)blockIdx.y % n_kv_heads, seq = (int)blockIdx.y / n_kv_heads;
   const int tile = (int)blockIdx.x / p.rows, r = (int)blockIdx.x % p.rows, row0 = (row_tiles - 1 - tile) * p.rows, row = row0 + r;
-  const int t0 = p.seq_start[seq], n_new = p.seq_start[seq + 1] - t0;
+  int t0, n_new;
+  c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (row >= n_new * p.group) return;
   const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
   const int used = (run.n_tiles + run.per - 1) / run.per;
@@ -489,7 +491,7 @@ static int launch_c4p(const Cache4PromptParams& p, const Cache4View& c, int n_se
 // Arguments as bt_cache4_attention (bfloat16).  scratch: 32-bit words for more than one split: n_seqs * n_kv_heads * row tiles (of `rows` rows:
 // max_new * (n_heads / n_kv_heads)) * splits * rows * (dim + 2).
 extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table,
-                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_seqs,
+                                int table_stride, int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs,
                                 int max_new, int n_heads, int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits,
                                 int rows, float* scratch, long long scratch_floats, cudaStream_t stream) {
   using namespace bt;
@@ -500,7 +502,7 @@ extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const
            "cache4_attention: bad sizes pages=%lld table_len=%d sequences=%d window=%d kept=%d", n_pages, table_len, n_seqs, window, keep_first);
   auto at16 = [](const void* x) { return (unsigned long long)x % 16 == 0; };
   BT_CHECK(at16(pool) && at16(q) && at16(out) && q_row % 8 == 0, "cache4_attention: pool, queries and results must lie on 16-byte boundaries");
-  if (n_seqs == 0 || max_new == 0) return 0;
+  if (n_seqs == 0 || max_new == 0 || n_tokens == 0) return 0;
   const int group = n_heads / n_kv_heads;
   BT_CHECK((long long)max_new * group < (1ll << 30), "cache4_attention: %d new tokens of %d heads are too many", max_new, group);
   const int row_tiles = (int)(((long long)max_new * group + rows - 1) / rows);
@@ -510,7 +512,7 @@ extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const
   const long long parts = units * row_tiles * n_splits * rows;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_heads, group, rows,
+  const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_tokens, n_heads, group, rows,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   if (dim == 64) return launch_c4p<64>(p, c, n_seqs, row_tiles, n_splits, stream);

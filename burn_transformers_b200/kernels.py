@@ -1936,9 +1936,9 @@ _ARGUMENTS = {
     "bt_qk_norm_rotary": "plplppppiiiiiffiip",
     "bt_cache4_append": "pllpllplppppiiipiiiip",
     "bt_cache4_gather": "pllpllplpppiiipiiiip",
-    "bt_cache4_attention": "plpplpiipppiiiiifiiip",
-    "bt_cache4_decode": "plpplpiipppiiiiifiiiiplp",
-    "bt_cache4_prompt": "plpplpiipppiiiiifiiiiplp",
+    "bt_cache4_attention": "plpplpiipppiiiiiifiiiiplip",
+    "bt_cache4_decode": "plpplpiipppiiiiiifiiiiplp",
+    "bt_cache4_prompt": "plpplpiipppiiiiiifiiiiplp",
 }
 
 
@@ -1991,6 +1991,9 @@ def _element_code(t, name) -> int:
     return code
 
 
+_INT_MAX = (1 << 31) - 1
+
+
 def _raw_stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
@@ -2002,6 +2005,8 @@ def _status_address(device: int) -> int:
     """The address of kernel_status (which stays where it is)."""
     hit = _STATUS_ADDRESS.get(device)
     if hit is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("the first of these calls on a device makes its status word and cannot be recorded: make one before the capture")
         hit = _STATUS_ADDRESS[device] = kernel_status(torch.device("cuda", device)).data_ptr()
     return hit
 
@@ -2152,20 +2157,26 @@ def _cache4_few(sms, units, pages, wide, head_dim):
     return best[1], best[2]
 
 
-def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first):
-    """Which kernel takes a step of these sizes in bfloat16, its warps a block ("few") or rows a block ("many"), its pieces of the keys,
+def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast):
+    """Which kernel takes a step of these sizes, its warps a block ("few") or rows a block ("many", "any"), its pieces of the keys,
     and the scratch that joining them takes: for the step itself, and for any of the same heads with fewer sequences or shorter ones.
 
-    "few": up to 16 columns (query heads of a key head, times new tokens) a key head, in blocks of 8 or 16; "many": the same as rows."""
-    if head_dim != 64 and head_dim != 128:
-        return "any", 0, 1, 0, 0
+    `fast` (bfloat16, on 16-byte boundaries) with heads of 64 or 128 channels: "few", up to 16 columns (query heads of a key head, times
+    new tokens) a key head, in blocks of 8 or 16, or "many", the same as rows.  Everything else: "any"."""
     columns = max_new * (n_heads // n_kv_heads)
     units = max(1, n_seqs * n_kv_heads)
-    span = max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE)
+    span = max(1, max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE))
     sms = _sm_count()
+    if not fast or (head_dim != 64 and head_dim != 128):
+        # blocks of 8 rows where there are several; keys in pieces of 256 at least, to eight blocks a multiprocessor
+        rows = 1 if columns <= 2 else 8
+        blocks = units * -(-columns // rows)
+        one, longest = rows * (head_dim + 2), -(-span // 256)
+        pieces = max(1, min(8 * sms // max(1, blocks), longest))
+        return "any", rows, pieces, blocks * pieces * one if pieces > 1 else 0, min(8 * sms, blocks * longest) * one
     if columns <= 16:
         wide = 8 if columns <= 8 else 16
-        pages = max(1, -(-span // PAGE_SIZE))
+        pages = -(-span // PAGE_SIZE)
         warps, pieces = _cache4_few(sms, units, pages, wide, head_dim)
         one = wide * (head_dim + 2)
         most = min(max(3 * sms, 3 * units), units * -(-pages // 4))
@@ -2174,11 +2185,12 @@ def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window
     # idle and the keys are too few to cut (two prompts of 1,024, 12 heads of 64: 23.6 us and 18.0; 8 of 512, 16 heads: 24.6 and 33.1)
     rows = 256
     tiles = -(-columns // rows)
-    pieces = max(1, min(sms // (units * tiles), -(-span // 1024)))
+    longest = -(-span // 1024)
+    pieces = max(1, min(sms // (units * tiles), longest))
     if pieces == 1 and 4 * units * tiles <= 3 * sms:
         rows = 128
     one = rows * (head_dim + 2)
-    return "many", rows, pieces, units * tiles * pieces * one if pieces > 1 else 0, min(sms, units * tiles * -(-span // 1024)) * one
+    return "many", rows, pieces, units * tiles * pieces * one if pieces > 1 else 0, min(sms, units * tiles * longest) * 256 * (head_dim + 2)
 
 
 def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
@@ -2193,7 +2205,7 @@ def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads,
     """32-bit words of `scratch` that cache4_attention wants for a step of these sizes, and at most for one of fewer or shorter
     sequences with as many new tokens."""
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
-    return _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)[4]
+    return max(_cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)[4] for fast in (True, False))
 
 
 def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads,
@@ -2222,9 +2234,8 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
-    kind, wide, splits, floats = "any", 0, 1, 0
-    if impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0:
-        kind, wide, splits, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first)
+    fast = impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0
+    kind, wide, pieces, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)
     partial = 0
     if floats:
         if scratch is None:
@@ -2232,11 +2243,12 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
         partial = _float_list(scratch, "scratch", device, floats)
     if _PROFILE is not None:
         _work()
-    head = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
-            _status_address(device), starts, pasts, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, window, keep_first)
+    call = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
+            _status_address(device), starts, pasts, n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, min(window, _INT_MAX),
+            min(keep_first, _INT_MAX), pieces, wide, partial, floats)
     if kind == "few":
-        _check(library().bt_cache4_decode(*head, splits, wide, partial, floats, _raw_stream(device)))
+        _check(library().bt_cache4_decode(*call, _raw_stream(device)))
     elif kind == "many":
-        _check(library().bt_cache4_prompt(*head, splits, wide, partial, floats, _raw_stream(device)))
+        _check(library().bt_cache4_prompt(*call, _raw_stream(device)))
     else:
-        _check(library().bt_cache4_attention(*head, code, _raw_stream(device)))
+        _check(library().bt_cache4_attention(*call, code, _raw_stream(device)))
