@@ -2,10 +2,10 @@
 // 32 channels up to 256, shared key heads, a window with kept first positions.
 //
 // A block serves one (sequence, key head) and up to 8 rows: row r is query head r % group of new token r / group.  With the keys that any
-// of its rows sees numbered in a row (kept first ones, then the window's run), it walks them in tiles of 128: a thread takes one key's codes
-// apart and forms its scores for all rows, the block each row's maximum and sum (a running softmax), then a thread mixes the tile's
-// values for one channel of all rows (for heads of fewer than 128 channels several threads do, each its share of the keys).  Keys that a
-// row does not see have the weight 0 and their values are left out, so that what lies there (NaN) does not matter.
+// of its rows sees numbered in a row (kept first ones, then the window's run), it walks them in tiles of 256: a thread takes two keys' codes
+// apart and forms their scores for all rows, the block each row's maximum and sum (a running softmax), then a thread mixes its share of
+// the tile's values for four channels of all rows.  Keys that a row does not see have the weight 0 and their values are left out, so that
+// what lies there (NaN) does not matter.
 //
 // What bounds it is the 32-bit multiply-adds and the reading of queries and weights from shared memory beside them; one row a block takes a
 // code apart for each multiply-add, eight for eight.  Where rows and heads do not fill the GPU the keys are cut into pieces, whose results a
@@ -14,7 +14,7 @@
 
 namespace bt {
 
-constexpr int C4S_THREADS = 128, C4S_TILE = 128;
+constexpr int C4S_THREADS = 128, C4S_KEYS = 2, C4S_TILE = C4S_KEYS * C4S_THREADS;
 
 struct Cache4AnyParams {
   const void* q;
@@ -72,80 +72,106 @@ cache4_attention_kernel(Cache4AnyParams p, Cache4View c) {
       x = to_float(reinterpret_cast<const T*>(p.q)[(at.t0 + row / p.group) * p.q_row + (long long)(kv_head * p.group + row % p.group) * dim + d]);
     s_q[r][d] = x;
   }
-  // channels of this thread, and which share of a tile's keys it mixes
-  const int shares = dim <= 64 ? C4S_THREADS / dim : 1, share = dim <= 64 ? tid / dim : 0, d0 = dim <= 64 ? tid % dim : tid;
-  float m[ROWS], l[ROWS], acc[2][ROWS];
+  // this thread's four channels, and which share of a tile's keys it mixes
+  const int quads = dim / 4, shares = C4S_THREADS / quads, share = tid / quads, d0 = tid % quads * 4;
+  float m[ROWS], l[ROWS], acc[4][ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     m[r] = -INFINITY;
-    l[r] = acc[0][r] = acc[1][r] = 0.f;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][r] = 0.f;
   }
   for (int first = begin; first < end; first += C4S_TILE) {
     const int count = min(C4S_TILE, end - first);
-    float score[ROWS];
-    bool sees[ROWS];
+    float score[C4S_KEYS][ROWS];
+    unsigned sees[C4S_KEYS];             // a bit a row
     __syncthreads();           // (the tile before has been mixed; the queries are there)
+    const uint4* codes[C4S_KEYS];
+    const unsigned char* scales[C4S_KEYS];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      score[r] = 0.f;
-      sees[r] = false;
-    }
-    if (tid < count) {
-      const int key = at.key(first + tid);
+    for (int k = 0; k < C4S_KEYS; ++k) {
+      const int j = min(tid + k * C4S_THREADS, count - 1);      // (a thread without a key of its own takes the last)
+      const int key = at.key(first + j), in_page = key % C4_PAGE;
       const unsigned char* rec = c4_page(c, seq, key / C4_PAGE, kv_head, dim);
-      const int in_page = key % C4_PAGE;
-      s_rec[tid] = rec;
-      s_in[tid] = in_page;
-      const uint4* codes = reinterpret_cast<const uint4*>(rec + in_page * (dim / 2));
-      const unsigned char* scales = rec + c4_key_scales(dim) + in_page * (dim / 32);
-      for (int g = 0; g < dim / 32; ++g) {
-        const uint4 raw = codes[g];
-        const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
-        const float s = c4_scale(scales[g]);
-        float part[ROWS];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) part[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float k[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) k[i] = c4_number(w[e >> 3] >> (4 * ((e & 7) + i)) & 15u);
-#pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const float4 q = *reinterpret_cast<const float4*>(&s_q[r][32 * g + e]);
-            part[r] = fmaf(k[0], q.x, fmaf(k[1], q.y, fmaf(k[2], q.z, fmaf(k[3], q.w, part[r]))));
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) score[r] = fmaf(part[r], s, score[r]);
+      if (tid + k * C4S_THREADS < count) {
+        s_rec[j] = rec;
+        s_in[j] = in_page;
       }
+      codes[k] = reinterpret_cast<const uint4*>(rec + in_page * (dim / 2));
+      scales[k] = rec + c4_key_scales(dim) + in_page * (dim / 32);
+      sees[k] = 0u;
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
+        score[k][r] = 0.f;
         const int pos = at.past + (at.row0 + r) / p.group;
-        sees[r] = r < at.n_rows && key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first);
-        score[r] *= p.scale;
+        if (tid + k * C4S_THREADS < count && r < at.n_rows && key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first))
+          sees[k] |= 1u << r;
+      }
+    }
+    for (int g = 0; g < dim / 32; ++g) {
+      unsigned w[C4S_KEYS][4];
+      float part[C4S_KEYS][ROWS];
+#pragma unroll
+      for (int k = 0; k < C4S_KEYS; ++k) {
+        const uint4 raw = codes[k][g];
+        w[k][0] = raw.x; w[k][1] = raw.y; w[k][2] = raw.z; w[k][3] = raw.w;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) part[k][r] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        float x[C4S_KEYS][4];
+#pragma unroll
+        for (int k = 0; k < C4S_KEYS; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[k][i] = c4_number(w[k][e >> 3] >> (4 * ((e & 7) + i)) & 15u);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float4 q = *reinterpret_cast<const float4*>(&s_q[r][32 * g + e]);
+#pragma unroll
+          for (int k = 0; k < C4S_KEYS; ++k)
+            part[k][r] = fmaf(x[k][0], q.x, fmaf(x[k][1], q.y, fmaf(x[k][2], q.z, fmaf(x[k][3], q.w, part[k][r]))));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < C4S_KEYS; ++k) {
+        const float s = c4_scale(scales[k][g]);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) score[k][r] = fmaf(part[k][r], s, score[k][r]);
       }
     }
     // each row's maximum over the tile (a maximum passes over NaN; the weight and the sum keep it)
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const float top = warp_max(sees[r] ? score[r] : -INFINITY);
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < C4S_KEYS; ++k) {
+        score[k][r] *= p.scale;
+        if (sees[k] >> r & 1u) top = fmaxf(top, score[k][r]);
+      }
+      top = warp_max(top);
       if (lane == 0) s_red[0][warp][r] = top;
     }
     __syncthreads();
-    float keep[ROWS], weight[ROWS];
+    float keep[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float m_new = m[r];
+      float m_new = m[r], sum = 0.f;
 #pragma unroll
       for (int i = 0; i < C4S_THREADS / 32; ++i) m_new = fmaxf(m_new, s_red[0][i][r]);
-      weight[r] = !sees[r] || (m_new == -INFINITY && score[r] == score[r]) ? 0.f : expf(score[r] - m_new);
+#pragma unroll
+      for (int k = 0; k < C4S_KEYS; ++k) {
+        const bool mine = sees[k] >> r & 1u;
+        const float weight = !mine || (m_new == -INFINITY && score[k][r] == score[k][r]) ? 0.f : expf(score[k][r] - m_new);
+        sum += weight;
+        // (a key that this row does not see: its values are left out, by a weight that no other has)
+        s_p[tid + k * C4S_THREADS][r] = mine ? weight : -1.f;
+      }
       keep[r] = m[r] == -INFINITY ? 0.f : expf(m[r] - m_new);
       m[r] = m_new;
-      const float sum = warp_sum(weight[r]);
+      sum = warp_sum(sum);
       if (lane == 0) s_red[1][warp][r] = sum;
-      // (a key that this row does not see: its values are left out, by a weight that no other has)
-      s_p[tid][r] = sees[r] ? weight[r] : -1.f;
     }
     __syncthreads();
 #pragma unroll
@@ -154,28 +180,28 @@ cache4_attention_kernel(Cache4AnyParams p, Cache4View c) {
 #pragma unroll
       for (int i = 0; i < C4S_THREADS / 32; ++i) sum += s_red[1][i][r];
       l[r] = l[r] * keep[r] + sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i][r] *= keep[r];
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int d = d0 + h * C4S_THREADS;
-      if (d >= dim || share >= shares || (h > 0 && dim <= C4S_THREADS)) continue;
-      float sum[ROWS];
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) sum[r] = 0.f;
-#pragma unroll 4
+    if (share < shares) {
+#pragma unroll 2
       for (int j = share; j < count; j += shares) {
         const unsigned char* rec = s_rec[j];
         const int in_page = s_in[j];
-        const unsigned n = rec[c4_value_codes(dim) + in_page * (dim / 2) + d / 2] >> (4 * (d & 1)) & 15u;
-        const float v = c4_number(n) * c4_scale(rec[c4_value_scales(dim) + in_page * (dim / 32) + d / 32]);
+        const unsigned n = *reinterpret_cast<const unsigned short*>(rec + c4_value_codes(dim) + in_page * (dim / 2) + d0 / 2);
+        const float s = c4_scale(rec[c4_value_scales(dim) + in_page * (dim / 32) + d0 / 32]);
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = c4_number(n >> (4 * i) & 15u) * s;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           const float w = s_p[j][r];
-          sum[r] = w >= 0.f || w != w ? fmaf(w, v, sum[r]) : sum[r];
+          if (w >= 0.f || w != w) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i][r] = fmaf(w, v[i], acc[i][r]);
+          }
         }
       }
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) acc[h][r] = acc[h][r] * keep[r] + sum[r];
     }
   }
   // the shares of a channel, joined in order (over the queries)
@@ -184,35 +210,34 @@ cache4_attention_kernel(Cache4AnyParams p, Cache4View c) {
     __syncthreads();
     if (share == from) {
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) s_acc[r][d0] = acc[0][r];
+      for (int r = 0; r < ROWS; ++r) *reinterpret_cast<float4*>(&s_acc[r][d0]) = make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]);
     }
     __syncthreads();
     if (share == 0) {
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) acc[0][r] += s_acc[r][d0];
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][r] += s_acc[r][d0 + i];
     }
   }
   if (share != 0) return;
   const long long unit = ((long long)seq * gridDim.y + kv_head) * ((int)gridDim.x / p.pieces) + row_block;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int d = d0 + h * C4S_THREADS;
-    if (d >= dim || (h > 0 && dim <= C4S_THREADS)) continue;
+  for (int r = 0; r < ROWS; ++r) {
+    if (r >= at.n_rows) continue;
+    const int row = at.row0 + r;
+    const long long place = (unit * p.pieces + piece) * ROWS + r;
+    T* dst = reinterpret_cast<T*>(p.out) + ((long long)(at.t0 + row / p.group) * p.n_heads + kv_head * p.group + row % p.group) * dim + d0;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (r >= at.n_rows) continue;
-      const int row = at.row0 + r;
-      if (p.pieces == 1) {
-        reinterpret_cast<T*>(p.out)[((long long)(at.t0 + row / p.group) * p.n_heads + kv_head * p.group + row % p.group) * dim + d] =
-            from_float<T>(acc[h][r] / l[r]);
-      } else {
-        const long long place = (unit * p.pieces + piece) * ROWS + r;
-        p.part[place * dim + d] = acc[h][r];
-        if (d == 0) {
-          p.part[p.part_ml + 2 * place] = m[r];
-          p.part[p.part_ml + 2 * place + 1] = l[r];
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      if (p.pieces == 1)
+        dst[i] = from_float<T>(acc[i][r] / l[r]);
+      else
+        p.part[place * dim + d0 + i] = acc[i][r];
+    }
+    if (p.pieces > 1 && d0 == 0) {
+      p.part[p.part_ml + 2 * place] = m[r];
+      p.part[p.part_ml + 2 * place + 1] = l[r];
     }
   }
 }
