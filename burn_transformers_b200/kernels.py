@@ -2127,7 +2127,6 @@ def _sm_count() -> int:
     return _SM_COUNTS[device]
 
 
-@functools.lru_cache(maxsize=4096)
 def _cache4_few(sms, units, pages, wide, head_dim):
     """(warps a block, pieces of the keys) for `units` blocks' worth of columns over `pages` pages each, at most.
 
@@ -2157,7 +2156,8 @@ def _cache4_few(sms, units, pages, wide, head_dim):
     return best[1], best[2]
 
 
-def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast):
+@functools.lru_cache(maxsize=4096)
+def _cache4_plan(sms, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast):
     """Which kernel takes a step of these sizes, its warps a block ("few") or rows a block ("many", "any"), its pieces of the keys,
     and the scratch that joining them takes: for the step itself, and for any of the same heads with fewer sequences or shorter ones.
 
@@ -2166,7 +2166,6 @@ def _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window
     columns = max_new * (n_heads // n_kv_heads)
     units = max(1, n_seqs * n_kv_heads)
     span = max(1, max_ctx if not window else min(max_ctx, window + max_new + keep_first + 2 * PAGE_SIZE))
-    sms = _sm_count()
     if not fast or (head_dim != 64 and head_dim != 128):
         # blocks of 8 rows where there are several; keys in pieces of 256 at least, to eight blocks a multiprocessor
         rows = 1 if columns <= 2 else 8
@@ -2205,7 +2204,7 @@ def cache4_attention_scratch_floats(n_tokens, n_seqs, max_new, max_ctx, n_heads,
     """32-bit words of `scratch` that cache4_attention wants for a step of these sizes, and at most for one of fewer or shorter
     sequences with as many new tokens."""
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
-    return max(_cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)[4] for fast in (True, False))
+    return max(_cache4_plan(_sm_count(), n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)[4] for fast in (True, False))
 
 
 def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads,
@@ -2235,7 +2234,7 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
     fast = impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0
-    kind, wide, pieces, floats, _ = _cache4_plan(n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)
+    kind, wide, pieces, floats, _ = _cache4_plan(_sm_count(), n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)
     partial = 0
     if floats:
         if scratch is None:
