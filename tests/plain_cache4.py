@@ -57,8 +57,9 @@ def attention(q, k, v, past, scale, window=0, keep_first=0):
 
 def allowed(dtype_bits, y, size, reach, count, dim):
     """How far a result may be from `y`: products and sums in 32 bits, and for 8-bit significands (bfloat16) the weights and the result
-    each rounded once."""
-    exact = size * 2.0 ** -24 * (2 * (dim + 8) * reach + 2 * count[:, None] + 64)[..., None]
+    each rounded once.  A weight below 2^-126 of the largest has no normal 32-bit number and may be 0: that much of a value, which is 25,088 at
+    most, for each key."""
+    exact = count[:, None, None] * 2.0 ** -126 * 25088 + size * 2.0 ** -24 * (2 * (dim + 8) * reach + 2 * count[:, None] + 64)[..., None]
     if dtype_bits == 8:
         return 2.0 ** -8 * (1 + 2.0 ** -7) * (np.abs(y) + size) + exact
     return exact + 2.0 ** -24 * np.abs(y)

@@ -160,11 +160,15 @@ def test_what_is_allowed_reaches_the_library(call, change):
         call(**change)
 
 
-def test_the_scratch_that_is_asked_for_covers_every_shorter_step():
-    """A recorded step keeps the scratch of its bounds: fewer tokens a sequence or shorter sequences never need more."""
-    for heads, kv, dim in ((32, 8, 128), (12, 12, 64), (8, 1, 64)):
-        for seqs in (1, 3, 64):
-            for window, keep in ((0, 0), (100, 0), (1000, 4)):
-                most = kernels.cache4_attention_scratch_floats(seqs, seqs, 1, 1 << 17, heads, kv, dim, window, keep)
-                for ctx in (1, 63, 64, 1000, 30_000):
-                    assert kernels.cache4_attention_scratch_floats(seqs, seqs, 1, ctx, heads, kv, dim, window, keep) <= most
+@pytest.mark.parametrize("heads, kv, dim", [(32, 8, 128), (12, 12, 64), (8, 1, 64), (6, 3, 96)])
+@pytest.mark.parametrize("new", [1, 3, 40, 700])
+@pytest.mark.parametrize("window, keep", [(0, 0), (100, 0), (1000, 4)])
+def test_the_scratch_that_is_asked_for_covers_every_smaller_step(heads, kv, dim, new, window, keep):
+    """A program keeps the scratch of its bounds: fewer or shorter sequences never need more, whichever kernel takes them."""
+    sizes = [(seqs, ctx) for seqs in (1, 2, 5, 64, 300) for ctx in (new, new + 63, new + 1000, new + 30_000, 1 << 17)]
+    asked = {s: kernels.cache4_attention_scratch_floats(s[0] * new, s[0], new, s[1], heads, kv, dim, window, keep) for s in sizes}
+    for seqs, ctx in sizes:
+        needs = [kernels._cache4_plan(148, fewer, new, shorter, heads, kv, dim, window, keep, fast)[3]
+                 for fewer in {1, 2, 3, 5, 17, 64, 300} if fewer <= seqs for shorter in {new, new + 63, new + 200, new + 1000, new + 9_000, ctx}
+                 if shorter <= ctx for fast in (True, False)]
+        assert max(needs) <= asked[seqs, ctx], (seqs, ctx)

@@ -229,3 +229,109 @@ def test_a_key_or_value_of_nan_reaches_the_queries_that_see_it_and_no_other(dtyp
                 hit[t, h * (heads // kv):(h + 1) * (heads // kv), channels] = True
         assert torch.equal(torch.isnan(got), hit), (where, which)
         assert torch.equal(got[~hit], clean.view(got.shape)[~hit])
+
+
+@pytest.mark.parametrize("heads, kv, dim, news", [(4, 4, 64, [1, 1]), (4, 4, 64, [40, 3]), (2, 2, 32, [2, 1]), (64, 1, 128, [1, 1])])
+def test_a_page_outside_the_pool_is_reported(heads, kv, dim, news):
+    step, rng = Step([100, 70], news), np.random.default_rng(1)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    k, v = (torch.zeros(step.n, kv, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for wrong in (-1, step.pages, 2 ** 31 - 1):
+        table = step.table.clone()
+        table[1, 0] = wrong
+        table[1, 1] = wrong
+        args = step.sizes(heads, kv, dim)
+        out = torch.empty(step.n, heads * dim, dtype=torch.bfloat16, device=DEV)
+        scratch = torch.empty(kernels.cache4_attention_scratch_floats(**args), device=DEV)
+        before = pool.clone()
+        calls = [lambda: kernels.cache4_attention(q, out, pool, table, step.width, step.seq_start, step.past, scale=1.0, scratch=scratch, **args),
+                 lambda: kernels.cache4_append(k, v, pool, step.positions, step.token_seq, step.ctx, table, step.width, n_tokens=step.n),
+                 lambda: kernels.cache4_gather(pool, step.positions, step.token_seq, table, step.width, k, v, n_tokens=step.n)]
+        for call in calls:
+            call()
+            with pytest.raises(KernelError, match="outside its table or pool"):
+                kernels.check_status(torch.device(DEV))
+        first = step.starts[1]
+        assert bool(torch.isnan(k[first:]).all()) and not bool(torch.isnan(k[:first]).any())
+        pages = [int(p) for p in step.lists[0]]
+        others = [p for p in range(step.pages) if p not in pages]
+        assert torch.equal(pool[others], before[others])          # (nothing of the second sequence went anywhere)
+        pool.copy_(before)
+        k.zero_()
+        v.zero_()
+
+
+def test_tokens_of_a_sequence_or_position_outside_the_table_are_reported():
+    kv, dim = 2, 64
+    pool = torch.zeros(3, kv, 68 * dim, dtype=torch.uint8, device=DEV)
+    k = torch.ones(4, kv, dim, dtype=torch.bfloat16, device=DEV)
+    table = ints([[0, 1]])
+    for seq, pos in (([0, 0, 0, 1], [0, 1, 2, 3]), ([0, 0, -1, 0], [0, 1, 2, 3]), ([0, 0, 0, 0], [0, 1, -5, 3])):
+        pool.zero_()
+        kernels.cache4_append(k, k, pool, ints(pos), ints(seq), ints([4]), table, 2, n_tokens=4)
+        with pytest.raises(KernelError, match="outside its table or pool"):
+            kernels.check_status(torch.device(DEV))
+        assert int((pool[0, 0, 64 * dim:66 * dim] != 0).sum()) == 3 * dim // 32      # (the three others are filed)
+
+
+@pytest.mark.parametrize("heads, kv, dim", [(4, 4, 64), (32, 4, 128), (3, 1, 96)])
+def test_what_a_step_may_leave_out(heads, kv, dim):
+    """No tokens, no sequences, sequences without tokens, starts that lie behind the step's tokens."""
+    step, rng = Step([30, 5, 64, 7], [0, 3, 0, 1]), np.random.default_rng(4)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n + 3, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, 0, 0, 0.1)
+    compare(step, got, q, keys, values, heads, kv, dim, 0, 0, 0.1)
+    out = torch.full((step.n, heads * dim), 5.0, dtype=torch.bfloat16, device=DEV)
+    args = step.sizes(heads, kv, dim)
+    scratch = torch.empty(kernels.cache4_attention_scratch_floats(**args), device=DEV)
+    for change in (dict(n_tokens=0), dict(n_seqs=0), dict(max_new=0)):
+        kernels.cache4_attention(q, out, pool, step.table, step.width, step.seq_start, step.past, scale=0.1, scratch=scratch, **{**args, **change})
+    assert bool((out == 5).all())
+    # the last sequence's tokens are not the step's: its rows stay as they are
+    kernels.cache4_attention(q[:3], out, pool, step.table, step.width, step.seq_start, step.past, scale=0.1, scratch=scratch, **{**args, "n_tokens": 3})
+    assert bool((out[3:] == 5).all()) and torch.equal(out[:3], got[:3])
+    empty = torch.empty(0, kv, dim, dtype=torch.bfloat16, device=DEV)
+    kernels.cache4_append(empty, empty, pool, ints([]), ints([]), step.ctx, step.table, step.width, n_tokens=0)
+    kernels.cache4_gather(pool, ints([]), ints([]), step.table, step.width, empty, empty, n_tokens=0)
+    kernels.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv, dim", [(2, 2, 64), (64, 1, 128), (24, 1, 64)])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+@pytest.mark.parametrize("news", [[1, 2], [90, 1]])
+def test_scales_rows_of_any_alignment_and_windows_of_any_length(dtype, heads, kv, dim, scale, news):
+    step, rng = Step([150, 10], news), np.random.default_rng(heads)
+    pool, keys, values = filled(step, kv, dim, rng)
+    for shift, window in ((0, 1 << 40), (1, 33)):
+        q = torch.tensor(rng.standard_normal((step.n, heads * dim + 9))).to(dtype).to(DEV)[:, shift:]
+        got = attend(step, q, pool, heads, kv, dim, window, 5, scale)
+        compare(step, got, q, keys, values, heads, kv, dim, window, 5, scale)
+
+
+@pytest.mark.parametrize("heads, kv, dim, news", [(2, 2, 64, [1, 1]), (4, 1, 128, [60, 1]), (2, 1, 96, [5, 1])])
+def test_queries_that_are_no_numbers(heads, kv, dim, news):
+    """A row of NaN or infinities is NaN, and no other row notices."""
+    step, rng = Step([500, 70], news), np.random.default_rng(3)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    clean = attend(step, q, pool, heads, kv, dim, 0, 0, 0.1).view(step.n, heads, dim)
+    for value in (float("nan"), float("inf"), float("-inf")):
+        bad = q.clone()
+        bad[-1, 3] = value
+        got = attend(step, bad, pool, heads, kv, dim, 0, 0, 0.1).view(step.n, heads, dim)
+        assert bool(torch.isnan(got[-1, 0]).all())
+        assert torch.equal(got[:-1], clean[:-1]) and torch.equal(got[-1, 1:], clean[-1, 1:])
+
+
+def test_a_window_over_pages_that_come_round():
+    """Pages of a ring hold the newest positions only; rows that have been overwritten are never looked at."""
+    for heads, kv, dim in ((2, 2, 64), (8, 1, 128), (2, 1, 96)):
+        for window, pasts, news in ((100, [1000, 130], [1, 1]), (60, [777, 64], [5, 30]), (20, [500, 3], [100, 2])):
+            step, rng = Step(pasts, news, ring=3), np.random.default_rng(window)
+            pool, keys, values = filled(step, kv, dim, rng)
+            q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+            got = attend(step, q, pool, heads, kv, dim, window, 0, 0.1)
+            compare(step, got, q, keys, values, heads, kv, dim, window, 0, 0.1)
