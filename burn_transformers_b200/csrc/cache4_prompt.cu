@@ -3,7 +3,7 @@
 //
 // A block serves one (sequence, key head) and 256 rows (or 128): row r is query head r % group of new token r / group, so that heads which
 // share a key head share its keys, however many new tokens there are.  The rows are two tiles of 128 (rows of the tensor memory), and the
-// visible keys go by in tiles of 128, in steps of 64.  Sixteen warps:
+// visible pages go by in steps of one (64 keys), staged two at a time.  Sixteen warps:
 //   0-3, 4-7  softmax, a thread a row of tile 0 or 1: a step's scores from tensor memory into registers, running maximum and sum in
 //         32-bit, weights as bfloat16 back over the scores they were made of, from where P V takes them.  The output accumulates in
 //         tensor memory and is rescaled only when a row's maximum has outgrown the one its weights are formed with by more than 2^8;
@@ -20,9 +20,9 @@
 // beforehand, for all blocks of rows at once: 316, but 91 for the short ones.
 // Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of tiles, whose results a second kernel joins in order.
 //
-// Masked keys get the weight 0 exactly.  A value filed as NaN reaches the rows that see its key and no other: in a tile that every row
-// of the block sees it is multiplied as it is; in the few others (seven at most: the diagonal's three, as many at the window's far edge,
-// the last kept one) it is multiplied as 0 and noted, and the rows look at the notes at the end.
+// Masked keys get the weight 0 exactly.  A value filed as NaN reaches the rows that see its key and no other: in a page that every row
+// of the block sees it is multiplied as it is; in the few others (eleven at most: five on the diagonal, as many at the window's far edge, the
+// last kept one) it is multiplied as 0 and noted, and the rows look at the notes at the end.
 // All hand-overs go through mbarriers; every wait is bounded, and one that runs out sets the status word.
 #include "attention_tcgen05.cuh"
 #include "cache4.cuh"
@@ -31,7 +31,7 @@
 namespace bt {
 
 constexpr int C4P_THREADS = 512;
-constexpr int C4P_EDGES = 8;            // tiles that not every row of a block sees: at most 7
+constexpr int C4P_EDGES = 12;           // pages that not every row of a block sees: at most 11
 
 struct Cache4PromptParams {
   const __nv_bfloat16* q;
@@ -51,19 +51,19 @@ struct C4pShape {
   static constexpr size_t SMEM = (size_t)6 * TILE;               // two tiles of queries, two stages of keys and of values
 };
 
-// The tiles of keys that a block's rows see, and how they are cut: the same for the attention and the kernel that joins.
+// The pages that a block's rows see, and how they are cut: the same for the attention and the kernel that joins.
 struct C4pRun {
-  int past, pos_first, pos_last, kept_only, kt_lo, n_tiles, per;
+  int past, pos_first, pos_last, kept_only, pg_lo, n_pages, per;
   __device__ C4pRun(int past_, int n_new, int row0, int rows, int group, int window, int keep_first, int n_splits) : past(past_) {
     pos_first = past + row0 / group;
     pos_last = past + min(n_new * group - 1, row0 + rows - 1) / group;
     const int lo = window > 0 ? max(0, pos_first - window + 1) : 0;
-    kt_lo = lo / TA_BK;
-    kept_only = window > 0 ? min((min(keep_first, pos_last + 1) + TA_BK - 1) / TA_BK, kt_lo) : 0;
-    n_tiles = kept_only + pos_last / TA_BK - kt_lo + 1;
-    per = (n_tiles + n_splits - 1) / n_splits;
+    pg_lo = lo / C4_PAGE;
+    kept_only = window > 0 ? min((min(keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;
+    n_pages = kept_only + pos_last / C4_PAGE - pg_lo + 1;
+    per = (n_pages + n_splits - 1) / n_splits;
   }
-  __device__ int tile_at(int i) const { return i < kept_only ? i : kt_lo + (i - kept_only); }
+  __device__ int page_at(int i) const { return i < kept_only ? i : pg_lo + (i - kept_only); }
 };
 
 // 32 channels of a row of keys or values (16 bytes of codes, one scale) as bfloat16, to their places in a tile.
@@ -90,7 +90,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   constexpr int TILE = C4pShape<HD>::TILE, CH = HD / 32, ISSUER = 12;
   extern __shared__ __align__(1024) unsigned char c4p_raw[];
   __shared__ __align__(8) unsigned long long bars[20];
-  __shared__ unsigned s_nan[C4P_EDGES][CH][4];      // a bit a key of a tile that not every row sees
+  __shared__ unsigned s_nan[C4P_EDGES][CH][2];      // a bit a key of a page that not every row sees
   __shared__ int s_edge_key[C4P_EDGES], s_edges;
   __shared__ unsigned s_tmem;
   __shared__ int s_failed;
@@ -108,8 +108,9 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   const int n_rows = min(p.rows, n_new * p.group - row0);
   if (n_rows <= 0) return;
   const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, (int)gridDim.z);
-  const int it0 = (int)blockIdx.z * run.per, n_tiles = min(run.n_tiles, it0 + run.per) - it0;
-  if (n_tiles <= 0) return;
+  // steps of a page each; two in a row are a tile of the stages
+  const int page0 = (int)blockIdx.z * run.per, n_steps = min(run.n_pages, page0 + run.per) - page0, n_tiles = (n_steps + 1) / 2;
+  if (n_steps <= 0) return;
   if ((ta_smem(c4p_raw) & 1023u) != 0) {      // the swizzled layouts need the alignment: refuse rather than compute nonsense
     if (tid == 0 && c.status) atomicExch(c.status, 10);
     return;
@@ -132,7 +133,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
     s_edges = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (tid < C4P_EDGES * CH * 4) (&s_nan[0][0][0])[tid] = 0u;
+  if (tid < C4P_EDGES * CH * 2) (&s_nan[0][0][0])[tid] = 0u;
   if (warp == ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(ta_smem(&s_tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -155,9 +156,6 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   __syncthreads();
   ta_fence_after();
   const unsigned tmem = s_tmem, tmem_o = tmem + 256;      // S of both tiles of rows, two steps each (64 columns, the weights over the first 32); O
-  // steps of 64 keys: the last tile's second half may lie past every row's last key
-  const bool ends_early = run.tile_at(it0 + n_tiles - 1) * TA_BK + 64 > run.pos_last;
-  const int n_steps = 2 * n_tiles - (ends_early ? 1 : 0);
 
   // registers: 512 threads x 128 at launch are 2 x 128 x 176 + 2 x 128 x 80
   if (warp < 8) {
@@ -175,7 +173,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       bool ok = true;
 #pragma unroll 1
       for (int j = 0; j < n_steps; ++j) {
-        const int key0 = run.tile_at(it0 + (j >> 1)) * TA_BK + 64 * (j & 1);
+        const int key0 = run.page_at(page0 + j) * C4_PAGE;
         const bool whole = key0 + 63 <= at_first && (p.window <= 0 || key0 > at_last - p.window || key0 + 64 <= p.keep_first);
         ok = __all_sync(0xffffffffu, ta_bar_wait(&s_full[2 * sub + (j & 1)], (j >> 1) & 1));
         if (!ok) break;                  // (uniform in the warp; the others run into their own bounds)
@@ -266,14 +264,14 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         unsigned lost = 0;
         auto look = [&](int key0, int word, unsigned bits) {
           while (bits) {
-            const int key = key0 + 32 * (word & 3) + __ffs(bits) - 1;
+            const int key = key0 + 32 * (word & 1) + __ffs(bits) - 1;
             bits &= bits - 1;
-            if (key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first)) lost |= 1u << (word >> 2);
+            if (key <= pos && (p.window <= 0 || key > pos - p.window || key < p.keep_first)) lost |= 1u << (word >> 1);
           }
         };
         const int edges = *(volatile int*)&s_edges;
         for (int e = 0; e < edges; ++e)
-          for (int j = 0; j < CH * 4; ++j) look(s_edge_key[e], j, s_nan[e][j >> 2][j & 3]);
+          for (int j = 0; j < CH * 2; ++j) look(s_edge_key[e], j, s_nan[e][j >> 1][j & 1]);
         const bool mine = sub * TA_BQ + r < n_rows;
         const bool cut = gridDim.z > 1;
         const float inv = cut ? 1.f : 1.f / l;
@@ -323,19 +321,23 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       unsigned long long *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
       const int codes_at = (values ? c4_value_codes(HD) : 0) + chunk * 16, scales_at = (values ? c4_value_scales(HD) : c4_key_scales(HD)) + chunk;
       const C4Bits bits;
-      // the records of the next 32 half tiles, one a lane.  (A half tile past the last key that a row sees repeats the last page: masked, and
-      // NaN there is nobody's)
-      auto record_of = [&](int half) {
-        const int it = min(half >> 1, n_tiles - 1), key = min(run.tile_at(it0 + it) * TA_BK + (half & 1) * C4_PAGE, run.pos_last);
-        return (unsigned long long)c4_page(c, seq, key / C4_PAGE, kv_head, HD);
+      // the records of the next 32 pages, one a lane (behind the last: the last again), and a bit a page that not every row sees
+      unsigned long long records;
+      unsigned narrow, narrow_now;
+      auto look_up = [&](int j) {
+        const int page = run.page_at(page0 + min(j, n_steps - 1)), key0 = page * C4_PAGE;
+        records = (unsigned long long)c4_page(c, seq, page, kv_head, HD);
+        const bool whole = key0 + C4_PAGE - 1 <= run.pos_first && (p.window <= 0 || key0 > run.pos_last - p.window || key0 + C4_PAGE <= p.keep_first);
+        narrow = __ballot_sync(0xffffffffu, !whole && j < n_steps);
       };
-      unsigned long long records = record_of(lane);
+      look_up(lane);
       uint4 raw[MOST];
       unsigned sc[MOST];
       auto fetch = [&](int it) {
         const unsigned char* rec0 = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, records, (2 * it) & 31));
         const unsigned char* rec1 = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, records, (2 * it + 1) & 31));
-        if ((it & 15) == 15) records = record_of(2 * it + 2 + lane);
+        narrow_now = narrow >> ((2 * it) & 31) & 3u;
+        if ((it & 15) == 15) look_up(2 * it + 2 + lane);
 #pragma unroll
         for (int j = 0; j < MOST; ++j) {
           const int unit = j * step + who;
@@ -351,15 +353,13 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       fetch(0);
 #pragma unroll 1
       for (int it = 0; it < n_tiles; ++it) {
-        const int s = it & 1, key0 = run.tile_at(it0 + it) * TA_BK;
-        const bool whole = key0 + TA_BK - 1 <= run.pos_first && (p.window <= 0 || key0 > run.pos_last - p.window || key0 + TA_BK <= p.keep_first);
-        const int edge = min(edges, C4P_EDGES - 1);
-        if (!whole) {
-          if (values && who == 0 && lane == 0) {
-            s_edge_key[edge] = key0;
-            *(volatile int*)&s_edges = edge + 1;
-          }
-          ++edges;
+        const int s = it & 1;
+        const unsigned now = narrow_now;
+        if (values && now && who == 0 && lane == 0) {
+          const int page = run.page_at(page0 + 2 * it + ((now & 1u) ? 0 : 1)), more = now == 3u ? 1 : 0;
+          s_edge_key[min(edges, C4P_EDGES - 1)] = page * C4_PAGE;
+          if (more) s_edge_key[min(edges + 1, C4P_EDGES - 1)] = run.page_at(page0 + 2 * it + 1) * C4_PAGE;
+          *(volatile int*)&s_edges = min(edges + 1 + more, C4P_EDGES);
         }
         if (it >= 2) ok = __all_sync(0xffffffffu, ta_bar_wait(&empty[s], ((it >> 1) - 1) & 1));
         if (!ok) break;
@@ -368,13 +368,15 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
           const int unit = j * step + who;
           if (unit >= UNITS) continue;
           const int r = SPAN * unit + sub_row;
+          const int half = SPAN * unit < C4_PAGE ? 0 : 1;
           unsigned sb = c4_scale_bits(sc[j]);
-          if (values && !whole && sc[j] == 255u) {
+          if (values && (now >> half & 1u) && sc[j] == 255u) {
             sb = 0u;
-            atomicOr(&s_nan[edge][chunk][r >> 5], 1u << (r & 31));
+            atomicOr(&s_nan[min(edges + (half & (int)now), C4P_EDGES - 1)][chunk][r / 32 & 1], 1u << (r & 31));
           }
           c4p_place(stage0 + s * TILE, r, chunk, raw[j], sb, bits);
         }
+        if (values) edges += __popc(now);
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         c4p_bar_arrive_warp(&full[s], lane);
         if (it + 1 < n_tiles) fetch(it + 1);
@@ -458,7 +460,7 @@ cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, i
   c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (row >= n_new * p.group) return;
   const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
-  const int used = (run.n_tiles + run.per - 1) / run.per;
+  const int used = (run.n_pages + run.per - 1) / run.per;
   float top = -INFINITY, sum = 0.f, o = 0.f;
   for (int s = 0; s < used; ++s) {
     const long long unit = (((long long)blockIdx.y * row_tiles + tile) * n_splits + s) * p.rows + r;
