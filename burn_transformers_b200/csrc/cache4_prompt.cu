@@ -12,13 +12,14 @@
 //   8-10, 11, 14 and 15  take the keys' and the values' codes apart: a lane reads 16 bytes (32 channels, one scale) of the next tile ahead,
 //         turns them into the exact bfloat16 values (cache4_codes.cuh) and stores them where the products read them.  A word of eight
 //         codes leaves as channels 0 4 1 5 2 6 3 7; the queries are stored in the same order, and the result's registers renamed.
-// What bounds it is the products of 64 columns: they take a tensor core as long as ones of 128 (69 cycles for 16 channels, measured), so that a
-// step of 256 rows takes it 1,500 cycles of the 1,860 it lasts; the exponentials take 1,024 of the special-function units'.  Whole tiles of 128
-// keys have cheaper products, but their scores and weights fill the tensor memory: each tile's next scores then wait for its last product
-// and the softmax for both, which came to the same for long prompts (2 x 4,096 tokens, 32 heads over 8 of 128: 328 us, 333 here) and is
-// slower for short ones (8 x 257 behind a window of 1,024: 82 us, 77 here).  One issuer for both tiles of rows: 376.  Taking the tiles apart
-// beforehand, for all blocks of rows at once: 316, but 91 for the short ones.
-// Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of tiles, whose results a second kernel joins in order.
+// What bounds it is the products of 64 columns: they take a tensor core as long as ones of 128 (69 cycles for 16 channels, measured), so
+// that a step of 256 rows takes it 1,500 cycles of the 1,860 it lasts; the exponentials take 1,024 of the special-function units'.
+// Products of whole tiles of 128 keys are cheaper, but their scores and weights fill the tensor memory: each tile's next scores then
+// wait for its last product and the softmax for both, which came to the same for long prompts (2 x 4,096 tokens, 32 heads over 8 of
+// 128: 328 us, 331 here: 830 TFLOP/s), and short ones also step over tiles of which they see half (8 x 257 behind a window of
+// 1,024: 82 us, 70 here).  One issuer for both tiles of rows: 376.  Taking the tiles apart beforehand, for all blocks of rows at once:
+// 316, but 91 for the short ones.  Where rows and heads do not fill the GPU the keys are cut into `n_splits` runs of pages, whose
+// results a second kernel joins in order.
 //
 // Masked keys get the weight 0 exactly.  A value filed as NaN reaches the rows that see its key and no other: in a page that every row
 // of the block sees it is multiplied as it is; in the few others (eleven at most: five on the diagonal, as many at the window's far edge, the

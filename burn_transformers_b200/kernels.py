@@ -2180,7 +2180,7 @@ def _cache4_plan(sms, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, w
         one = wide * (head_dim + 2)
         most = min(max(3 * sms, 3 * units), units * -(-pages // 4))
         return "few", warps, pieces, units * pieces * one if pieces > 1 else 0, most * one
-    # a block a multiprocessor; pieces of eight tiles of 128 keys at least.  Blocks of 128 rows where 256 would leave a quarter of them
+    # a block a multiprocessor; pieces of 1,024 keys at least.  Blocks of 128 rows where 256 would leave a quarter of them
     # idle and the keys are too few to cut (two prompts of 1,024, 12 heads of 64: 23.6 us and 18.0; 8 of 512, 16 heads: 24.6 and 33.1)
     rows = 256
     tiles = -(-columns // rows)
