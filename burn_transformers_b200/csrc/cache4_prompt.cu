@@ -513,8 +513,8 @@ extern "C" int bt_cache4_prompt(const void* q, long long q_row, void* out, const
   BT_CHECK(units <= 65535 && row_tiles <= 65535 && n_splits >= 1 && n_splits <= 65535, "cache4_attention: grid too large (%lld sequences' heads, %d tiles of rows)",
            units, row_tiles);
   const long long parts = units * row_tiles * n_splits * rows;
-  BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
-           "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
+  BT_CHECK(n_splits == 1 || (scratch != nullptr && at16(scratch) && scratch_floats >= parts * (dim + 2)),
+           "cache4_attention: %d splits need %lld floats of scratch on a 16-byte boundary", n_splits, parts * (dim + 2));
   const Cache4PromptParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_tokens, n_heads, group, rows,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};

@@ -2212,11 +2212,11 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     """Causal attention of a step's queries over a layer's 4-bit pages, which hold the step's own keys and values too.
 
     q: rows whose first n_heads * head_dim elements are the query heads (bfloat16 or 32-bit); out: [tokens, n_heads * head_dim] of
-    the same type.  Sequence s brings the tokens seq_start[s] .. seq_start[s + 1] behind past_len[s] others, at most `max_new` of
+    the same type, elsewhere.  Sequence s brings the tokens seq_start[s] .. seq_start[s + 1] behind past_len[s] others, at most `max_new` of
     them, and is no longer than `max_ctx` after the step.  A query at position p sees the keys j <= p with j > p - window (`window`
     0: all) or j < keep_first.  Rows of `out` behind the last sequence stay as they are.  Where the pages come round, what a query
     sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0.  `scratch`: 32-bit, cache4_attention_scratch_floats
-    of the same sizes (more does no harm); two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that
+    of the same sizes (more does no harm), on a 16-byte boundary; two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that
     takes every case.  A page outside the pool is reported by `check_status`, as is a kernel that gave up waiting."""
     code = _element_code(q, "q")
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
@@ -2240,6 +2240,8 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
         if scratch is None:
             raise ShapeError(f"cache4_attention: a step of these sizes needs {floats} floats of scratch")
         partial = _float_list(scratch, "scratch", device, floats)
+        if partial % 16:
+            raise ShapeError("scratch: must start on a 16-byte boundary")
     if _PROFILE is not None:
         _work()
     call = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,

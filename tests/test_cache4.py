@@ -142,6 +142,10 @@ CASES = [
     (attend, dict(impl="fast"), ShapeError, "unknown kernel"),
     (attend, dict(max_new=1, max_ctx=250 * 64, table_len=250, table=ints(3, 250), scratch=None), ShapeError, "floats of scratch"),
     (attend, dict(max_new=1, max_ctx=250 * 64, table_len=250, table=ints(3, 250), scratch=dev(100, dtype=torch.float32)), ShapeError, "scratch"),
+    (attend, dict(max_new=1, max_ctx=250 * 64, table_len=250, table=ints(3, 250), scratch=dev(1 << 20, dtype=torch.float32)[1:]), ShapeError,
+     "16-byte"),
+    (attend, dict(q=dev(40, 256), out=dev(40, 256), n_tokens=40, n_seqs=1, max_new=40, max_ctx=250 * 64, table_len=250, table=ints(3, 250),
+                  scratch=dev(1 << 22, dtype=torch.float32)[3:]), ShapeError, "16-byte"),
 ]
 
 
