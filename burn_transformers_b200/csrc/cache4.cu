@@ -58,32 +58,68 @@ struct C4Row {
   }
 };
 
-// The smallest scale byte with 7 s >= top (finite, not negative); 254 where none has.
+// The smallest scale byte with 7 s >= top (finite, not negative); 254 where none has.  The byte is the bits of top / 7 above the third of
+// its fraction, rounded up.  bfloat16: top has 8 significant bits and 7 s at most 7, so that top is 7 s or more than 2^-9 away from it,
+// and a seventh that is 2^-11 too small takes either to its place.  32-bit: from what may be one too low, by comparing (7 s is exact).
+template <typename T>
 __device__ __forceinline__ int c4_scale_byte(float top) {
-  // the bits of top / 7 above the third of its fraction are the byte, give or take one for the rounding
+  if constexpr (sizeof(T) == 2) {
+    constexpr float kSeventh = (float)((1.0 - 1.0 / 2048.0) / 7.0);
+    return min(max((int)((__float_as_uint(top * kSeventh) + 0xfffffu) >> 20) - 107 * 8, 0), 254);
+  }
   const int near = (int)(__float_as_uint(top * (1.f / 7.f)) >> 20) - 107 * 8 - 1;
   int b = min(max(near, 0), 254);
 #pragma unroll
-  for (int i = 0; i < 3; ++i) b += b < 254 && 7.f * c4_scale((unsigned)b) < top ? 1 : 0;      // (7 s is exact)
+  for (int i = 0; i < 3; ++i) b += b < 254 && 7.f * c4_scale((unsigned)b) < top ? 1 : 0;
   return b;
 }
 
-// round(x / s), ties to even, plus a constant: the bits of a sum that rounds to whole numbers.  `inv`: 1 / s, nearly.
-// bfloat16 x: the corrected quotient is x / s rounded to 24 bits, which is no tie unless x / s is one (x and (k + 1/2) s have 8
-// significant bits each, so that they are equal or differ by more than 2^-9 of x).  32-bit x may lie closer to a tie than a quotient
-// tells: the rest x - r s, which is exact, says on which side.
-constexpr unsigned kC4Whole = 0x4b400000u;       // 1.5 x 2^23
-template <typename T>
+// A sum that rounds to whole numbers, ties to even: the bits of round(x / s) + kC4Whole.
+constexpr float kC4Round = 12582912.f + 8.f;         // 1.5 x 2^23, and the code of 0
+constexpr unsigned kC4Whole = 0x4b400000u;
+
+// 32-bit x may lie closer to a tie than a quotient tells: the rest x - r s, which is exact, says on which side.  `inv`: 1 / s, nearly.
 __device__ __forceinline__ unsigned c4_code(float x, float s, float inv) {
   float r = x * inv;
-  r = fmaf(fmaf(-r, s, x), inv, r);
-  if constexpr (sizeof(T) == 4) {
-    r = rintf(r);
-    const float rest = fmaf(-r, s, x), half = 0.5f * s;
-    const bool odd = (int)fminf(fmaxf(r, -8.f), 8.f) & 1;
-    if (fabsf(rest) > half || (fabsf(rest) == half && odd)) r += rest > 0.f ? 1.f : -1.f;
+  r = rintf(fmaf(fmaf(-r, s, x), inv, r));
+  const float rest = fmaf(-r, s, x), half = 0.5f * s;
+  const bool odd = (int)fminf(fmaxf(r, -8.f), 8.f) & 1;
+  if (fabsf(rest) > half || (fabsf(rest) == half && odd)) r += rest > 0.f ? 1.f : -1.f;
+  return __float_as_uint(r + kC4Round);
+}
+
+// Two bfloat16 x at once.  x / s is a tie or 2^-9 away from one at least (8 significant bits over 4, 7 at most), so that a quotient rounded to
+// whole multiples of 2^-11, by adding 1.5 x 2^12, is as good as the exact one, and 1 / s may be a step off.
+__device__ __forceinline__ void c4_codes2(float x, float y, float inv, unsigned& cx, unsigned& cy) {
+  constexpr float kFine = 6144.f;
+  asm("{\n .reg .b64 v, i, f, c;\n mov.b64 v, {%2, %3};\n mov.b64 i, {%4, %4};\n mov.b64 f, {%5, %5};\n mov.b64 c, {%6, %6};\n"
+      " fma.rn.f32x2 v, v, i, f;\n add.rn.f32x2 v, v, c;\n mov.b64 {%0, %1}, v;\n}\n"
+      : "=r"(cx), "=r"(cy) : "f"(x), "f"(y), "f"(inv), "f"(kFine), "f"(kC4Round - kFine));
+}
+
+// Eight channels' codes, the first lowest, each plus kC4Whole; x is taken into +-7 s first if it is to be `bounded`.
+template <typename T, bool VEC>
+__device__ __forceinline__ unsigned c4_word(const C4Row<T, VEC>& x, float s, bool bounded) {
+  const float most = 7.f * s;
+  unsigned word = 0;
+  if constexpr (sizeof(T) == 2) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+#pragma unroll
+    for (int j = 6; j >= 0; j -= 2) {
+      unsigned a, b;
+      if (bounded)
+        c4_codes2(fminf(fmaxf(x.at(j), -most), most), fminf(fmaxf(x.at(j + 1), -most), most), inv, a, b);
+      else
+        c4_codes2(x.at(j), x.at(j + 1), inv, a, b);
+      word = (word * 16u + b) * 16u + a;
+    }
+  } else {
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int j = 7; j >= 0; --j) word = word * 16u + c4_code(bounded ? fminf(fmaxf(x.at(j), -most), most) : x.at(j), s, inv);
   }
-  return __float_as_uint(r + __uint_as_float(kC4Whole + 8u));
+  return word;
 }
 
 // Where the tokens t0 .. of a block lie: the byte offset of their page in the pool and their place in it, -1 for one that is not there.
@@ -148,17 +184,10 @@ cache4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Cache4Row
       top = max(top, __shfl_xor_sync(quad, top, 1));
       top = max(top, __shfl_xor_sync(quad, top, 2));
       const bool fine = top < 0x7f800000u;
-      const int b = fine ? c4_scale_byte(__uint_as_float(top)) : 255;
-      const float s = c4_scale((unsigned)b), inv = __frcp_rn(s);
-      const float most = b == 254 ? 7.f * s : INFINITY;      // the largest scale: what its seventh multiple does not reach stays at it
-      unsigned word = 0;
-      if (b == 254) {
-#pragma unroll
-        for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(fminf(fmaxf(x[i].at(j), -most), most), s, inv);
-      } else {
-#pragma unroll
-        for (int j = 7; j >= 0; --j) word = word * 16u + c4_code<T>(x[i].at(j), s, inv);
-      }
+      const int b = fine ? c4_scale_byte<T>(__uint_as_float(top)) : 255;
+      const float s = c4_scale((unsigned)b);
+      // the largest scale: what its seventh multiple does not reach stays at it
+      unsigned word = b == 254 ? c4_word(x[i], s, true) : c4_word(x[i], s, false);
       word = fine ? word - 0x11111111u * kC4Whole : 0x88888888u;
       *reinterpret_cast<unsigned*>(codes + s_page[t] + s_row[t] * (dim / 2)) = word;
       if ((at & 3) == 0) scales[s_page[t] + s_row[t] * (dim / 32)] = (unsigned char)b;
