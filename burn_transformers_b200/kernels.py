@@ -2130,28 +2130,29 @@ def _sm_count() -> int:
 def _cache4_few(sms, units, pages, wide, head_dim):
     """(warps a block, pieces of the keys) for `units` blocks' worth of columns over `pages` pages each, at most.
 
-    By a model of what was measured, in us: with n warps on its multiprocessor, in fours, a page keeps a warp 0.75 + 0.2 n (0.5 + 0.11 n with
-    heads of 64 channels); a call costs 4 from end to end, joining pieces 3 more.  Calls that more than fill the GPU go by what a multiprocessor gets
-    done, a page in 0.27 (0.16), and by what a block's beginning and end take of it: 4 by itself, 1.6 beside one other, 1.2 beside two.  More
-    warps a block serve calls that do not fill the GPU without joining anything; pieces serve those with few sequences and heads."""
-    base, step, shared = (0.75, 0.2, 0.27) if head_dim == 128 else (0.5, 0.11, 0.16)
+    By a model of what was measured, in us.  A call costs 4 from end to end, a block 0.45, joining pieces 3.1 and 0.05 a piece.  Among n warps
+    on its multiprocessor a page keeps a warp 0.61 + 0.03 n, and 0.68 for every four of them or part of four.  Calls with more blocks than run
+    at once go by what a multiprocessor gets done, a page in 0.18, by what a block's beginning and end take of it (4.9 by itself, 1.55 beside one
+    other, 0.95 beside two), and by 0.14 of the last block.  Heads of 64 channels take 0.53 of that a page, 16 columns 1.56.  Against
+    every choice timed at 48 sizes, 1 to 128 sequences of 100 to 32,766 tokens, what it chooses is 1.4 % slower than the best on average and 19 % at most
+    (with whole rounds of blocks instead, for calls of up to two: 9 % and 43 %)."""
+    factor = (0.53 if head_dim == 64 else 1.0) * (1.56 if wide == 16 else 1.0)
     most = 12 if wide == 8 else 8
     best = (math.inf, 4, 1)
-    for warps in (4, 6, 8, 12):
+    for warps in (4, 6, 8, 10, 12):
         if warps > most:
             continue
         side = most // warps
         room = sms * side
-        for pieces in {1, 2, 3, room // units, sms // units}:
-            if pieces < 1 or (pieces > 1 and (pieces - 1) * 4 >= pages) or pieces > 1024:
+        for pieces in {1, 2, 3, 4, 6, room // units, sms // units}:
+            if pieces < 1 or (pieces > 1 and ((pieces - 1) * 4 >= pages or units * pieces > room)) or pieces > 1024:
                 continue
             blocks, rounds = units * pieces, -(-(-(-pages // pieces)) // warps)
-            cost = 4.0 + (3.0 if pieces > 1 else 0.0)
-            if blocks <= 2 * room:
-                beside = min(side, -(-blocks // sms)) * warps
-                cost += -(-blocks // room) * rounds * (base + step * 4 * -(-beside // 4))
-            else:
-                cost += units * pages * shared / sms + blocks * (4.0, 1.6, 1.2)[side - 1] / sms + 0.25 * rounds * (base + step * most)
+            beside = min(side, -(-blocks // sms)) * warps
+            one = 0.45 + factor * rounds * (0.61 + 0.03 * beside + 0.68 * -(-beside // 4))
+            cost = 4.0 + one + (3.1 + 0.05 * pieces if pieces > 1 else 0.0)
+            if blocks > room:
+                cost += max(0.0, (factor * units * pages * 0.18 + blocks * (4.9, 1.55, 0.95)[side - 1]) / sms - one) + 0.14 * one
             best = min(best, (cost, warps, pieces))
     return best[1], best[2]
 
@@ -2178,7 +2179,7 @@ def _cache4_plan(sms, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, w
         pages = -(-span // PAGE_SIZE)
         warps, pieces = _cache4_few(sms, units, pages, wide, head_dim)
         one = wide * (head_dim + 2)
-        most = min(max(3 * sms, 3 * units), units * -(-pages // 4))
+        most = min(3 * sms, units * -(-pages // 4))
         return "few", warps, pieces, units * pieces * one if pieces > 1 else 0, most * one
     # a block a multiprocessor; pieces of 1,024 keys at least.  Blocks of 128 rows where 256 would leave a quarter of them
     # idle and the keys are too few to cut (two prompts of 1,024, 12 heads of 64: 23.6 us and 18.0; 8 of 512, 16 heads: 24.6 and 33.1)
