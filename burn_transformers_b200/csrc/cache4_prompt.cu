@@ -449,31 +449,59 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   if (tid == 0 && s_failed && c.status) atomicExch(c.status, 10);
 }
 
-// Joins the runs of keys of a block's rows in their order: a block a row, a thread a channel.
+// Joins the runs of keys of a block's rows: a warp a row, a lane HD / 32 channels; weights of 32 runs at once, values in the runs' order.
+constexpr int C4P_JOIN_WARPS = 8;
 template <int HD>
-__global__ void __launch_bounds__(HD)
+__global__ void __launch_bounds__(32 * C4P_JOIN_WARPS)
 cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, int n_splits) {
+  constexpr int CH = HD / 32;
   pdl_trigger();
   pdl_wait();
-  const int kv_head = (int)blockIdx.y % n_kv_heads, seq = (int)blockIdx.y / n_kv_heads;
-  const int tile = (int)blockIdx.x / p.rows, r = (int)blockIdx.x % p.rows, row0 = (row_tiles - 1 - tile) * p.rows, row = row0 + r;
+  const int kv_head = (int)blockIdx.y % n_kv_heads, seq = (int)blockIdx.y / n_kv_heads, lane = threadIdx.x & 31;
+  const int place = (int)blockIdx.x * C4P_JOIN_WARPS + ((int)threadIdx.x >> 5);
+  const int tile = place / p.rows, r = place % p.rows, row0 = (row_tiles - 1 - tile) * p.rows, row = row0 + r;
   int t0, n_new;
   c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (row >= n_new * p.group) return;
   const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
   const int used = (run.n_pages + run.per - 1) / run.per;
-  float top = -INFINITY, sum = 0.f, o = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const long long unit = (((long long)blockIdx.y * row_tiles + tile) * n_splits + s) * p.rows + r;
-    const float m = p.part[p.part_ml + 2 * unit], l = p.part[p.part_ml + 2 * unit + 1], x = p.part[unit * HD + threadIdx.x];
-    const float m_new = fmaxf(top, m), use = m_new == -INFINITY ? 0.f : m_new;
-    const float a = ta_exp2(top - use), b = ta_exp2(m - use);
-    sum = sum * a + l * b;
-    o = o * a + x * b;
-    top = m_new;
+  const long long unit0 = ((long long)blockIdx.y * row_tiles + tile) * n_splits * p.rows + r;      // run s: p.rows further
+  const float2* ml = reinterpret_cast<const float2*>(p.part + p.part_ml);
+  float top = -INFINITY;
+  for (int s = lane; s < used; s += 32) top = fmaxf(top, ml[unit0 + (long long)s * p.rows].x);
+  top = warp_max(top);
+  const float use = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, o[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) o[i] = 0.f;
+  for (int s0 = 0; s0 < used; s0 += 32) {
+    float weight = 0.f;
+    if (s0 + lane < used) {
+      const float2 mine = ml[unit0 + (long long)(s0 + lane) * p.rows];
+      weight = ta_exp2(mine.x - use);
+      sum += mine.y * weight;
+    }
+    const int count = min(32, used - s0);
+#pragma unroll 4
+    for (int s = 0; s < count; ++s) {
+      const float* part = p.part + (unit0 + (long long)(s0 + s) * p.rows) * HD + lane * CH;
+      const float w = __shfl_sync(0xffffffffu, weight, s);
+      float x[CH];
+      if constexpr (CH == 4)
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part);
+      else
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) o[i] = fmaf(x[i], w, o[i]);
+    }
   }
+  sum = warp_sum(sum);
   const int token = row / p.group, head = kv_head * p.group + row % p.group;
-  p.out[((long long)(t0 + token) * p.n_heads + head) * HD + threadIdx.x] = __float2bfloat16_rn(o / sum);
+  unsigned* dst = reinterpret_cast<unsigned*>(p.out + ((long long)(t0 + token) * p.n_heads + head) * HD + lane * CH);
+  if constexpr (CH == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(ta_pack(o[0] / sum, o[1] / sum), ta_pack(o[2] / sum, o[3] / sum));
+  else
+    *dst = ta_pack(o[0] / sum, o[1] / sum);
 }
 
 template <int HD>
@@ -484,8 +512,8 @@ static int launch_c4p(const Cache4PromptParams& p, const Cache4View& c, int n_se
   BT_CHECK(allow_shared_memory(allowed, kern, smem), "cache4_attention: cannot reserve %zu bytes of shared memory", smem);
   BT_PDL_OK("cache4_prompt", launch_pdl(kern, dim3(n_seqs * c.n_kv_heads, row_tiles, n_splits), dim3(C4P_THREADS), smem, stream, 1, p, c));
   if (n_splits > 1)
-    BT_PDL_OK("cache4_prompt_join", launch_pdl(cache4_prompt_join_kernel<HD>, dim3(row_tiles * p.rows, n_seqs * c.n_kv_heads), dim3(HD), 0, stream,
-                                               1, p, c.n_kv_heads, row_tiles, n_splits));
+    BT_PDL_OK("cache4_prompt_join", launch_pdl(cache4_prompt_join_kernel<HD>, dim3(row_tiles * (p.rows / C4P_JOIN_WARPS), n_seqs * c.n_kv_heads),
+                                               dim3(32 * C4P_JOIN_WARPS), 0, stream, 1, p, c.n_kv_heads, row_tiles, n_splits));
   return 0;
 }
 

@@ -335,3 +335,49 @@ def test_a_window_over_pages_that_come_round():
             q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
             got = attend(step, q, pool, heads, kv, dim, window, 0, 0.1)
             compare(step, got, q, keys, values, heads, kv, dim, window, 0, 0.1)
+
+
+def test_every_bfloat16_as_the_largest_of_a_group():
+    """Each finite magnitude once: its scale is the smallest that reaches it, with ties and near ties of that scale beside it."""
+    bits = np.arange(0x7f80, dtype=np.uint32)
+    top = (bits << 16).view(np.float32).astype(np.float64)
+    s = plain.SCALES[np.minimum(np.searchsorted(7.0 * plain.SCALES, top), 254)]
+    rng = np.random.default_rng(11)
+    x = s[:, None] * (rng.integers(-7, 7, (len(top), 32)) + 0.5) * (1 + rng.integers(-1, 2, (len(top), 32)) * 2.0 ** -7)
+    x = np.clip(x, -top[:, None], top[:, None])
+    x[np.arange(len(top)), rng.integers(0, 32, len(top))] = top * rng.choice([-1, 1], len(top))
+    kv, dim = 2, 128
+    rows = x.reshape(-1, kv, dim)
+    step = Step([0], [len(rows)])
+    for shift in (0, 1):                                 # in 16-byte pieces, and one by one
+        wide = torch.zeros(len(rows), kv * dim + 8, dtype=torch.bfloat16, device=DEV)
+        k = wide.as_strided((len(rows), kv, dim), (kv * dim + 8, dim, 1), shift)
+        k.copy_(torch.tensor(rows).bfloat16())
+        v = torch.flip(k, (0,))
+        pool = torch.zeros(step.pages, kv, kernels.cache4_record_bytes(dim), dtype=torch.uint8, device=DEV)
+        kernels.cache4_append(k, v, pool, step.positions, step.token_seq, step.ctx, step.table, step.width, n_tokens=step.n)
+        got_k, got_v = (torch.empty(len(rows), kv, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        kernels.cache4_gather(pool, step.positions, step.token_seq, step.table, step.width, got_k, got_v, n_tokens=step.n)
+        assert np.array_equal(host(got_k), plain.held(host(k))) and np.array_equal(host(got_v), plain.held(host(v)))
+
+
+@pytest.mark.parametrize("heads, kv, dim, pasts, news", [
+    (4, 4, 64, [1900], [201]), (4, 4, 128, [1900], [201]), (64, 8, 128, [1206, 33], [14, 9]), (3, 1, 128, [4439], [204]),
+    (8, 8, 64, [3500, 0, 700], [40, 17, 1]), (16, 2, 128, [5825, 100, 2000], [31, 30, 1]), (10, 2, 64, [2500], [700]), (32, 4, 128, [4000, 9], [250, 1])])
+@pytest.mark.parametrize("window, keep", [(0, 0), (900, 5)])
+def test_rows_of_both_kinds_in_pieces(heads, kv, dim, pasts, news, window, keep):
+    step, rng = Step(pasts, news), np.random.default_rng(heads + dim + window)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, 0.15)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, 0.15)
+    assert torch.equal(got, attend(step, q, pool, heads, kv, dim, window, keep, 0.15))
+    if kernels._sm_count() == 148:
+        kind, _, pieces, *_ = kernels._cache4_plan(148, len(pasts), max(news), max(step.lens), heads, kv, dim, window, keep, True)
+        assert kind == "many" and (pieces > 1 or window)
+
+
+@pytest.mark.parametrize("heads, kv, dim, pasts, news", [(4, 4, 64, [1500, 300], [90, 2]), (4, 1, 128, [1500, 3000], [40, 64])])
+@pytest.mark.parametrize("window, keep", [(0, 0), (700, 3)])
+def test_values_of_nan_in_pieces(heads, kv, dim, pasts, news, window, keep):
+    test_a_key_or_value_of_nan_reaches_the_queries_that_see_it_and_no_other(torch.bfloat16, heads, kv, dim, pasts, news, window, keep)
