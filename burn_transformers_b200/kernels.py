@@ -1978,10 +1978,12 @@ def _float_list(t, name, device, count) -> int:
 
 def _row_stride(t, name, device, dtype, count, width, written=False) -> int:
     """Elements between the rows of `t`: at least `count` rows of at least `width` contiguous elements (apart, if they are written)."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.size(0) >= count
-            and t.size(1) >= width and (t.stride(1) == 1 or width == 1) and (not written or count < 2 or t.stride(0) >= width)):
-        _fault(t, name, device, dtype, f"at least {count} rows of at least {width} elements", "contiguous within a row, rows apart")
-    return t.stride(0)
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device:
+        shape, stride = t.shape, t.stride()
+        if (len(shape) == 2 and shape[0] >= count and shape[1] >= width and (stride[1] == 1 or width == 1)
+                and (not written or count < 2 or stride[0] >= width)):
+            return stride[0]
+    _fault(t, name, device, dtype, f"at least {count} rows of at least {width} elements", "contiguous within a row, rows apart")
 
 
 def _element_code(t, name) -> int:
@@ -2049,25 +2051,31 @@ def cache4_record_bytes(head_dim: int) -> int:
     return 68 * head_dim
 
 
-def _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs) -> None:
+def _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs):
+    """The pool's pages, and how many the table has room for: sequences, pages of a sequence."""
     if head_dim <= 0 or head_dim > 256 or head_dim % 32:
         cache4_record_bytes(head_dim)
-    if not (isinstance(pool, torch.Tensor) and pool.dtype is torch.uint8 and pool.get_device() == device and pool.dim() == 3
-            and pool.shape[0] >= 1 and pool.shape[1] == n_kv_heads and pool.shape[2] == 68 * head_dim and pool.is_contiguous()):
+    shape = pool.shape if isinstance(pool, torch.Tensor) else ()
+    if not (len(shape) == 3 and pool.dtype is torch.uint8 and pool.get_device() == device and shape[0] >= 1 and shape[1] == n_kv_heads
+            and shape[2] == 68 * head_dim and pool.is_contiguous()):
         _fault(pool, "pool", device, torch.uint8, f"[pages, {n_kv_heads}, {68 * head_dim}]")
-    if not (isinstance(table, torch.Tensor) and table.dtype is torch.int32 and table.get_device() == device and table.dim() == 2
-            and table.shape[0] >= n_seqs and table.shape[1] >= table_len >= 1 and table.is_contiguous()):
-        if isinstance(table, torch.Tensor) and table.dim() == 2 and not 1 <= table_len <= table.shape[1]:
-            raise ShapeError(f"table: rows of {table.shape[1]} pages hold no list of {table_len}")
+    lists = table.shape if isinstance(table, torch.Tensor) else ()
+    if not (len(lists) == 2 and table.dtype is torch.int32 and table.get_device() == device and lists[0] >= n_seqs and lists[1] >= table_len >= 1
+            and table.is_contiguous()):
+        if len(lists) == 2 and not 1 <= table_len <= lists[1]:
+            raise ShapeError(f"table: rows of {lists[1]} pages hold no list of {table_len}")
         _fault(table, "table", device, torch.int32, f"[at least {n_seqs} sequences, at least {table_len} pages]")
+    return shape[0], lists[0], lists[1]
 
 
-def _cache4_heads(t, name, device, dtype, count, heads, dim, written=False) -> None:
-    """`t` as [tokens, key heads, channels] with contiguous channels."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.dim() == 3 and t.shape[0] >= count
-            and t.shape[1] == heads and t.shape[2] == dim and t.stride(2) == 1
-            and not (written and ((count > 1 and t.stride(0) == 0) or (heads > 1 and t.stride(1) == 0)))):
-        _fault(t, name, device, dtype, f"[at least {count} tokens, {heads} key heads, {dim} channels]", "contiguous channels")
+def _cache4_heads(t, name, device, dtype, count, heads, dim, written=False):
+    """The strides of `t`, [tokens, key heads, channels] with contiguous channels."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device:
+        shape, stride = t.shape, t.stride()
+        if (len(shape) == 3 and shape[0] >= count and shape[1] == heads and shape[2] == dim and stride[2] == 1
+                and not (written and ((count > 1 and stride[0] == 0) or (heads > 1 and stride[1] == 0)))):
+            return stride
+    _fault(t, name, device, dtype, f"[at least {count} tokens, {heads} key heads, {dim} channels]", "contiguous channels")
 
 
 def cache4_append(k, v, pool, positions, token_seq, ctx_len, table, table_len, *, n_tokens):
@@ -2081,19 +2089,20 @@ def cache4_append(k, v, pool, positions, token_seq, ctx_len, table, table_len, *
     A token whose sequence, position or page lies outside the table or the pool is not filed; `check_status` reports it."""
     code = _element_code(k, "k")
     device = torch.cuda.current_device()
-    if n_tokens < 0 or k.dim() != 3:
-        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(k.shape)}")
-    heads, dim = k.shape[1], k.shape[2]
-    _cache4_pages(pool, table, table_len, device, heads, dim, 0)
-    _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim)
-    _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim)
+    shape = k.shape
+    if n_tokens < 0 or len(shape) != 3:
+        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(shape)}")
+    heads, dim = shape[1], shape[2]
+    pages, n_lists, width = _cache4_pages(pool, table, table_len, device, heads, dim, 0)
+    k_step = _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim)
+    v_step = _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim)
     at, seq = _int_list(positions, "positions", device, n_tokens), _int_list(token_seq, "token_seq", device, n_tokens)
     length = _int_list(ctx_len, "ctx_len", device, 0)
     if _PROFILE is not None:
         _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
     _check(library().bt_cache4_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), pool.data_ptr(), pool.shape[0], at, seq, length,
-        table.data_ptr(), min(table.shape[0], ctx_len.shape[0]), table.shape[1], table_len, _status_address(device), n_tokens, heads, dim,
+        k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq, length,
+        table.data_ptr(), min(n_lists, ctx_len.shape[0]), width, table_len, _status_address(device), n_tokens, heads, dim,
         code, _raw_stream(device)))
 
 
@@ -2103,28 +2112,30 @@ def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_token
     or the pool yields NaN, and `check_status` reports it."""
     code = _element_code(k, "k")
     device = torch.cuda.current_device()
-    if n_tokens < 0 or k.dim() != 3:
-        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(k.shape)}")
-    heads, dim = k.shape[1], k.shape[2]
-    _cache4_pages(pool, table, table_len, device, heads, dim, 0)
-    _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim, True)
-    _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim, True)
+    shape = k.shape
+    if n_tokens < 0 or len(shape) != 3:
+        raise ShapeError(f"k: expected [tokens, key heads, channels] for {n_tokens} tokens, found shape {list(shape)}")
+    heads, dim = shape[1], shape[2]
+    pages, n_lists, width = _cache4_pages(pool, table, table_len, device, heads, dim, 0)
+    k_step = _cache4_heads(k, "k", device, k.dtype, n_tokens, heads, dim, True)
+    v_step = _cache4_heads(v, "v", device, k.dtype, n_tokens, heads, dim, True)
     at, seq = _int_list(positions, "positions", device, n_tokens), _int_list(token_seq, "token_seq", device, n_tokens)
     if _PROFILE is not None:
         _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
     _check(library().bt_cache4_gather(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), pool.data_ptr(), pool.shape[0], at, seq,
-        table.data_ptr(), table.shape[0], table.shape[1], table_len, _status_address(device), n_tokens, heads, dim, code, _raw_stream(device)))
+        k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq,
+        table.data_ptr(), n_lists, width, table_len, _status_address(device), n_tokens, heads, dim, code, _raw_stream(device)))
 
 
 _SM_COUNTS: dict = {}
 
 
-def _sm_count() -> int:
-    device = torch.cuda.current_device()
-    if device not in _SM_COUNTS:
-        _SM_COUNTS[device] = torch.cuda.get_device_properties(device).multi_processor_count
-    return _SM_COUNTS[device]
+def _sm_count(device: int | None = None) -> int:
+    device = torch.cuda.current_device() if device is None else device
+    hit = _SM_COUNTS.get(device)
+    if hit is None:
+        hit = _SM_COUNTS[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return hit
 
 
 def _cache4_few(sms, units, pages, wide, head_dim):
@@ -2216,7 +2227,7 @@ def _cache4_plan(sms, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, w
 def _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first) -> None:
     if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise ShapeError(f"cache4_attention: {n_heads} query heads cannot share {n_kv_heads} key heads")
-    if min(n_tokens, n_seqs, max_new, max_ctx, window, keep_first) < 0:
+    if n_tokens < 0 or n_seqs < 0 or max_new < 0 or max_ctx < 0 or window < 0 or keep_first < 0:
         raise ShapeError(f"cache4_attention: {n_tokens} tokens of {n_seqs} sequences, {max_new} new at most, context {max_ctx}, window {window}, "
                          f"kept positions {keep_first}: none may be negative")
 
@@ -2243,10 +2254,11 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
     device = torch.cuda.current_device()
     width = n_heads * head_dim
-    _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs)
+    pages, _, list_width = _cache4_pages(pool, table, table_len, device, n_kv_heads, head_dim, n_seqs)
     row = _row_stride(q, "q", device, q.dtype, n_tokens, width)
-    if not (isinstance(out, torch.Tensor) and out.dtype is q.dtype and out.get_device() == device and out.dim() == 2 and out.shape[1] == width
-            and out.shape[0] >= n_tokens and out.is_contiguous()):
+    shape = out.shape if isinstance(out, torch.Tensor) else ()
+    if not (len(shape) == 2 and shape[1] == width and shape[0] >= n_tokens and out.dtype is q.dtype and out.get_device() == device
+            and out.is_contiguous()):
         _fault(out, "out", device, q.dtype, f"[at least {n_tokens}, {width}]")
     starts, pasts = _int_list(seq_start, "seq_start", device, n_seqs + 1), _int_list(past_len, "past_len", device, n_seqs)
     if max_ctx > table_len * PAGE_SIZE and (keep_first or not window or table_len * PAGE_SIZE < window + max_new - 1):
@@ -2254,8 +2266,9 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
                          f"(window {window}, kept positions {keep_first}, {max_new} new tokens)")
     if impl not in (None, "any"):
         raise ShapeError(f"cache4_attention: unknown kernel {impl!r}")
-    fast = impl is None and code == 1 and (q.data_ptr() | out.data_ptr() | pool.data_ptr()) % 16 == 0 and row % 8 == 0
-    kind, wide, pieces, floats, _ = _cache4_plan(_sm_count(), n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)
+    q_at, out_at, pool_at = q.data_ptr(), out.data_ptr(), pool.data_ptr()
+    fast = impl is None and code == 1 and (q_at | out_at | pool_at) % 16 == 0 and row % 8 == 0
+    kind, wide, pieces, floats, _ = _cache4_plan(_sm_count(device), n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, window, keep_first, fast)
     partial = 0
     if floats:
         if scratch is None:
@@ -2265,7 +2278,7 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
             raise ShapeError("scratch: must start on a 16-byte boundary")
     if _PROFILE is not None:
         _work()
-    call = (q.data_ptr(), row, out.data_ptr(), pool.data_ptr(), pool.shape[0], table.data_ptr(), table.shape[1], table_len,
+    call = (q_at, row, out_at, pool_at, pages, table.data_ptr(), list_width, table_len,
             _status_address(device), starts, pasts, n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, min(window, _INT_MAX),
             min(keep_first, _INT_MAX), pieces, wide, partial, floats)
     if kind == "few":

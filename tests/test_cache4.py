@@ -41,7 +41,7 @@ def no_device(monkeypatch):
         raise Reached
     monkeypatch.setattr(kernels, "library", reached)
     monkeypatch.setattr(kernels.torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(kernels, "_sm_count", lambda: 148)
+    monkeypatch.setattr(kernels, "_sm_count", lambda device=None: 148)
     monkeypatch.setattr(kernels, "_status_address", lambda device: 0)
     monkeypatch.setattr(kernels, "_raw_stream", lambda device: 0)
 
