@@ -94,7 +94,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   __shared__ unsigned s_nan[C4P_EDGES][CH][2];      // a bit a key of a page that not every row sees
   __shared__ int s_edge_key[C4P_EDGES], s_edges;
   __shared__ unsigned s_tmem;
-  __shared__ int s_failed;
+  __shared__ int failed;
   unsigned char *Qs = c4p_raw, *Ks = Qs + 2 * TILE, *Vs = Ks + 2 * TILE;
   unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // [stage]
   unsigned long long *s_full = bars + 8, *p_ready = bars + 12, *o_done = bars + 16;      // [tile of rows][step parity]
@@ -130,7 +130,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       ta_bar_init(&p_ready[s], 4);
       ta_bar_init(&o_done[s], 1);
     }
-    s_failed = 0;
+    failed = 0;
     s_edges = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -259,7 +259,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
       if (ok) ok = __all_sync(0xffffffffu, ta_bar_wait(&o_done[2 * sub + ((n_steps - 1) & 1)], ((n_steps - 1) >> 1) & 1));
       ta_fence_after();
       if (!ok) {
-        s_failed = 1;
+        failed = 1;
       } else {
         // channels whose values are NaN for a key that this row sees, but were multiplied as 0
         unsigned lost = 0;
@@ -382,7 +382,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
         c4p_bar_arrive_warp(&full[s], lane);
         if (it + 1 < n_tiles) fetch(it + 1);
       }
-      if (!ok) s_failed = 1;
+      if (!ok) failed = 1;
     }
     if (warp == ISSUER || (warp == ISSUER + 1 && n_sub > 1)) {
       // ---- issuers, one a tile of rows.  Instruction descriptors: 32-bit accumulator, bfloat16 operands, M = 128; S: N = 64, both K-major;
@@ -436,17 +436,17 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
           scores(j + 2);
         }
       }
-      if (!ok && lane == 0) s_failed = 1;
+      if (!ok && lane == 0) failed = 1;
     }
   }
   ta_fence_before();
   __syncthreads();
-  if (s_failed) let_copies_land();
+  if (failed) let_copies_land();
   if (warp == ISSUER) {
     ta_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
   }
-  if (tid == 0 && s_failed && c.status) atomicExch(c.status, 10);
+  if (tid == 0 && failed && c.status) atomicExch(c.status, 10);
 }
 
 // Joins the runs of keys of a block's rows: a warp a row, a lane HD / 32 channels; weights of 32 runs at once, values in the runs' order.
