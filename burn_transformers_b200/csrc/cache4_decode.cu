@@ -14,9 +14,10 @@
 //
 // What bounds it: a page takes a warp a chain of dependent steps (1.45 us by itself, 3.2 beside eleven others, 0.27 a page and
 // multiprocessor), and 168 registers allow 12 warps; the integer pipe, which takes the codes apart (7 operations for a word of eight), is
-// active 64 % of the time, memory 61 % (64 sequences of 1,000 to 8,000 tokens, 32 heads over 8 of 128: 77 us, 4.1 TB/s).  Half precision,
-// which needs 5 operations for a word, came to the same.  A block has 4 to 12 warps and the run is cut into `n_splits` pieces as the caller's
-// model of their cost says (kernels.py); the pieces' results (maximum, sum, weighted values) are joined in order by a second kernel.
+// active 53 to 64 % of the time, memory 61 % (64 sequences of 1,000 to 8,000 tokens, 32 heads over 8 of 128: 78 us, 4.0 TB/s).  Half precision,
+// which needs 5 operations for a word, came to the same; 16 warps of 128 registers, fed in half pages so that their rings fit, to 86; the
+// longest sequences first to 81 where they came first anyway.  A block has 4 to 12 warps and the run is cut into `n_splits` pieces as the
+// caller's model of their cost says (kernels.py); the pieces' results (maximum, sum, weighted values) are joined in order by a second kernel.
 // Keys that a column does not see get the weight 0 exactly, and what lies in a page past the sequence's end (any bytes) is never
 // multiplied; a value filed as NaN reaches the columns that see its key and no other.
 #include "cache4.cuh"

@@ -9,6 +9,8 @@
 // and sines once, in shared memory, and a lane keeps what its eight pairs are multiplied by in registers; it holds 16 channels of a head
 // (the two pieces of 8 that turn into one another, or 16 in a row), so that nothing but the norm's sum goes between lanes.  How many
 // heads a warp takes: all of them when there are enough tokens to fill the GPU, as few as fit its lanes when there are not.
+// 16,384 tokens of 32 + 8 heads of 128 channels, bfloat16: 63 us, 5.3 TB/s (with factors formed for every head and single
+// multiply-adds: 94); 8 tokens: 2.3.
 #include "common.cuh"
 
 namespace bt {
