@@ -288,6 +288,13 @@ int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool
 int bt_qk_norm_rotary(const void* src, long long src_row, void* dst, long long dst_row, const int* positions, const float* freq,
                       const float* q_weight, const float* k_weight, int n_tokens, int n_heads, int n_kv_heads, int dim, int rot, float eps,
                       float size, int interleaved, int dtype, cudaStream_t stream);
+// The same with their arguments in one record, in order and without gaps (packed_calls.cu).
+int bt_qk_norm_rotary_packed(const void* record, int bytes);
+int bt_cache4_append_packed(const void* record, int bytes);
+int bt_cache4_gather_packed(const void* record, int bytes);
+int bt_cache4_attention_packed(const void* record, int bytes);
+int bt_cache4_decode_packed(const void* record, int bytes);
+int bt_cache4_prompt_packed(const void* record, int bytes);
 int bt_add_vector(float* x, const float* vec, long long n_rows, int width, cudaStream_t stream);
 int bt_add_rows(float* x, const float* a, const float* b, const float* c, long long n, cudaStream_t stream);
 

@@ -9,7 +9,8 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -1930,22 +1931,29 @@ def gla_scan(proj, q_off, k_off, v_off, q_scale: float, dt, log_scale: float, st
 
 # ---- queries and keys normed and turned; a cache held in 4 bits -------------------------------
 # A decode step makes these calls once a layer and kernels of a few microseconds wait for them: their checks are single expressions
-# that name a fault only once they have found one, and the library's functions take plain integers (`_ARGUMENTS`).
+# that name a fault only once they have found one, and the library takes the arguments as one record (csrc/packed_calls.cu).
 
-_ARGUMENTS = {
-    "bt_qk_norm_rotary": "plplppppiiiiiffiip",
-    "bt_cache4_append": "pllpllplppppiiipiiiip",
-    "bt_cache4_gather": "pllpllplpppiiipiiiip",
-    "bt_cache4_attention": "plpplpiipppiiiiiifiiiiplip",
-    "bt_cache4_decode": "plpplpiipppiiiiiifiiiiplp",
-    "bt_cache4_prompt": "plpplpiipppiiiiiifiiiiplp",
-}
+_RECORDS = {name: struct.Struct("=" + letters) for name, letters in {
+    "bt_qk_norm_rotary_packed": "QqQqQQQQiiiiiffiiQ",
+    "bt_cache4_append_packed": "QqqQqqQqQQQQiiiQiiiiQ",
+    "bt_cache4_gather_packed": "QqqQqqQqQQQiiiQiiiiQ",
+    "bt_cache4_attention_packed": "QqQQqQiiQQQiiiiiifiiiiQqiQ",
+    "bt_cache4_decode_packed": "QqQQqQiiQQQiiiiiifiiiiQqQ",
+    "bt_cache4_prompt_packed": "QqQQqQiiQQQiiiiiifiiiiQqQ",
+}.items()}
 
 
 def _declare(lib) -> None:
-    kinds = {"p": c_void_p, "l": c_longlong, "i": c_int, "f": c_float}
-    for name, letters in _ARGUMENTS.items():
-        getattr(lib, name).argtypes = [kinds[c] for c in letters]
+    for name in _RECORDS:
+        getattr(lib, name).argtypes = [c_char_p, c_int]
+
+
+def _call_packed(name: str, *args) -> None:
+    try:
+        record = _RECORDS[name].pack(*args)
+    except (struct.error, OverflowError) as error:
+        raise ShapeError(f"{name}: an argument does not fit its 32 or 64 bits: {error}") from None
+    _check(getattr(library(), name)(record, len(record)))
 
 
 def _fault(t, name, device, dtype, shape, note="contiguous") -> None:
@@ -2040,8 +2048,8 @@ def qk_norm_rotary(proj, positions, inv_freq, *, n_tokens, n_heads, n_kv_heads, 
         qw, kw = _float_list(q_weight, "q_weight", device, head_dim), _float_list(k_weight, "k_weight", device, head_dim)
     if _PROFILE is not None:
         _work(10.0 * n_tokens * width, 2.0 * n_tokens * width * proj.element_size())
-    _check(library().bt_qk_norm_rotary(proj.data_ptr(), row, to.data_ptr(), to_row, at, freq, qw, kw, n_tokens, n_heads, n_kv_heads, head_dim,
-                                       rot_dims, eps, size, 1 if interleaved else 0, code, _raw_stream(device)))
+    _call_packed("bt_qk_norm_rotary_packed", proj.data_ptr(), row, to.data_ptr(), to_row, at, freq, qw, kw, n_tokens, n_heads, n_kv_heads, head_dim,
+                 rot_dims, eps, size, 1 if interleaved else 0, code, _raw_stream(device))
 
 
 def cache4_record_bytes(head_dim: int) -> int:
@@ -2100,10 +2108,10 @@ def cache4_append(k, v, pool, positions, token_seq, ctx_len, table, table_len, *
     length = _int_list(ctx_len, "ctx_len", device, 0)
     if _PROFILE is not None:
         _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
-    _check(library().bt_cache4_append(
-        k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq, length,
+    _call_packed(
+        "bt_cache4_append_packed", k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq, length,
         table.data_ptr(), min(n_lists, ctx_len.shape[0]), width, table_len, _status_address(device), n_tokens, heads, dim,
-        code, _raw_stream(device)))
+        code, _raw_stream(device))
 
 
 def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_tokens):
@@ -2122,9 +2130,9 @@ def cache4_gather(pool, positions, token_seq, table, table_len, k, v, *, n_token
     at, seq = _int_list(positions, "positions", device, n_tokens), _int_list(token_seq, "token_seq", device, n_tokens)
     if _PROFILE is not None:
         _work(0.0, 2 * n_tokens * heads * dim * (k.element_size() + 17 / 32))
-    _check(library().bt_cache4_gather(
-        k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq,
-        table.data_ptr(), n_lists, width, table_len, _status_address(device), n_tokens, heads, dim, code, _raw_stream(device)))
+    _call_packed(
+        "bt_cache4_gather_packed", k.data_ptr(), k_step[0], k_step[1], v.data_ptr(), v_step[0], v_step[1], pool.data_ptr(), pages, at, seq,
+        table.data_ptr(), n_lists, width, table_len, _status_address(device), n_tokens, heads, dim, code, _raw_stream(device))
 
 
 _SM_COUNTS: dict = {}
@@ -2282,8 +2290,8 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
             _status_address(device), starts, pasts, n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, min(window, _INT_MAX),
             min(keep_first, _INT_MAX), pieces, wide, partial, floats)
     if kind == "few":
-        _check(library().bt_cache4_decode(*call, _raw_stream(device)))
+        _call_packed("bt_cache4_decode_packed", *call, _raw_stream(device))
     elif kind == "many":
-        _check(library().bt_cache4_prompt(*call, _raw_stream(device)))
+        _call_packed("bt_cache4_prompt_packed", *call, _raw_stream(device))
     else:
-        _check(library().bt_cache4_attention(*call, code, _raw_stream(device)))
+        _call_packed("bt_cache4_attention_packed", *call, code, _raw_stream(device))

@@ -1,5 +1,8 @@
 """What the calls of the 4-bit cache and of the norm with rotation refuse, and how a step is cut into pieces: no device is needed (a
 tensor that says it lies on one, and a library that must not be reached)."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -176,3 +179,18 @@ def test_the_scratch_that_is_asked_for_covers_every_smaller_step(heads, kv, dim,
                  for fewer in {1, 2, 3, 5, 17, 64, 300} if fewer <= seqs for shorter in {new, new + 63, new + 200, new + 1000, new + 9_000, ctx}
                  if shorter <= ctx for fast in (True, False)]
         assert max(needs) <= asked[seqs, ctx], (seqs, ctx)
+
+
+def test_records_are_laid_out_as_the_library_reads_them():
+    api = (Path(kernels.__file__).parent / "csrc" / "api.h").read_text()
+    letters = {"long long": "q", "int": "i", "float": "f", "cudaStream_t": "Q"}
+    for name, record in kernels._RECORDS.items():
+        parameters = re.search(rf"int {name.removesuffix('_packed')}\(([^)]*)\);", api).group(1).split(",")
+        kinds = ["Q" if "*" in p else letters[p.rsplit(" ", 1)[0].strip()] for p in parameters]
+        assert record.format == "=" + "".join(kinds), name
+
+
+@pytest.mark.parametrize("call, change", [(rotary, dict(eps=1e300)), (rotary, dict(size=-1e39)), (attend, dict(scale=1e300))])
+def test_arguments_that_fit_no_record(call, change):
+    with pytest.raises(ShapeError, match="does not fit"):
+        call(**change)
