@@ -14,10 +14,10 @@
 //
 // What bounds it: a page takes a warp a chain of dependent steps (1.45 us by itself, 3.2 beside eleven others, 0.27 a page and
 // multiprocessor), and 168 registers allow 12 warps; the integer pipe, which takes the codes apart (7 operations for a word of eight), is
-// active 53 to 64 % of the time, memory 61 % (64 sequences of 1,000 to 8,000 tokens, 32 heads over 8 of 128: 78 us, 4.0 TB/s).  Half precision,
-// which needs 5 operations for a word, came to the same; 16 warps of 128 registers, fed in half pages so that their rings fit, to 86; the
-// longest sequences first to 81 where they came first anyway.  A block has 4 to 12 warps and the run is cut into `n_splits` pieces as the
-// caller's model of their cost says (kernels.py); the pieces' results (maximum, sum, weighted values) are joined in order by a second kernel.
+// active 53 to 64 % of the time, memory 60 % (64 sequences of 1,000 to 8,000 tokens, 32 heads over 8 of 128: 81 us, 3.9 TB/s).  Half precision,
+// which needs 5 operations for a word, came to the same; 16 warps of 128 registers, fed in half pages so that their rings fit, to 7 us more.
+// A block has 4 to 12 warps and the run is cut into `n_splits` pieces as the caller's model of their cost says (kernels.py); the
+// pieces' results (maximum, sum, weighted values) are joined in order by a second kernel.
 // Keys that a column does not see get the weight 0 exactly, and what lies in a page past the sequence's end (any bytes) is never
 // multiplied; a value filed as NaN reaches the columns that see its key and no other.
 #include "cache4.cuh"
@@ -35,6 +35,7 @@ struct Cache4DecodeParams {
   __nv_bfloat16* out;
   const int *seq_start, *past_len;
   int n_tokens, n_heads, group, col_blocks, max_new, slots;
+  int sorted;                  // the longest sequences go first
   float scale_log2;
   int window, keep_first;
   float* part;                 // [unit][split][columns][HD], then [unit][split][columns][2]
@@ -54,6 +55,51 @@ __device__ __forceinline__ float c4d_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// A block's sequence: the rank-th, or the one with the rank-th longest run of keys, where blocks wait for others to end: a long sequence
+// that is begun late is waited for.  64 sequences of 1,000 to 8,000 tokens in any order: 81 us; in their own order 79 where the longest happen to
+// come first, 97 where they come last, 110 to 115 where they are mixed (128 of 500 to 2,000: 60; 56, 60, 64).  Every thread takes some
+// sequences and counts those that go before; what the block needs of its own is asked for meanwhile.
+constexpr int C4D_SORTED = 128;           // sequences that are sorted, at most
+struct C4dSequence {
+  int seq, past, t0, n_new;
+};
+__device__ __forceinline__ C4dSequence c4d_sequence(const Cache4DecodeParams& p, int n_seqs, int rank) {
+  C4dSequence at;
+  if (!p.sorted) {
+    at.seq = rank;
+    at.past = p.past_len[rank];
+    c4_new_tokens(p.seq_start, rank, p.n_tokens, at.t0, at.n_new);
+    return at;
+  }
+  __shared__ __align__(16) int s_key[C4D_SORTED];      // no two alike
+  __shared__ C4dSequence s_at;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  for (int i = tid; i < C4D_SORTED; i += threads) {
+    int past = i < n_seqs ? max(p.past_len[i], 0) : 0;
+    if (p.window > 0) past = min(past, p.window);
+    s_key[i] = i < n_seqs ? min(past, (1 << 23) - 1) * C4D_SORTED + (C4D_SORTED - i) : 0;
+  }
+  __syncthreads();
+  for (int i = tid; i < n_seqs; i += threads) {
+    at.seq = i;
+    at.past = p.past_len[i];
+    c4_new_tokens(p.seq_start, i, p.n_tokens, at.t0, at.n_new);
+    const int mine = s_key[i];
+    int before[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int j = 0; j < n_seqs; j += 4) {
+      const int4 other = *reinterpret_cast<const int4*>(&s_key[j]);
+      before[0] += other.x > mine;
+      before[1] += other.y > mine;
+      before[2] += other.z > mine;
+      before[3] += other.w > mine;
+    }
+    if (before[0] + before[1] + before[2] + before[3] == rank) s_at = at;
+  }
+  __syncthreads();
+  return s_at;
+}
+
 template <bool V>
 struct C4dFlag {
   static constexpr bool value = V;
@@ -75,13 +121,12 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int n_warps = (int)blockDim.x >> 5;
-  const int split = blockIdx.x, n_splits = gridDim.x, seq = blockIdx.z;
+  const int split = blockIdx.x, n_splits = gridDim.x;
   const int kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS;
-  int t0, n_new;
-  c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
+  const C4dSequence at_seq = c4d_sequence(p, gridDim.z, blockIdx.z);
+  const int seq = at_seq.seq, past = at_seq.past, t0 = at_seq.t0, n_new = at_seq.n_new;
   const int n_cols = n_new * p.group - col0;
   if (n_cols <= 0) return;
-  const int past = p.past_len[seq];
   const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
   // the pages that any column sees: kept ones before the window's, then the window's
   const int lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
@@ -493,6 +538,8 @@ static int launch_c4d(Cache4DecodeParams p, const Cache4View& c, int n_seqs, int
   const int sms = sm_count() > 0 ? sm_count() : 148;
   int side = (int)(blocks <= sms ? 1 : blocks <= 2ll * sms ? 2 : 3);
   if (side > MOST / n_warps) side = MOST / n_warps;
+  // blocks that wait for others to end
+  p.sorted = blocks > (long long)side * sms && n_seqs > 1 && n_seqs <= C4D_SORTED;
   p.slots = (WHOLE / side - 2048) / (n_warps * c4_record(HD));
   if (p.slots > C4D_MOST_SLOTS) p.slots = C4D_MOST_SLOTS;
   const size_t smem = (size_t)n_warps * p.slots * c4_record(HD);
@@ -536,7 +583,7 @@ extern "C" int bt_cache4_decode(const void* q, long long q_row, void* out, const
   const long long parts = (long long)n_seqs * n_kv_heads * blocks * n_splits * 8 * nt;
   BT_CHECK(n_splits == 1 || (scratch != nullptr && scratch_floats >= parts * (dim + 2)),
            "cache4_attention: %d splits need %lld floats of scratch", n_splits, parts * (dim + 2));
-  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_tokens, n_heads, group, blocks, max_new, 0,
+  const Cache4DecodeParams p{(const __nv_bfloat16*)q, q_row, (__nv_bfloat16*)out, seq_start, past_len, n_tokens, n_heads, group, blocks, max_new, 0, 0,
                              scale * 1.4426950408889634f, window, keep_first, scratch, parts * dim};
   const Cache4View c{(unsigned char*)pool, n_pages, table, table_stride, table_len, n_kv_heads, status};
   if (dim == 64) return nt == 1 ? launch_c4d<64, 1>(p, c, n_seqs, n_splits, n_warps, stream) : launch_c4d<64, 2>(p, c, n_seqs, n_splits, n_warps, stream);

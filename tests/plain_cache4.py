@@ -8,7 +8,7 @@ SCALES = np.array([(8 + b % 8) * 2.0 ** (b // 8 - 23) for b in range(255)])
 def held(x):
     """What rows of numbers are held as: [..., dim], dim a multiple of 32."""
     x = np.asarray(x, dtype=np.float64)
-    g = x.reshape(*x.shape[:-1], -1, GROUP)
+    g = x.reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP)
     bad = ~np.isfinite(g).all(-1)
     top = np.where(bad, 0.0, np.abs(np.where(np.isfinite(g), g, 0.0)).max(-1))
     s = SCALES[np.minimum(np.searchsorted(7.0 * SCALES, top), 254)][..., None]

@@ -381,3 +381,24 @@ def test_rows_of_both_kinds_in_pieces(heads, kv, dim, pasts, news, window, keep)
 @pytest.mark.parametrize("window, keep", [(0, 0), (700, 3)])
 def test_values_of_nan_in_pieces(heads, kv, dim, pasts, news, window, keep):
     test_a_key_or_value_of_nan_reaches_the_queries_that_see_it_and_no_other(torch.bfloat16, heads, kv, dim, pasts, news, window, keep)
+
+
+@pytest.mark.parametrize("seqs, new", [(50, 1), (112, 2), (128, 1), (131, 1)])
+@pytest.mark.parametrize("heads, kv, dim", [(8, 8, 64), (16, 4, 128)])
+@pytest.mark.parametrize("window, keep", [(0, 0), (100, 3)])
+def test_more_sequences_than_run_at_once(seqs, new, heads, kv, dim, window, keep):
+    """Lengths in any order, many of them alike, sequences without tokens among them: the blocks are not begun in their order."""
+    rng = np.random.default_rng(seqs + dim)
+    pasts = [int(p) for p in rng.choice([0, 5, 63, 64, 200, 200, 391], seqs)]
+    news = [int(n) for n in rng.integers(0, new + 1, seqs)]
+    news[3] = new
+    step = Step(pasts, news)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, 0.2)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, 0.2)
+    # the same sequences the other way round: every one's result to the bit
+    back = Step(pasts[::-1], news[::-1])
+    order = torch.cat([torch.arange(step.starts[s], step.starts[s + 1]) for s in reversed(range(seqs))]).to(DEV)
+    back.table = torch.flip(step.table, (0,)).contiguous()
+    assert torch.equal(attend(back, q[order], pool, heads, kv, dim, window, keep, 0.2), got[order])
