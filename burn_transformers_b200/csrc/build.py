@@ -98,7 +98,7 @@ def build(verbose: bool = True) -> Path:
     def compile_one(src: Path):
         # per-file stamps keep unchanged objects
         obj = out_dir / (src.stem + ".o")
-        own = hashlib.sha256(src.read_bytes() + b"".join(p.read_bytes() for p in sorted(CSRC.glob("*.cuh")))
+        own = hashlib.sha256(src.read_bytes() + b"".join(p.read_bytes() for p in sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")))
                              + " ".join(NVCC_FLAGS).encode()).hexdigest()
         own_file = out_dir / (src.stem + ".stamp")
         if obj.is_file() and own_file.is_file() and own_file.read_text() == own:
