@@ -284,7 +284,7 @@ int bt_cache4_decode(const void* q, long long q_row, void* out, const void* pool
 int bt_cache4_prompt(const void* q, long long q_row, void* out, const void* pool, long long n_pages, const int* table, int table_stride,
                      int table_len, int* status, const int* seq_start, const int* past_len, int n_tokens, int n_seqs, int max_new, int n_heads,
                      int n_kv_heads, int dim, float scale, int window, int keep_first, int n_splits, int rows, float* scratch,
-                     long long scratch_floats, cudaStream_t stream);
+                     long long scratch_floats, int behind_others, cudaStream_t stream);
 int bt_qk_norm_rotary(const void* src, long long src_row, void* dst, long long dst_row, const int* positions, const float* freq,
                       const float* q_weight, const float* k_weight, int n_tokens, int n_heads, int n_kv_heads, int dim, int rot, float eps,
                       float size, int interleaved, int dtype, cudaStream_t stream);

@@ -1939,7 +1939,7 @@ _RECORDS = {name: struct.Struct("=" + letters) for name, letters in {
     "bt_cache4_gather_packed": "QqqQqqQqQQQiiiQiiiiQ",
     "bt_cache4_attention_packed": "QqQQqQiiQQQiiiiiifiiiiQqiQ",
     "bt_cache4_decode_packed": "QqQQqQiiQQQiiiiiifiiiiQqQ",
-    "bt_cache4_prompt_packed": "QqQQqQiiQQQiiiiiifiiiiQqQ",
+    "bt_cache4_prompt_packed": "QqQQqQiiQQQiiiiiifiiiiQqiQ",
 }.items()}
 
 
@@ -2292,6 +2292,6 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     if kind == "few":
         _call_packed("bt_cache4_decode_packed", *call, _raw_stream(device))
     elif kind == "many":
-        _call_packed("bt_cache4_prompt_packed", *call, _raw_stream(device))
+        _call_packed("bt_cache4_prompt_packed", *call, 1 if max_ctx > max_new else 0, _raw_stream(device))
     else:
         _call_packed("bt_cache4_attention_packed", *call, code, _raw_stream(device))

@@ -402,3 +402,23 @@ def test_more_sequences_than_run_at_once(seqs, new, heads, kv, dim, window, keep
     order = torch.cat([torch.arange(step.starts[s], step.starts[s + 1]) for s in reversed(range(seqs))]).to(DEV)
     back.table = torch.flip(step.table, (0,)).contiguous()
     assert torch.equal(attend(back, q[order], pool, heads, kv, dim, window, keep, 0.2), got[order])
+
+
+@pytest.mark.parametrize("seqs, new, longest", [(9, 70, 300), (12, 33, 200), (40, 20, 100)])
+@pytest.mark.parametrize("heads, kv, dim", [(64, 8, 128), (32, 16, 64)])
+@pytest.mark.parametrize("window, keep", [(0, 0), (150, 3)])
+def test_more_portions_than_run_at_once(seqs, new, longest, heads, kv, dim, window, keep):
+    """Pasts in any order, sequences without tokens among them: the blocks are not begun in their order, and the results do not show it."""
+    rng = np.random.default_rng(seqs + dim)
+    pasts = [int(p) for p in rng.choice([0, 7, 64, 190, 190, longest], seqs)]
+    news = [int(n) for n in rng.integers(0, new + 1, seqs)]
+    news[2] = new
+    step = Step(pasts, news)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, 0.2)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, 0.2)
+    back = Step(pasts[::-1], news[::-1])
+    order = torch.cat([torch.arange(step.starts[s], step.starts[s + 1]) for s in reversed(range(seqs))]).to(DEV)
+    back.table = torch.flip(step.table, (0,)).contiguous()
+    assert torch.equal(attend(back, q[order], pool, heads, kv, dim, window, keep, 0.2), got[order])
