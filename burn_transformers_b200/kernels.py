@@ -2176,6 +2176,12 @@ def _cache4_few(sms, units, pages, wide, head_dim):
     return best[1], best[2]
 
 
+def _cache4_pages_seen(tokens, max_ctx, window):
+    """Pages that `tokens` new tokens in a row see at most (kept first ones aside): what the keys of a prompt are cut by and its scratch counted by."""
+    whole = -(-max(1, max_ctx) // PAGE_SIZE)
+    return min(whole, -(-(window + tokens) // PAGE_SIZE) + 1) if window else whole
+
+
 def _cache4_many(sms, units, columns, max_new, max_ctx, window, head_dim):
     """(rows a block, pieces of the keys) for `units` times `columns` rows of `max_new` new tokens, with a multiprocessor for each block.
 
@@ -2189,7 +2195,7 @@ def _cache4_many(sms, units, columns, max_new, max_ctx, window, head_dim):
     best = (math.inf, 256, 1)
     for rows, page in ((256, 0.95), (128, 0.5 if head_dim == 64 else 0.9)):
         blocks = units * -(-columns // rows)
-        pages = min(whole, -(-(window + rows * max_new // columns) // PAGE_SIZE) + 1) if window else whole
+        pages = _cache4_pages_seen(min(rows, columns) * max_new // columns, max_ctx, window)
         mean = min(pages, whole * (0.55 * (1.0 - fresh) + 0.5 * fresh))
         for pieces in {1, 2, 3, 4, 6, sms // blocks, -(-pages // 16), -(-pages // 8)}:
             if pieces < 1 or (pieces > 1 and (2 * pieces > pages + 1 or blocks * pieces > sms)):
@@ -2228,7 +2234,8 @@ def _cache4_plan(sms, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, head_dim, w
         return "few", warps, pieces, units * pieces * one if pieces > 1 else 0, most * one
     rows, pieces = _cache4_many(sms, units, columns, max_new, max_ctx, window, head_dim)
     one = rows * (head_dim + 2)
-    most = min(sms, units * -(-columns // 128) * -(-span // (2 * PAGE_SIZE)))
+    # (pieces of two pages at least, in all no more blocks than multiprocessors)
+    most = min(sms, units * -(-columns // 128) * ((_cache4_pages_seen(max_new, max_ctx, window) + 1) // 2))
     return "many", rows, pieces, units * -(-columns // rows) * pieces * one if pieces > 1 else 0, most * 256 * (head_dim + 2)
 
 

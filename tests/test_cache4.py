@@ -1,5 +1,7 @@
 """What the calls of the 4-bit cache and of the norm with rotation refuse, and how a step is cut into pieces: no device is needed (a
 tensor that says it lies on one, and a library that must not be reached)."""
+import math
+import random
 import re
 from pathlib import Path
 
@@ -194,3 +196,40 @@ def test_records_are_laid_out_as_the_library_reads_them():
 def test_arguments_that_fit_no_record(call, change):
     with pytest.raises(ShapeError, match="does not fit"):
         call(**change)
+
+
+# heads, key heads, new tokens, longest sequence, window, kept positions: few rows behind a window of a few pages, one or two blocks
+FEW_ROWS_IN_A_WINDOW = [(1, 1, 56, 1023, 415, 0), (2, 2, 56, 3301, 448, 0), (4, 2, 16, 23_538, 482, 0), (2, 1, 12, 3025, 467, 0), (1, 1, 25, 12_292, 334, 1),
+                        (2, 2, 40, 10_764, 433, 0)]
+
+
+@pytest.mark.parametrize("heads, kv, new, ctx, window, keep", FEW_ROWS_IN_A_WINDOW)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_scratch_that_is_asked_for_is_taken(heads, kv, new, ctx, window, keep, dim):
+    sizes = dict(n_tokens=new, n_seqs=1, max_new=new, max_ctx=ctx, n_heads=heads, n_kv_heads=kv, head_dim=dim, window=window, keep_first=keep)
+    floats = kernels.cache4_attention_scratch_floats(**sizes)
+    width = -(-ctx // 64)
+    with pytest.raises(Reached):
+        attend(q=dev(new, heads * dim), out=dev(new, heads * dim), pool=dev(2, kv, 68 * dim, dtype=torch.uint8), table=ints(1, width), table_len=width,
+               seq_start=ints(2), past_len=ints(1), scratch=dev(floats, dtype=torch.float32), **sizes)
+
+
+def test_scratch_over_random_sizes():
+    """What is asked for covers the step itself and any of fewer or shorter sequences, over sizes of every order."""
+    rng = random.Random(4)
+
+    def spread(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    for _ in range(3000):
+        kv, group, dim = rng.choice((1, 1, 2, 3, 8)), rng.choice((1, 1, 2, 4, 8)), rng.choice((32, 64, 128, 128))
+        seqs, new = spread(1, 40), spread(1, 400)
+        ctx = new + rng.choice((0, spread(1, 40_000)))
+        window, keep = rng.choice(((0, 0), (spread(1, 3000), rng.choice((0, 1, 4, 70, 500))), (rng.randint(300, 520), 0)))
+        sms = rng.choice((148, 148, 16, 132))
+        plan = lambda n, c, fast: kernels._cache4_plan(sms, n, new, c, kv * group, kv, dim, window, keep, fast)      # noqa: E731
+        asked = max(plan(seqs, ctx, fast)[4] for fast in (True, False))
+        for fewer in {1, max(1, seqs // 2), seqs}:
+            for shorter in {new, new + (ctx - new) // 3, new + (ctx - new) * 2 // 3, ctx}:
+                needs = max(plan(fewer, shorter, fast)[3] for fast in (True, False))
+                assert needs <= asked, (sms, seqs, new, ctx, kv, group, dim, window, keep, fewer, shorter)
