@@ -13,13 +13,10 @@ class SideBySideMixers(Mixer):
 
     def __init__(self, left: Mixer, right: Mixer):
         self.left, self.right = left, right
-        a, b = left.cache_need(), right.cache_need()
-        if a.kv is not None and b.kv is not None:
-            raise ShapeError("mixers side by side: only one of the two may keep keys and values in pages")
-        names = [s.name for s in a.states + b.states]
+        need = self.cache_need()
+        names = [s.name for s in need.states]
         if len(set(names)) != len(names):
             raise ShapeError(f"mixers side by side: their states share a name ({names})")
-        self._need = CacheNeed(kv=a.kv if a.kv is not None else b.kv, states=a.states + b.states)
         # the rows are read twice, so they are real rows and no handle for a product to resolve
         self.accepts_lazy_norm = False
 
@@ -31,7 +28,11 @@ class SideBySideMixers(Mixer):
         return self.left.graph_safe and self.right.graph_safe
 
     def cache_need(self):
-        return self._need
+        # (asked of the two each time: how a mixer holds its keys and values may be set after it was put here)
+        a, b = self.left.cache_need(), self.right.cache_need()
+        if a.kv is not None and b.kv is not None:
+            raise ShapeError("mixers side by side: only one of the two may keep keys and values in pages")
+        return CacheNeed(kv=a.kv if a.kv is not None else b.kv, states=a.states + b.states)
 
     def forward(self, ctx, x, residual, entry, owns_cache=True):
         self.left.forward(ctx, x, residual, entry, owns_cache)

@@ -2,9 +2,12 @@
 import pytest
 import torch
 
+import gokezen_configs
 from burn_transformers_b200.cache import CacheBank, CacheConfig, CacheNeed, KvSpec
 from burn_transformers_b200.config import Gpt2Config
+from burn_transformers_b200.config.gokezen import GokezenConfig
 from burn_transformers_b200.errors import CacheError, ShapeError
+from burn_transformers_b200.models.gokezen import build_gokezen
 from burn_transformers_b200.models.gpt2 import build_gpt2
 from burn_transformers_b200.parts import CausalSelfAttention
 
@@ -61,3 +64,19 @@ def test_norms_of_heads_are_tensors_of_the_part():
     part = CausalSelfAttention(128, 4, 2, 32, 0.125, qk_norm_eps=1e-6, cache_bits=4, window=100, keep_first=4)
     assert part.specs()["q_norm.weight"].shape == (32,) and part.specs()["k_norm.weight"].shape == (32,)
     assert part.cache_need().kv == KvSpec(2, 32, bits=4)
+
+
+def gokezen_plan(config):
+    return build_gokezen(GokezenConfig.from_dict(config))
+
+
+@pytest.mark.parametrize("config", [gokezen_configs.ONLY_LEFT, gokezen_configs.ODD])
+def test_mixers_side_by_side_hold_their_cache_in_4_bits(config):
+    plan = gokezen_plan(config)
+    before = plan.cache_needs()
+    plan.hold_cache_in(4)
+    for need, was in zip(plan.cache_needs(), before):
+        assert need.kv.bits == 4 and (need.kv.n_kv_heads, need.kv.head_dim) == (was.kv.n_kv_heads, was.kv.head_dim)
+        assert need.states == was.states
+    bank = CacheBank(plan.cache_needs(), CacheConfig(64 * 8, 2, 200), torch.bfloat16, "cpu")
+    assert all(g.k.dtype == torch.uint8 for g in bank.groups)
