@@ -79,15 +79,18 @@ class ModelPlan:
         return WeightPlan(tensors, self.namespaces, self.probe, self.ignored, dict(self.tied), dict(self.sources))
 
     def hold_cache_in(self, bits: int) -> None:
-        """Has every mixer that can hold its keys and values in `bits` bits do so; before an engine makes its cache."""
+        """Has every mixer that can hold its keys and values in `bits` bits do so, or raises and changes nothing; before an engine makes its
+        cache."""
         able = [part for part in self.all_parts() if hasattr(part, "hold_cache_in")]
         if not able:
             raise CacheError(f"cache_bits {bits}: no attention of this model has a cache that can be held in fewer bits")
+        try:
+            for part in able:
+                part.check_cache_bits(bits)
+        except ShapeError as error:
+            raise CacheError(f"cache_bits {bits}: {error}") from None
         for part in able:
-            try:
-                part.hold_cache_in(bits)
-            except ShapeError as error:
-                raise CacheError(f"cache_bits {bits}: {error}") from None
+            part.hold_cache_in(bits)
 
     def cache_needs(self) -> list[CacheNeed]:
         """One entry per call of the schedule; readers of another call's cache need nothing."""

@@ -73,13 +73,17 @@ class CausalSelfAttention(Mixer):
         if cache_bits is not None:
             self.hold_cache_in(cache_bits)
 
-    def hold_cache_in(self, bits: int) -> None:
-        """Has the cache hold this layer's keys and values in `bits` (4) bits; before the engine makes its cache."""
+    def check_cache_bits(self, bits: int) -> None:
+        """Raises what stands against holding this layer's keys and values in `bits` bits."""
         if bits != 4:
             raise ShapeError(f"a cache holds keys and values in the model's type or in 4 bits, not in {bits}")
         if self.head_dim % 32 or not self.causal:
             raise ShapeError(f"a cache in 4 bits takes causal attention over heads of a multiple of 32 channels, not of {self.head_dim}")
-        self.cache_bits = 4
+
+    def hold_cache_in(self, bits: int) -> None:
+        """Has the cache hold this layer's keys and values in `bits` (4) bits; before the engine makes its cache."""
+        self.check_cache_bits(bits)
+        self.cache_bits = bits
 
     def bind(self, tensors):
         if self.positions is not None and hasattr(self.positions, "inv_freq"):

@@ -80,3 +80,12 @@ def test_mixers_side_by_side_hold_their_cache_in_4_bits(config):
         assert need.states == was.states
     bank = CacheBank(plan.cache_needs(), CacheConfig(64 * 8, 2, 200), torch.bfloat16, "cpu")
     assert all(g.k.dtype == torch.uint8 for g in bank.groups)
+
+
+@pytest.mark.parametrize("bits, config, words", [(4, gokezen_configs.MIXED, "not of 16"), (8, gokezen_configs.ONLY_LEFT, "not in 8")])
+def test_a_plan_that_is_refused_stays_as_it_was(bits, config, words):
+    plan = gokezen_plan(config)
+    before = plan.cache_needs()
+    with pytest.raises(CacheError, match=words):
+        plan.hold_cache_in(bits)
+    assert plan.cache_needs() == before
