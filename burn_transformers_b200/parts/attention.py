@@ -147,9 +147,10 @@ class CausalSelfAttention(Mixer):
             k = proj[:n, self.q_width:self.q_width + self.kv_width].view(n, self.n_kv_heads, self.head_dim)
             v = proj[:n, self.q_width + self.kv_width:].view(n, self.n_kv_heads, self.head_dim)
             kernels.cache4_append(k, v, pool, ctx.positions, ctx.token_seq, ctx.ctx_len, table, group.table_len, n_tokens=n)
-        # (bounded by the cache's longest sequence, not by the step's: how the keys are cut, and with it the last bits of the results, is then
-        # the same for a step that is recorded and one that is not)
-        sizes = dict(n_tokens=n, n_seqs=ctx.n_seqs, max_new=1 if ctx.is_decode else ctx.max_new, max_ctx=ctx.cache.config.max_context,
+        # (where sequences go on, bounded by the cache's longest, not by the step's: how the keys are cut, and with it the last bits of the
+        # results, is then the same for a step that is recorded and one that is not.  Prompts without a past are recorded by their sizes)
+        max_ctx = ctx.max_new if ctx.fresh and not ctx.is_decode else ctx.cache.config.max_context
+        sizes = dict(n_tokens=n, n_seqs=ctx.n_seqs, max_new=1 if ctx.is_decode else ctx.max_new, max_ctx=max_ctx,
                      n_heads=self.n_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, window=self.window or 0, keep_first=self.keep_first)
         floats = kernels.cache4_attention_scratch_floats(**sizes)
         scratch = ctx.ws.take((floats,), torch.float32) if floats else None

@@ -6,10 +6,11 @@ import gokezen_configs
 from burn_transformers_b200.cache import CacheBank, CacheConfig, CacheNeed, KvSpec
 from burn_transformers_b200.config import Gpt2Config
 from burn_transformers_b200.config.gokezen import GokezenConfig
+from burn_transformers_b200.engine import StepBuilder, StepEntry
 from burn_transformers_b200.errors import CacheError, ShapeError
 from burn_transformers_b200.models.gokezen import build_gokezen
 from burn_transformers_b200.models.gpt2 import build_gpt2
-from burn_transformers_b200.parts import CausalSelfAttention
+from burn_transformers_b200.parts import CausalSelfAttention, attention
 
 
 def test_a_group_in_4_bits_is_one_pool_of_bytes():
@@ -89,3 +90,37 @@ def test_a_plan_that_is_refused_stays_as_it_was(bits, config, words):
     with pytest.raises(CacheError, match=words):
         plan.hold_cache_in(bits)
     assert plan.cache_needs() == before
+
+
+@pytest.fixture
+def asked(monkeypatch):
+    """The sizes that a layer hands to the attention over its 4-bit cache; nothing is computed."""
+    calls = []
+    monkeypatch.setattr(attention.kernels, "cache4_append", lambda *args, **kw: None)
+    monkeypatch.setattr(attention.kernels, "cache4_attention_scratch_floats", lambda **kw: 0)
+    monkeypatch.setattr(attention.kernels, "cache4_attention", lambda *args, **kw: calls.append(kw))
+    monkeypatch.setattr(attention, "linear", lambda *args, **kw: None)
+    return calls
+
+
+def steps_of(part, runs, max_context=640, max_tokens=64 * 20):
+    """Has `part` take steps of new tokens a sequence, (3, 1) for two sequences, one after another."""
+    part.t_qkv_weight = part.t_qkv_bias = part.t_out_weight = part.t_out_bias = None
+    part.nk_qkv_weight = part.nk_out_weight = False
+    cache = CacheBank([part.cache_need()], CacheConfig(max_tokens, 4, max_context), torch.bfloat16, "cpu")
+    builder = StepBuilder(cache, torch.bfloat16, "cpu")
+    slots = [cache.acquire() for _ in runs[0]]
+    for news in runs:
+        cache.reserve([(s, cache.length(s) + n) for s, n in zip(slots, news)])
+        ctx = builder.build([StepEntry(s, [0] * n, []) for s, n in zip(slots, news)])
+        builder.ws.reset()
+        part.forward(ctx, torch.zeros(sum(news), part.width), torch.zeros(sum(news), part.width), 0)
+        for s, n in zip(slots, news):
+            cache.commit(s, cache.length(s) + n)
+    return cache
+
+
+def test_prompts_without_a_past_are_planned_as_such(asked):
+    """Steps whose sequences all begin are bounded by their own tokens; others by the cache's longest sequence, as recorded ones are."""
+    steps_of(CausalSelfAttention(128, 2, 2, 64, 0.125, cache_bits=4), [(200, 33), (1, 1), (7, 2)])
+    assert [(kw["max_new"], kw["max_ctx"]) for kw in asked] == [(200, 200), (1, 640), (7, 640)]
