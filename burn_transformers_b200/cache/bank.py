@@ -109,6 +109,10 @@ class CacheBank:
             else:
                 table_len = min(self.table_width, pages_for(spec.window))
                 n_pages = min(budget_pages, config.max_slots * table_len)
+                # in 4 bits a sequence keeps every position (and takes portions of any length) while that takes no more than its ring in the
+                # model's type would; there are then as many times more pages as it may hold, so that there is room for what had room
+                if spec.bits is not None and self.table_width * 68 <= table_len * 2 * PAGE_SIZE * kv_dtype.itemsize:
+                    table_len, n_pages = self.table_width, n_pages * self.table_width // table_len
             shape = (len(entries), n_pages, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
             # (a group without values keeps an empty value pool, so that every group has the same two fields)
             v_shape = shape if spec.has_values else (len(entries), 0, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)

@@ -34,9 +34,10 @@ class CausalSelfAttention(Mixer):
     [head_dim]), before `positions` turns it, in the same pass where `positions` offers it.
 
     `cache_bits` 4 (or `hold_cache_in(4)`): the cache holds keys and values in 4-bit codes (csrc/cache4.cuh).  Every query then attends over
-    what the cache holds, the step's own keys and values too, so that a sequence's results do not depend on the portions that it
-    came in.  With a `window`, positions below `keep_first` stay visible beside it (of a cache in 4 bits only), and the cache keeps
-    every position.
+    held values, the step's own too: a sequence's portions change nothing but roundings (of sums, and in bfloat16 of the softmax weights,
+    which are rounded relative to the largest score that a warp or piece has met: up to 2^-9 of each).  With a `window` the cache keeps what
+    the window needs, or every position where that takes no more than the window's ring in the model's type (cache/bank.py); positions below
+    `keep_first` (of a cache in 4 bits only) stay visible beside the window, and the cache then keeps every position.
     """
 
     accepts_lazy_norm = True
@@ -110,7 +111,8 @@ class CausalSelfAttention(Mixer):
 
     def cache_need(self):
         if self.cache_bits is not None:
-            return CacheNeed(kv=KvSpec(self.n_kv_heads, self.head_dim, bits=self.cache_bits))
+            # (kept first positions lie in pages that come round to nothing else)
+            return CacheNeed(kv=KvSpec(self.n_kv_heads, self.head_dim, None if self.keep_first else self.window, bits=self.cache_bits))
         return CacheNeed(kv=KvSpec(self.n_kv_heads, self.head_dim, self.window))
 
     def _splits(self, ctx) -> int:
@@ -139,14 +141,37 @@ class CausalSelfAttention(Mixer):
         if self.positions is not None:
             self.positions.rotate(ctx, proj, *heads)
 
+    def _step_pages(self, ctx):
+        """Pages of the step's own for sequences that begin with it: (pool, table, table_len).  Sequence s has the pages from
+        seq_start[s] // 64 + s on, as many as its tokens can fill."""
+        table_len = -(-ctx.max_new // PAGE_SIZE)
+        pool = ctx.ws.take((ctx.n_tokens // PAGE_SIZE + ctx.n_seqs, self.n_kv_heads, kernels.cache4_record_bytes(self.head_dim)), torch.uint8)
+        table = ctx.ws.take((ctx.n_seqs, table_len), torch.int32)
+        first, count = ctx.ws.take((ctx.n_seqs,), torch.int32), ctx.ws.take((max(ctx.n_seqs, table_len),), torch.int32)
+        torch.arange(count.shape[0], out=count)
+        torch.div(ctx.seq_start[:ctx.n_seqs], PAGE_SIZE, rounding_mode="floor", out=first)
+        first.add_(count[:ctx.n_seqs])
+        torch.add(first[:, None], count[:table_len], out=table)
+        return pool, table, table_len
+
     def _forward_4_bits(self, ctx, proj, residual, entry, owns_cache) -> None:
         n = ctx.n_tokens
         pool, _, group, g = ctx.cache.layer_pools(entry)
-        table = ctx.tables[g]
+        table, table_len = ctx.tables[g], group.table_len
+        # prompts that a ring does not hold whole: their queries attend over pages that live as long as the step
+        longer = group.is_ring and self.window is not None and not ctx.is_decode and ctx.max_new > table_len * PAGE_SIZE - self.window + 1
+        if longer and not (ctx.fresh and owns_cache):
+            # (the engine refuses such a step before the cache changes; this guards direct users of the part)
+            raise CacheError("a step that brings this many tokens to sequences that already hold some would overwrite keys of a "
+                             "windowed layer's ring that its first tokens still see")
         if owns_cache:
             k = proj[:n, self.q_width:self.q_width + self.kv_width].view(n, self.n_kv_heads, self.head_dim)
             v = proj[:n, self.q_width + self.kv_width:].view(n, self.n_kv_heads, self.head_dim)
-            kernels.cache4_append(k, v, pool, ctx.positions, ctx.token_seq, ctx.ctx_len, table, group.table_len, n_tokens=n)
+            new = (ctx.positions, ctx.token_seq, ctx.ctx_len)
+            kernels.cache4_append(k, v, pool, *new, table, table_len, n_tokens=n)
+            if longer:
+                pool, table, table_len = self._step_pages(ctx)
+                kernels.cache4_append(k, v, pool, *new, table, table_len, n_tokens=n)
         # (where sequences go on, bounded by the cache's longest, not by the step's: how the keys are cut, and with it the last bits of the
         # results, is then the same for a step that is recorded and one that is not.  Prompts without a past are recorded by their sizes)
         max_ctx = ctx.max_new if ctx.fresh and not ctx.is_decode else ctx.cache.config.max_context
@@ -155,7 +180,7 @@ class CausalSelfAttention(Mixer):
         floats = kernels.cache4_attention_scratch_floats(**sizes)
         scratch = ctx.ws.take((floats,), torch.float32) if floats else None
         mixed = ctx.ws.take((n, self.q_width), ctx.dtype)
-        kernels.cache4_attention(proj, mixed, pool, table, group.table_len, ctx.seq_start, ctx.past_len, scale=self.scale, scratch=scratch, **sizes)
+        kernels.cache4_attention(proj, mixed, pool, table, table_len, ctx.seq_start, ctx.past_len, scale=self.scale, scratch=scratch, **sizes)
         linear(ctx, mixed, self.t_out_weight, self.t_out_bias if self.has_bias else None, residual, m=n,
                residual=residual, w_is_nk=self.nk_out_weight)
 

@@ -75,12 +75,13 @@ def case(tmp_path, config, seed=21):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("positions, ring", [(400, False), (900, True)])
 @pytest.mark.parametrize("schedule", ["whole", "tail", "portions"])
-def test_an_engine_in_32_bits(tmp_path, monkeypatch, schedule):
-    folder, config, weights, seqs = case(tmp_path, gc.ONLY_LEFT)
+def test_an_engine_in_32_bits(tmp_path, monkeypatch, schedule, positions, ring):
+    folder, config, weights, seqs = case(tmp_path, dict(gc.ONLY_LEFT, max_positions=positions))
     ref, sure = reference(config, weights, seqs, monkeypatch)
-    engine = Engine.from_folder(folder, "float32", max_tokens=64 * 16, cache_bits=4)
-    assert all(g.k.dtype == torch.uint8 for g in engine.cache.groups)
+    engine = Engine.from_folder(folder, "float32", max_tokens=64 * 16, max_context=positions, cache_bits=4)
+    assert [(g.k.dtype, g.is_ring) for g in engine.cache.groups] == [(torch.uint8, ring)]
     # (15 tokens: what any cache of a window of 50 takes behind others)
     got = {"whole": lambda: replay.whole(engine, seqs), "tail": lambda: replay.tail_one_by_one(engine, seqs, tail=70),
            "portions": lambda: in_portions(engine, seqs, 15)}[schedule]()

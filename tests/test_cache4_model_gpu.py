@@ -7,7 +7,7 @@ import torch
 import burn_transformers_b200 as bt
 import plain_cache4 as plain
 from burn_transformers_b200 import kernels
-from burn_transformers_b200.cache import CacheBank, CacheConfig
+from burn_transformers_b200.cache import CacheBank, CacheConfig, CacheNeed, KvSpec
 from burn_transformers_b200.engine import StepBuilder, StepEntry
 from burn_transformers_b200.parts import CausalSelfAttention, HalfSplitRotary, InterleavedRotary
 from burn_transformers_b200.weights import MATRIX, random_tensors
@@ -204,3 +204,35 @@ def test_the_calls_of_a_step_recorded_together_and_replayed(heads, kv, dim):
     kernels.check_status(torch.device(DEV))
     for lane in range(2):
         assert torch.equal(torch.stack(got[lane]), want[lane])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads, kv, dim, window", [(4, 2, 64, 100), (2, 2, 128, 150), (8, 1, 32, 64), (3, 3, 96, 1)])
+def test_a_layer_over_a_ring_and_over_every_position(dtype, heads, kv, dim, window):
+    """Prompts longer than the ring, single tokens across its turns, and the longest portions that it takes: the same bits as over a cache
+    that keeps every position."""
+    width, longest = 96, 64 * 40
+    part = CausalSelfAttention(width, heads, kv, dim, dim ** -0.5, cache_bits=4, window=window)
+    bound(part, dtype)
+    caches = [CacheBank([need], CacheConfig(64 * 100, 4, longest), dtype, DEV) for need in (part.cache_need(), CacheNeed(kv=KvSpec(kv, dim, bits=4)))]
+    ring = caches[0].groups[0]
+    assert ring.is_ring and not caches[1].groups[0].is_ring
+    run = caches[0].max_continued_run
+    builders = [StepBuilder(cache, dtype, DEV) for cache in caches]
+    slots = [[cache.acquire() for _ in range(3)] for cache in caches]
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for news in [[400, 1, 200]] + [[1, 1, 1]] * 3 + [[run, 1, min(run, 2)]] * 4 + [[1, 1, 1]] * 70 + [[min(run, 5), run, run]] * 3:
+        x = torch.randn(sum(news), width, generator=gen, device=DEV).to(dtype)
+        residual = torch.randn(sum(news), width, generator=gen, device=DEV)
+        results = []
+        for cache, builder, ids in zip(caches, builders, slots):
+            cache.reserve([(s, cache.length(s) + n) for s, n in zip(ids, news)])
+            ctx = builder.build([StepEntry(s, [0] * n, []) for s, n in zip(ids, news)])
+            out = residual.clone()
+            builder.ws.reset()
+            part.forward(ctx, x, out, 0)
+            results.append(out)
+            for s, n in zip(ids, news):
+                cache.commit(s, cache.length(s) + n)
+        kernels.check_status(torch.device(DEV))
+        assert bool(torch.isfinite(results[0]).all()) and torch.equal(*results), news

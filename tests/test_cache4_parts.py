@@ -1,4 +1,6 @@
 """What holds its keys and values in 4 bits, and what refuses to, without a device."""
+import random
+
 import pytest
 import torch
 
@@ -124,3 +126,87 @@ def test_prompts_without_a_past_are_planned_as_such(asked):
     """Steps whose sequences all begin are bounded by their own tokens; others by the cache's longest sequence, as recorded ones are."""
     steps_of(CausalSelfAttention(128, 2, 2, 64, 0.125, cache_bits=4), [(200, 33), (1, 1), (7, 2)])
     assert [(kw["max_new"], kw["max_ctx"]) for kw in asked] == [(200, 200), (1, 640), (7, 640)]
+
+
+def windowed(window, keep=0, dim=64):
+    return CausalSelfAttention(128, 2, 2, dim, 0.125, cache_bits=4, window=window, keep_first=keep)
+
+
+def nbytes(bank):
+    return sum(g.k.nbytes + g.v.nbytes for g in bank.groups)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window, context", [(1, 64), (50, 400), (64, 4096), (130, 640), (512, 1900), (512, 4096), (512, 16_384), (5000, 4096)])
+@pytest.mark.parametrize("slots, tokens", [(1, 64), (3, 1000), (8, 4096), (64, 4096), (7, 100_000)])
+def test_a_window_in_4_bits_takes_no_more_than_in_the_model_type(dtype, window, context, slots, tokens):
+    """Neither bytes nor, for any lengths of the sequences, room."""
+    config = CacheConfig(tokens, slots, context)
+    part = windowed(window)
+    assert part.cache_need().kv.window == window
+    plain = CacheBank([CacheNeed(kv=KvSpec(2, 64, window))], config, dtype, "cpu")
+    packed = CacheBank([part.cache_need()], config, dtype, "cpu")
+    assert nbytes(packed) <= nbytes(plain)
+    assert packed.groups[0].k.dtype == torch.uint8 and (packed.groups[0].is_ring or packed.groups[0].whole)
+    if packed.groups[0].is_ring:
+        assert packed.max_continued_run == plain.max_continued_run and nbytes(packed) * 2 * plain.groups[0].k.element_size() * 64 == nbytes(plain) * 68
+    rng = random.Random(window + slots)
+    for _ in range(20):
+        wanted = [rng.choice((1, 64, rng.randint(1, context), context)) for _ in range(slots)]
+        held = []
+        for bank in (plain, packed):
+            slot_ids, room = [bank.acquire() for _ in wanted], 0
+            for slot, length in zip(slot_ids, wanted):
+                try:
+                    bank.reserve([(slot, length)])
+                    room += 1
+                except CacheError:
+                    break
+            bank.check()
+            for slot in slot_ids:
+                bank.release(slot)
+            held.append(room)
+        assert held[1] >= held[0]
+
+
+def test_kept_positions_need_every_page():
+    bank = CacheBank([windowed(50, 4).cache_need()], CacheConfig(4096, 2, 4096), torch.bfloat16, "cpu")
+    assert not bank.groups[0].is_ring and bank.max_continued_run is None
+
+
+def test_a_prompt_longer_than_the_ring_attends_over_pages_of_its_step(asked, monkeypatch):
+    filed, read = [], []
+    monkeypatch.setattr(attention.kernels, "cache4_append", lambda k, v, pool, *args, **kw: filed.append((pool, args[3], args[4])))
+    monkeypatch.setattr(attention.kernels, "cache4_attention",
+                        lambda q, out, pool, table, table_len, *args, **kw: read.append((pool, table.clone(), table_len, kw["max_ctx"])))
+    news = (200, 1, 65, 64)
+    cache = steps_of(windowed(100), [news, (1, 1, 1, 1), (29, 2, 1, 3)], max_context=4096)
+    ring = cache.groups[0]
+    assert ring.is_ring and ring.table_len == 2 and cache.max_continued_run == 29
+    # the prompts: filed in the ring and in the step's own pages, read from those
+    assert len(filed) == 4 and [f[0].data_ptr() == ring.k[0].data_ptr() for f in filed] == [True, False, True, True]
+    pool, table, table_len, bound = read[0]
+    assert pool.data_ptr() == filed[1][0].data_ptr() and (table_len, bound) == (4, 200) and pool.shape[1:] == (2, 68 * 64)
+    pages = [table[i, :-(-n // 64)].tolist() for i, n in enumerate(news)]
+    flat = sum(pages, [])
+    assert len(set(flat)) == len(flat) and min(flat) >= 0 and max(flat) < pool.shape[0]
+    # and later steps from the ring
+    assert [(r[0].data_ptr() == ring.k[0].data_ptr(), r[2], r[3]) for r in read[1:]] == [(True, 2, 4096)] * 2
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_pages_of_a_step_for_any_lengths(asked, monkeypatch, seed):
+    read = []
+    monkeypatch.setattr(attention.kernels, "cache4_attention", lambda q, out, pool, table, *args, **kw: read.append((pool, table.clone())))
+    rng = random.Random(seed)
+    for _ in range(20):
+        news = tuple(rng.choice((1, 63, 64, 65, 128, rng.randint(1, 500))) for _ in range(4)) [:rng.randint(1, 4)] + (200,)
+        steps_of(windowed(100), [news[-4:]], max_context=4096)
+        pool, table = read.pop()
+        flat = sum((table[i, :-(-n // 64)].tolist() for i, n in enumerate(news[-4:])), [])
+        assert len(set(flat)) == len(flat) and min(flat) >= 0 and max(flat) < pool.shape[0]
+
+
+def test_a_run_that_the_ring_does_not_hold_is_refused(asked):
+    with pytest.raises(CacheError, match="ring"):
+        steps_of(windowed(100), [(5, 200), (30, 1)], max_context=4096)
