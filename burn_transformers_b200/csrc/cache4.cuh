@@ -50,6 +50,15 @@ __device__ __forceinline__ void c4_new_tokens(const int* seq_start, int seq, int
   n_new = min(seq_start[seq + 1], n_tokens) - t0;
 }
 
+// A sequence's length before the step.  One that no sequence has is reported and taken for 0: positions, and with them the places in
+// the table, are never negative.
+__device__ __forceinline__ int c4_past(const int* past_len, int seq, int* status) {
+  const int past = past_len[seq];
+  if ((unsigned)past <= 1u << 30) return past;
+  if (status) atomicExch(status, 9);
+  return 0;
+}
+
 // Which keys the query at `pos` sees: `kept` first ones (0 .. kept - 1) and the run lo .. pos, which does not overlap them.
 __device__ __forceinline__ void c4_seen(int pos, int window, int keep_first, int& kept, int& lo) {
   lo = window > 0 ? max(0, pos - window + 1) : 0;

@@ -32,12 +32,12 @@ struct Cache4AnyParams {
 // A block's rows and the keys that any of them sees.
 struct C4Any {
   int t0, n_rows, row0, past, kept, lo, n_keys;
-  __device__ C4Any(const Cache4AnyParams& p, int seq, int row_block, int rows) {
+  __device__ C4Any(const Cache4AnyParams& p, int seq, int row_block, int rows, int* status) {
     int n_new;
     c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
     row0 = row_block * rows;
     n_rows = min(rows, n_new * p.group - row0);
-    past = p.past_len[seq];
+    past = c4_past(p.past_len, seq, status);
     const int first = past + row0 / p.group, last = past + (row0 + max(n_rows, 1) - 1) / p.group;
     int none;
     c4_seen(first, p.window, p.keep_first, none, lo);
@@ -62,7 +62,7 @@ cache4_attention_kernel(Cache4AnyParams p, Cache4View c) {
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = p.dim, seq = blockIdx.z, kv_head = blockIdx.y;
   const int piece = (int)blockIdx.x % p.pieces, row_block = (int)blockIdx.x / p.pieces;
-  const C4Any at(p, seq, row_block, ROWS);
+  const C4Any at(p, seq, row_block, ROWS, c.status);
   if (at.n_rows <= 0) return;
   const int per = (at.n_keys + p.pieces - 1) / p.pieces, begin = piece * per, end = min(at.n_keys, begin + per);
   if (begin >= end) return;
@@ -250,7 +250,7 @@ cache4_attention_join_kernel(Cache4AnyParams p) {
   pdl_trigger();
   pdl_wait();
   const int seq = blockIdx.z, kv_head = blockIdx.y, row_block = (int)blockIdx.x / ROWS, r = (int)blockIdx.x % ROWS, dim = p.dim;
-  const C4Any at(p, seq, row_block, ROWS);
+  const C4Any at(p, seq, row_block, ROWS, nullptr);
   if (r >= at.n_rows) return;
   const int per = (at.n_keys + p.pieces - 1) / p.pieces, used = (at.n_keys + per - 1) / per;
   const long long unit = ((long long)seq * gridDim.y + kv_head) * ((int)gridDim.x / ROWS) + row_block;

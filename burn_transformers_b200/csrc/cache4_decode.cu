@@ -63,11 +63,11 @@ constexpr int C4D_SORTED = 128;           // sequences that are sorted, at most
 struct C4dSequence {
   int seq, past, t0, n_new;
 };
-__device__ __forceinline__ C4dSequence c4d_sequence(const Cache4DecodeParams& p, int n_seqs, int rank) {
+__device__ __forceinline__ C4dSequence c4d_sequence(const Cache4DecodeParams& p, int n_seqs, int rank, int* status) {
   C4dSequence at;
   if (!p.sorted) {
     at.seq = rank;
-    at.past = p.past_len[rank];
+    at.past = c4_past(p.past_len, rank, status);
     c4_new_tokens(p.seq_start, rank, p.n_tokens, at.t0, at.n_new);
     return at;
   }
@@ -82,7 +82,7 @@ __device__ __forceinline__ C4dSequence c4d_sequence(const Cache4DecodeParams& p,
   __syncthreads();
   for (int i = tid; i < n_seqs; i += threads) {
     at.seq = i;
-    at.past = p.past_len[i];
+    at.past = c4_past(p.past_len, i, status);
     c4_new_tokens(p.seq_start, i, p.n_tokens, at.t0, at.n_new);
     const int mine = s_key[i];
     int before[4] = {0, 0, 0, 0};
@@ -123,7 +123,7 @@ cache4_decode_kernel(Cache4DecodeParams p, Cache4View c) {
   const int n_warps = (int)blockDim.x >> 5;
   const int split = blockIdx.x, n_splits = gridDim.x;
   const int kv_head = (int)blockIdx.y / p.col_blocks, col0 = (int)blockIdx.y % p.col_blocks * COLS;
-  const C4dSequence at_seq = c4d_sequence(p, gridDim.z, blockIdx.z);
+  const C4dSequence at_seq = c4d_sequence(p, gridDim.z, blockIdx.z, c.status);
   const int seq = at_seq.seq, past = at_seq.past, t0 = at_seq.t0, n_new = at_seq.n_new;
   const int n_cols = n_new * p.group - col0;
   if (n_cols <= 0) return;
@@ -494,7 +494,7 @@ cache4_join_kernel(Cache4DecodeParams p, int n_splits) {
   int t0, n_new;
   c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (col0 + col >= n_new * p.group) return;
-  const int past = p.past_len[seq];
+  const int past = c4_past(p.past_len, seq, nullptr);
   const int pos_first = past + col0 / p.group, pos_last = past + min(n_new * p.group - 1, col0 + COLS - 1) / p.group;
   const int pg_lo = (p.window > 0 ? max(0, pos_first - p.window + 1) : 0) / C4_PAGE;
   const int kept_only = p.window > 0 ? min((min(p.keep_first, pos_last + 1) + C4_PAGE - 1) / C4_PAGE, pg_lo) : 0;

@@ -102,7 +102,7 @@ __device__ __forceinline__ int2 c4p_place_of(const Cache4PromptParams& p, int se
       const int s = tid / tiles, row0 = tid % tiles * p.rows;
       int t0, n_new, pages = 0;
       c4_new_tokens(p.seq_start, s, p.n_tokens, t0, n_new);
-      if (n_new * p.group > row0) pages = max(0, C4pRun(p.past_len[s], n_new, row0, p.rows, p.group, p.window, p.keep_first, 1).n_pages);
+      if (n_new * p.group > row0) pages = max(0, C4pRun(c4_past(p.past_len, s, nullptr), n_new, row0, p.rows, p.group, p.window, p.keep_first, 1).n_pages);
       mine = min(pages, (1 << 23) - 1) * C4P_SORTED + C4P_SORTED - tid;
     }
     s_key[tid] = mine;
@@ -146,7 +146,7 @@ cache4_prompt_kernel(Cache4PromptParams p, Cache4View c) {
   const int row0 = tile * p.rows;
   const int n_rows = min(p.rows, n_new * p.group - row0);
   if (n_rows <= 0) return;
-  const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, (int)gridDim.z);
+  const C4pRun run(c4_past(p.past_len, seq, c.status), n_new, row0, p.rows, p.group, p.window, p.keep_first, (int)gridDim.z);
   // steps of a page each; two in a row are a tile of the stages
   const int page0 = (int)blockIdx.z * run.per, n_steps = min(run.n_pages, page0 + run.per) - page0, n_tiles = (n_steps + 1) / 2;
   if (n_steps <= 0) return;
@@ -501,7 +501,7 @@ cache4_prompt_join_kernel(Cache4PromptParams p, int n_kv_heads, int row_tiles, i
   int t0, n_new;
   c4_new_tokens(p.seq_start, seq, p.n_tokens, t0, n_new);
   if (row >= n_new * p.group) return;
-  const C4pRun run(p.past_len[seq], n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
+  const C4pRun run(c4_past(p.past_len, seq, nullptr), n_new, row0, p.rows, p.group, p.window, p.keep_first, n_splits);
   const int used = (run.n_pages + run.per - 1) / run.per;
   const long long unit0 = ((long long)blockIdx.y * row_tiles + tile) * n_splits * p.rows + r;      // run s: p.rows further
   const float2* ml = reinterpret_cast<const float2*>(p.part + p.part_ml);

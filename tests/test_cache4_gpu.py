@@ -422,3 +422,28 @@ def test_more_portions_than_run_at_once(seqs, new, longest, heads, kv, dim, wind
     order = torch.cat([torch.arange(step.starts[s], step.starts[s + 1]) for s in reversed(range(seqs))]).to(DEV)
     back.table = torch.flip(step.table, (0,)).contiguous()
     assert torch.equal(attend(back, q[order], pool, heads, kv, dim, window, keep, 0.2), got[order])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv, dim", [(4, 4, 64), (16, 4, 128)])
+@pytest.mark.parametrize("seqs, new", [(2, 1), (2, 90), (70, 1), (30, 60)])
+@pytest.mark.parametrize("window, keep", [(0, 0), (90, 3)])
+def test_a_past_that_no_sequence_has_is_reported(dtype, heads, kv, dim, seqs, new, window, keep):
+    """It counts as none; the other sequences do not notice."""
+    step, rng = Step([150 + 2 * s for s in range(seqs)], [new] * seqs), np.random.default_rng(1)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).to(dtype).to(DEV)
+    clean, past = attend(step, q, pool, heads, kv, dim, window, keep, 0.1), step.past
+    step.past = past.clone()
+    step.past[1] = 0
+    none = attend(step, q, pool, heads, kv, dim, window, keep, 0.1)[new:2 * new]
+    for wrong in (-1, -64, -2 ** 31, 2 ** 31 - 1):
+        step.past[1] = wrong
+        args = step.sizes(heads, kv, dim, window, keep)
+        out = torch.empty(step.n, heads * dim, dtype=dtype, device=DEV)
+        scratch = torch.empty(kernels.cache4_attention_scratch_floats(**args), device=DEV)
+        kernels.cache4_attention(q, out, pool, step.table, step.width, step.seq_start, step.past, scale=0.1, scratch=scratch, **args)
+        with pytest.raises(KernelError, match="outside its table or pool"):
+            kernels.check_status(torch.device(DEV))
+        assert torch.equal(out[new:2 * new], none)
+        assert torch.equal(out[:new], clean[:new]) and torch.equal(out[2 * new:], clean[2 * new:])
