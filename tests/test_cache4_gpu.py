@@ -447,3 +447,13 @@ def test_a_past_that_no_sequence_has_is_reported(dtype, heads, kv, dim, seqs, ne
             kernels.check_status(torch.device(DEV))
         assert torch.equal(out[new:2 * new], none)
         assert torch.equal(out[:new], clean[:new]) and torch.equal(out[2 * new:], clean[2 * new:])
+
+
+@pytest.mark.parametrize("heads, kv, dim, pasts, news", [(4, 2, 64, [70, 300, 0], [3, 1, 2]), (8, 1, 128, [900, 3000], [1, 1]), (6, 3, 64, [0, 65], [140, 90])])
+@pytest.mark.parametrize("window, keep", [(0, 0), (100, 3)])
+def test_the_kernel_for_every_case_when_it_is_asked_for(heads, kv, dim, pasts, news, window, keep):
+    step, rng = Step(pasts, news), np.random.default_rng(dim)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, dim ** -0.5, impl="any")
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, dim ** -0.5)
