@@ -23,6 +23,7 @@ import dataclasses
 import torch
 
 from ..errors import CacheError
+from ..kernels import cache4_record_bytes
 from . import native
 from .spec import PAGE_SIZE, CacheConfig, CacheNeed, KvSpec
 
@@ -111,14 +112,15 @@ class CacheBank:
                 n_pages = min(budget_pages, config.max_slots * table_len)
                 # in 4 bits a sequence keeps every position (and takes portions of any length) while that takes no more than its ring in the
                 # model's type would; there are then as many times more pages as it may hold, so that there is room for what had room
-                if spec.bits is not None and self.table_width * 68 <= table_len * 2 * PAGE_SIZE * kv_dtype.itemsize:
+                in_type = 2 * PAGE_SIZE * spec.head_dim * kv_dtype.itemsize
+                if spec.bits is not None and self.table_width * cache4_record_bytes(spec.head_dim) <= table_len * in_type:
                     table_len, n_pages = self.table_width, n_pages * self.table_width // table_len
             shape = (len(entries), n_pages, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
             # (a group without values keeps an empty value pool, so that every group has the same two fields)
             v_shape = shape if spec.has_values else (len(entries), 0, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
             dtype = kv_dtype
             if spec.bits is not None:      # a record of bytes a page and head: codes and scales of keys and values
-                dtype, shape, v_shape = torch.uint8, (*shape[:3], 68 * spec.head_dim), (len(entries), 0, spec.n_kv_heads, 0)
+                dtype, shape, v_shape = torch.uint8, (*shape[:3], cache4_record_bytes(spec.head_dim)), (len(entries), 0, spec.n_kv_heads, 0)
             group = KvGroup(spec, entries, table_len, _PageBooks(self, len(self.groups), n_pages),
                             torch.zeros(shape, dtype=dtype, device=self.device),
                             torch.zeros(v_shape, dtype=dtype, device=self.device),

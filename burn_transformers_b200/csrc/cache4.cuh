@@ -12,7 +12,7 @@
 
 namespace bt {
 
-constexpr int C4_PAGE = 64, C4_GROUP = 32;
+constexpr int C4_PAGE = 64;
 
 __host__ __device__ constexpr int c4_record(int dim) { return 68 * dim; }
 __host__ __device__ constexpr int c4_value_codes(int dim) { return 32 * dim; }
