@@ -4,8 +4,9 @@
 // round(x / s), ties to even, at most 7 in size: all decided exactly, so that the result does not depend on how a division rounds.
 // A group that holds an infinity or NaN is filed as NaN.  Values beyond what the format holds (25,088) are held as its largest.
 //
-// Bound by memory and by the integer pipe, and for a decode step by latency: 8,592 tokens of 8 heads of 128 channels, bfloat16, are filed in
-// 11.5 us (3.9 TB/s; 16.8 with scales by comparison and codes one by one) and read back in 7.4 (6.0 TB/s into L2); 64 tokens take 2.1 and 1.9.
+// 8,592 tokens of 8 heads of 128 channels, bfloat16, are filed in 11.5 us (3.9 TB/s; 16.8 with scales by comparison and codes one by one) and
+// read back in 7.4 (6.0 TB/s into L2); 64 tokens take 2.1 and 1.9.  Reading back is bound by its stores, a decode step by latency.  Filing of many
+// is bound by no unit alone (issue slots 56 % active, integer pipe 43): warps wait for their tokens' places and for the four lanes' maxima.
 // Four lanes share a group, a lane moves 8 channels in 16-byte pieces (32-bit inputs: two) and the four bytes of their codes beside its
 // neighbours'.  A block takes several tokens, a thread the same 8 channels of each, four of them in flight; where a token's records lie is
 // looked up once a block, while the first rows come.  Four tokens a block: 11.3; eight in flight: 12.2.

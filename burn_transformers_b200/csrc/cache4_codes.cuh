@@ -1,6 +1,6 @@
 // Codes of the 4-bit cache (cache4.cuh) as bfloat16 values, two at a time.
 //
-// A code n becomes the bfloat16 128 + n by setting the exponent's bits over it; (128 + n) s - 136 s, one multiply-add, is the value
+// The usual way to widen small whole numbers: a code n becomes the bfloat16 128 + n by setting the exponent's bits over it; (128 + n) s - 136 s, one multiply-add, is the value
 // (n - 8) s exactly: 136 s = 17 s 2^3 has 8 significant bits, and the value has 7.
 #pragma once
 #include "common.cuh"

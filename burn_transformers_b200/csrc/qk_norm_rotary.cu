@@ -3,7 +3,8 @@
 // Per token and head: y = x / sqrt(mean(x^2) + eps) * weight (one weight for all query heads, one for all key heads; without
 // weights x as it is), then pairs of the first `rot` channels, (i, i + rot / 2) or (2i, 2i + 1), turned by pos * f_i with cosine and
 // sine times `size`.  Sums and products are 32-bit, rounded once.  Angles: pos * f_i is formed in 64 bits and taken into one turn
-// there, so that far positions lose nothing (a 32-bit product is off by pos * f / 2^24: 0.06 at position 10^6).
+// there, so that far positions lose nothing by the product (in 32 bits it is off by pos * f / 2^24: 0.06 at position 10^6).  The frequencies
+// come as 32-bit numbers: where they were rounded to that, the angle of f itself is off by up to pos / 2^25, 0.03 there.
 //
 // Bound by memory: every channel is read and written once.  A warp takes one token and some of its heads.  Its lanes form the token's cosines
 // and sines once, in shared memory, and a lane keeps what its eight pairs are multiplied by in registers; it holds 16 channels of a head

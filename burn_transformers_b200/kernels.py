@@ -2153,8 +2153,8 @@ def _cache4_few(sms, units, pages, wide, head_dim):
     on its multiprocessor a page keeps a warp 0.61 + 0.03 n, and 0.68 for every four of them or part of four.  Calls with more blocks than run
     at once go by what a multiprocessor gets done, a page in 0.18, by what a block's beginning and end take of it (4.9 by itself, 1.55 beside one
     other, 0.95 beside two), and by 0.14 of the last block.  Heads of 64 channels take 0.53 of that a page, 16 columns 1.56.  Against
-    every choice timed at 48 sizes, 1 to 128 sequences of 100 to 32,766 tokens, what it chooses is 1.4 % slower than the best on average and 19 % at most
-    (with whole rounds of blocks instead, for calls of up to two: 9 % and 43 %)."""
+    every choice timed at 48 sizes, 1 to 128 sequences of 100 to 32,766 tokens, what it chooses is 1.9 % slower than the best on average and 23 % at most;
+    against those whose pieces run at once, which are all it looks at, 1.4 and 19 % (with whole rounds of blocks instead, for calls of up to two: 9 and 43 %)."""
     factor = (0.53 if head_dim == 64 else 1.0) * (1.56 if wide == 16 else 1.0)
     most = 12 if wide == 8 else 8
     best = (math.inf, 4, 1)
