@@ -31,7 +31,8 @@ def main(argv=None) -> int:
     parser.add_argument("max_new_tokens", nargs="?", type=int, default=32)
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     parser.add_argument("--cache-bits", type=int, choices=[4], default=None,
-                        help="4: softmax attention keeps keys and values in 4-bit codes (default: in --dtype)")
+                        help="4: softmax attention keeps keys and values in 4-bit codes, 0.27 of bfloat16's bytes, for long contexts and "
+                             "large batches: short ones take longer a step (default: in --dtype)")
     parser.add_argument("--strategy", choices=["greedy", "sample"], default=None)
     parser.add_argument("--temperature", type=float, default=None)
     parser.add_argument("--top-k", type=int, default=None)
