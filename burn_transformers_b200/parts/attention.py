@@ -35,7 +35,7 @@ class CausalSelfAttention(Mixer):
 
     `cache_bits` 4 (or `hold_cache_in(4)`): the cache holds keys and values in 4-bit codes (csrc/cache4.cuh).  Every query then attends over
     held values, the step's own too: a sequence's portions change nothing but roundings (of sums, and in bfloat16 of the softmax weights,
-    which are rounded relative to the largest score that a warp or piece has met: up to 2^-9 of each).  With a `window` the cache keeps what
+    which are rounded relative to the largest score that a warp or piece has met: up to 2^-8 of each).  With a `window` the cache keeps what
     the window needs, or every position where that takes no more than the window's ring in the model's type (cache/bank.py); positions below
     `keep_first` (of a cache in 4 bits only) stay visible beside the window, and the cache then keeps every position.
     """
