@@ -2264,7 +2264,8 @@ def cache4_attention(q, out, pool, table, table_len, seq_start, past_len, *, n_t
     0: all) or j < keep_first.  Rows of `out` behind the last sequence stay as they are.  Where the pages come round, what a query
     sees must still be held: `table_len` * 64 >= window + max_new - 1 and keep_first 0.  `scratch`: 32-bit, cache4_attention_scratch_floats
     of the same sizes (more does no harm), on a 16-byte boundary; two calls that may run at the same time need one each.  `impl` "any" asks for the kernel that
-    takes every case.  A page outside the pool is reported by `check_status`, as is a kernel that gave up waiting."""
+    takes every case.  A page outside the pool and a past that no sequence has (which counts as none) are reported by `check_status`, as is a
+    kernel that gave up waiting.  A `max_ctx` of `max_new` says that no sequence has a past: the kernels then start in another order."""
     code = _element_code(q, "q")
     _cache4_sizes(n_tokens, n_seqs, max_new, max_ctx, n_heads, n_kv_heads, window, keep_first)
     device = torch.cuda.current_device()

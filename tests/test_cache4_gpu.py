@@ -457,3 +457,13 @@ def test_the_kernel_for_every_case_when_it_is_asked_for(heads, kv, dim, pasts, n
     q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
     got = attend(step, q, pool, heads, kv, dim, window, keep, dim ** -0.5, impl="any")
     compare(step, got, q, keys, values, heads, kv, dim, window, keep, dim ** -0.5)
+
+
+@pytest.mark.parametrize("heads, kv, dim", [(1, 1, 128), (2, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("past, new, window, keep", [(967, 56, 415, 0), (3013, 12, 467, 0), (5000, 25, 334, 1), (2000, 17, 512, 70)])
+def test_few_rows_behind_a_window(heads, kv, dim, past, new, window, keep):
+    step, rng = Step([past], [new]), np.random.default_rng(new)
+    pool, keys, values = filled(step, kv, dim, rng)
+    q = torch.tensor(rng.standard_normal((step.n, heads * dim))).bfloat16().to(DEV)
+    got = attend(step, q, pool, heads, kv, dim, window, keep, dim ** -0.5)
+    compare(step, got, q, keys, values, heads, kv, dim, window, keep, dim ** -0.5)
